@@ -219,6 +219,73 @@ int tp_amd_nll_loss_backward(const tp_amd_tensor* grad_output, const tp_amd_tens
                              int64_t ignore_index, const tp_amd_tensor* total_weight,
                              tp_amd_tensor* result);
 
+/* ---- the attention layer (no reference counterpart) ---------------------- */
+
+/* qk_norm_rope: the norm of every head's query and key and the rotation by
+ * its token's position, in one pass.  query [tokens..., Hq, D] and key
+ * [tokens..., Hk, D] of one float dtype share their token axes; views of a
+ * packed projection are read in place.  Per head row x: r = 1 /
+ * sqrt(mean(x^2) + eps), n = x r weight (query_weight / key_weight [D] of
+ * the operands' dtype, NULL for 1), and with c, s the cosines and sines in
+ * row ``position`` of ``table`` (float32 [P, R], R even and at most D: R / 2
+ * cosines, then R / 2 sines) pair j of n becomes (a c - b s, b c + a s).
+ * Pair j is elements (j, j + R / 2), or (2 j, 2 j + 1) when ``interleaved``;
+ * elements from R on keep n.  ``positions`` int32 / int64 broadcast to the
+ * token axes; one outside [0, P) reads nothing and gives rows of NaN.
+ * Results query_out, key_out (dense, the operands' dtype) and float32
+ * query_rstd [tokens..., Hq], key_rstd [tokens..., Hk].  float32 arithmetic,
+ * rounded once.  Declined for heads wider than 1024, other dtypes, or
+ * operands on different devices. */
+int tp_amd_qk_norm_rope(const tp_amd_tensor* query, const tp_amd_tensor* key, const tp_amd_tensor* table,
+                        const tp_amd_tensor* positions, const tp_amd_tensor* query_weight,
+                        const tp_amd_tensor* key_weight, double eps, int interleaved, tp_amd_tensor* query_out,
+                        tp_amd_tensor* key_out, tp_amd_tensor* query_rstd, tp_amd_tensor* key_rstd);
+/* qk_norm_rope_backward: the gradients of query, key and both weights from
+ * those of the results, with the forward's operands and statistics.
+ * output_mask (4 ints; NULL = all) selects them; a weight's gradient may be
+ * had for the weight NULL (1) too.  No token gives zero weight gradients.
+ * Sums in a fixed order. */
+int tp_amd_qk_norm_rope_backward(const tp_amd_tensor* grad_query, const tp_amd_tensor* grad_key,
+                                 const tp_amd_tensor* query, const tp_amd_tensor* key, const tp_amd_tensor* table,
+                                 const tp_amd_tensor* positions, const tp_amd_tensor* query_rstd,
+                                 const tp_amd_tensor* key_rstd, const tp_amd_tensor* query_weight,
+                                 const tp_amd_tensor* key_weight, int interleaved, const int* output_mask,
+                                 tp_amd_tensor* dquery, tp_amd_tensor* dkey, tp_amd_tensor* dquery_weight,
+                                 tp_amd_tensor* dkey_weight);
+
+/* sliding_window_attention: causal attention with a sliding window and a few
+ * first tokens that stay visible.  query [B, Tq, Hq, D], key and value
+ * [B, Tk, Hk, D] of one float dtype, Hq a multiple of Hk (query head h reads
+ * key head h / (Hq / Hk)), D at most 128 (wider heads are declined).  A cache
+ * is read in place; so is any view with a dense last axis, rows of whole
+ * 16-byte packets on 16-byte boundaries and strides under 16 MiB a token
+ * (others are copied).
+ *   lengths [B] (int32 / int64; NULL: Tk): keys sequence b holds, clamped to
+ *     0 .. Tk.  Keys past them are not read.
+ *   starts [B] (NULL: lengths[b] - Tq): the position of query 0 of sequence b.
+ * Query i stands at p = starts[b] + i and sees key j if j <= p and
+ * (j > p - window or j < sinks); window < 0 is none.  A query outside
+ * 0 <= p < lengths[b] is not read; it, and one that sees no key, gives a row of
+ * zeros and an lse of -inf.  Of the other keys a block of
+ * neighbouring queries reads those that some query of it sees, so a value that is not
+ * finite reaches queries of its block that do not see it, and no others.
+ * out [B, Tq, Hq, D] = softmax(scale q.k) v and float32 lse [B, Hq, Tq], the
+ * natural logarithm of each row's sum of exponentials; scale > 0.  Scores,
+ * statistics and sums are float32, probabilities are rounded to the
+ * operands' dtype. */
+int tp_amd_sliding_window_attention(const tp_amd_tensor* query, const tp_amd_tensor* key, const tp_amd_tensor* value,
+                                    int64_t window, int64_t sinks, double scale, const tp_amd_tensor* lengths,
+                                    const tp_amd_tensor* starts, tp_amd_tensor* out, tp_amd_tensor* lse);
+/* sliding_window_attention_backward: dquery, dkey and dvalue from the
+ * forward's operands and results.  Key heads' gradients sum over their query
+ * heads; rows of queries and keys outside their sequence get zeros.  Sums in
+ * a fixed order. */
+int tp_amd_sliding_window_attention_backward(const tp_amd_tensor* grad_out, const tp_amd_tensor* query, const tp_amd_tensor* key,
+                                             const tp_amd_tensor* value, const tp_amd_tensor* out, const tp_amd_tensor* lse,
+                                             int64_t window, int64_t sinks, double scale, const tp_amd_tensor* lengths,
+                                             const tp_amd_tensor* starts, tp_amd_tensor* dquery, tp_amd_tensor* dkey,
+                                             tp_amd_tensor* dvalue);
+
 /* ---- host-only helpers (Cnnl.cpp:107-205); no device work --------------- */
 
 /* binary_result_dtype (Cnnl.cpp:178-192) for two tensors' dtypes and

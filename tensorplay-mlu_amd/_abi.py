@@ -221,6 +221,11 @@ PROTOTYPES = {
     "tp_amd_embedding_dense_backward": (i32, [T, T, i64, i64, i32, T]),
     "tp_amd_nll_loss": (i32, [T, T, T, i64, i64, T, T]),
     "tp_amd_nll_loss_backward": (i32, [T, T, T, T, i64, i64, T, T]),
+    "tp_amd_qk_norm_rope": (i32, [T, T, T, T, T, T, f64, i32, T, T, T, T]),
+    "tp_amd_qk_norm_rope_backward": (i32, [T, T, T, T, T, T, T, T, T, T, i32, C.POINTER(C.c_int),
+                                           T, T, T, T]),
+    "tp_amd_sliding_window_attention": (i32, [T, T, T, i64, i64, f64, T, T, T, T]),
+    "tp_amd_sliding_window_attention_backward": (i32, [T, T, T, T, T, T, i64, i64, f64, T, T, T, T, T]),
     "tp_amd_binary_result_dtype": (i32, [i32, i32, i32, i32]),
     "tp_amd_broadcast_shape": (i32, [I64P, i32, I64P, i32, I64P, C.POINTER(C.c_int)]),
     "tp_amd_is_dense": (i32, [T]),

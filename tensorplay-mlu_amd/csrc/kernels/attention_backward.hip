@@ -1,0 +1,434 @@
+// Gradients of causal attention with a sliding window and first tokens that
+// stay visible.
+//
+// From the forward's l (the logarithm of a row's sum): P_ij = e^(s_ij - l_i),
+// D_i = sum_d do_i o_i, dS_ij = P_ij (do_i . v_j - D_i), and
+// dq_i = scale sum_j dS_ij k_j, dk_j = scale sum_i dS_ij q_i,
+// dv_j = sum_i P_ij do_i, a key head's gradients over all its query heads.
+//
+// Two kernels form P and dS again, each for the sums it owns, so that nothing
+// is added by atomics and the same call gives the same bits: one walks the keys
+// that 128 queries see (dq, and D for the other), one the queries that see 128
+// keys, all heads of the group in turn (dk, dv).  Together 14 flops a visible
+// pair and element where a single pass with atomics would need 10.  Keys that
+// stay visible to every later query have many more of them than the others:
+// their walks are cut into parts of about the others' length, and with few
+// blocks all walks are, the parts' float32 sums joined in order by a third
+// kernel.  P and dS are rounded to the operands' type for the matrix
+// instruction; sums are float32.
+
+#include <algorithm>
+
+#include "attention_tiles.h"
+#include "../allocator.h"
+#include "../common.h"
+#include "../runtime.h"
+
+namespace tp_amd {
+
+namespace attention {
+
+namespace {
+
+struct Backward {
+    Shape s;
+    TokenRows q, k, v, o, dout;
+    const float* lse;
+    float* delta;  // [batch][heads][queries]
+    void *dq, *dk, *dv;
+    float scale, scale2;  // scale2: times log2 e
+    int blocks;           // of 128 queries (dq) or keys (dk, dv) a head
+    // dk, dv: the first sink_blocks blocks of a head walk in sink_parts parts,
+    // the others in near_parts; parts of more than one leave float32 sums.
+    int sink_blocks, sink_parts, near_parts;
+    float* part;  // [head][part][2][128][dim]
+    int per_head() const { return sink_blocks * sink_parts + (blocks - sink_blocks) * near_parts; }
+};
+
+template <typename T>
+constexpr int kRows = sizeof(S_<T>) == 2 ? 64 : 32;  // of an LDS tile
+
+template <typename T, int DT>
+__global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 && DT == 4 ? 1 : 2) void attention_dq_kernel(Backward p) {
+    using S = S_<T>;
+    constexpr int BK = kRows<T>, NS = BK / 32;
+    using Keys = Tile<T, DT, BK, 4>;
+    __shared__ __attribute__((aligned(1024))) char k0s[Keys::kBytes];
+    __shared__ __attribute__((aligned(1024))) char v0s[Keys::kBytes];
+    __shared__ __attribute__((aligned(1024))) char k1s[Keys::kBytes];
+    __shared__ __attribute__((aligned(1024))) char v1s[Keys::kBytes];
+
+    const int id = xcd_run(blockIdx.x, gridDim.x);
+    const int g = id % p.s.group, rest = id / p.s.group;
+    const int qb = p.blocks - 1 - rest % p.blocks, bh = rest / p.blocks;
+    const int hk = bh % p.s.kv_heads, b = bh / p.s.kv_heads;
+    const int h = hk * p.s.group + g;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int lane = threadIdx.x % kWave, l32 = lane % 32, half = lane / 32;
+    const Sequence seq = sequence_of(p.s, b);
+
+    const int mine = qb * 128 + wave * 32 + l32;
+    const bool alive = mine >= seq.first && mine < seq.end;
+    const int row = seq.start + mine;
+    const int b0 = max(qb * 128, seq.first), b1 = min(qb * 128 + 128, seq.end) - 1;
+    const int w0 = seq.start + max(qb * 128 + wave * 32, seq.first);
+    const int w1 = seq.start + min(qb * 128 + wave * 32 + 32, seq.end) - 1;
+
+    f32x16 dq[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) dq[d] = zeros();
+    if (b0 <= b1) {
+        const int p0 = seq.start + b0, p1 = seq.start + b1;
+        const KeyTiles tiles(p.s.rule, p0, p1, BK);
+        const S* kh = static_cast<const S*>(p.k.data) + b * p.k.batch + hk * p.k.head;
+        const S* vh = static_cast<const S*>(p.v.data) + b * p.v.batch + hk * p.v.head;
+        auto keep = [&](int j) { return j <= p1 && (j >= tiles.low_key || j < p.s.rule.sinks); };
+        auto issue = [&](int i, char* kt, char* vt) {
+            const int r0 = tiles.at(i) * BK;
+            Keys::issue(kt, kh, p.k.token, r0, p.s.dim, wave, lane, keep);
+            Keys::issue(vt, vh, p.v.token, r0, p.s.dim, wave, lane, keep);
+        };
+        if (tiles.count > 0) issue(0, k0s, v0s);
+        uint4 qf[Keys::kSteps], df[Keys::kSteps];
+        float delta = 0.0f;
+        {
+            auto rows_of = [&](const TokenRows& t) {
+                const S* at = static_cast<const S*>(t.data) + b * t.batch + h * t.head + static_cast<int64_t>(qb * 128) * t.token;
+                return buffer_over(at, static_cast<uint32_t>((127 * t.token + p.s.dim) * sizeof(S)));
+            };
+            auto row_bytes = [&](const TokenRows& t) { return static_cast<uint32_t>((wave * 32 + l32) * t.token * sizeof(S)); };
+            const Rsrc rq = rows_of(p.q), rd = rows_of(p.dout), ro = rows_of(p.o);
+#pragma unroll
+            for (int s = 0; s < Keys::kSteps; ++s) {
+                qf[s] = load_fragment<T>(rq, alive, row_bytes(p.q), s, half, p.s.dim);
+                df[s] = load_fragment<T>(rd, alive, row_bytes(p.dout), s, half, p.s.dim);
+                const uint4 of = load_fragment<T>(ro, alive, row_bytes(p.o), s, half, p.s.dim);
+                float x[Packet<T>::N], y[Packet<T>::N];
+                unpack<T>(df[s], x);
+                unpack<T>(of, y);
+#pragma unroll
+                for (int j = 0; j < Packet<T>::N; ++j) delta = fmaf(x[j], y[j], delta);
+            }
+        }
+        delta = both_halves(delta, SumOf{});
+        const int64_t stat = (static_cast<int64_t>(b) * p.s.heads + h) * p.s.queries + mine;
+        float bias = 0.0f;
+        if (alive) {
+            bias = -p.lse[stat] * kLog2E;
+            if (half == 0) p.delta[stat] = delta;
+        }
+        typename Keys::ByRows rows;
+        typename Keys::Transposed cols;
+        rows.init(lane);
+        cols.init(lane);
+        auto step = [&](int i, const char* kt, const char* vt, char* kn, char* vn) {
+            meet();
+            if (i + 1 < tiles.count) issue(i + 1, kn, vn);
+            const int j0 = tiles.at(i) * BK;
+            if (!p.s.rule.any_sees(w0, w1, j0, j0 + BK - 1)) return;
+            const bool whole = p.s.rule.all_see(w0, w1, j0, j0 + BK - 1);
+#pragma unroll
+            for (int u = 0; u < NS; ++u) {
+                f32x16 s = zeros(), ds = zeros();
+#pragma unroll
+                for (int f = 0; f < Keys::kSteps; ++f) {
+                    s = mma<T>(rows.read(kt, u, f), qf[f], s);
+                    ds = mma<T>(rows.read(vt, u, f), df[f], ds);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) ds[e] = __builtin_amdgcn_exp2f(fmaf(s[e], p.scale2, bias)) * (ds[e] - delta);
+                if (!whole) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        if (!p.s.rule.sees(row, j0 + 32 * u + row_of(e, half))) ds[e] = 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int f = 0; f < kFragsOf32<T>; ++f) {
+                    const uint4 sf = pack_rows<T>(ds, f);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) dq[d] = mma<T>(cols.read(kt, d, u, f), sf, dq[d]);
+                }
+            }
+        };
+        for (int i = 0; i < tiles.count; i += 2) {
+            step(i, k0s, v0s, k1s, v1s);
+            if (i + 1 >= tiles.count) break;
+            step(i + 1, k1s, v1s, k0s, v0s);
+        }
+    }
+    if (mine >= p.s.queries) return;
+    S* out = static_cast<S*>(p.dq) + ((static_cast<int64_t>(b) * p.s.queries + mine) * p.s.heads + h) * p.s.dim;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int at = 32 * d + row_of(e, half);
+            if (at >= p.s.dim) continue;
+            const auto value = [&](int j) { return alive ? dq[d][e + j] * p.scale : 0.0f; };
+            store4<T>(out + at, value(0), value(1), value(2), value(3));
+        }
+}
+
+template <typename T, int DT>
+__global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 ? 1 : 2) void attention_dkv_kernel(Backward p) {
+    using S = S_<T>;
+    constexpr int BQ = kRows<T>, NS = BQ / 32;
+    using Rows = Tile<T, DT, BQ, 4>;
+    __shared__ __attribute__((aligned(1024))) char q0s[Rows::kBytes];
+    __shared__ __attribute__((aligned(1024))) char d0s[Rows::kBytes];
+    __shared__ __attribute__((aligned(1024))) char q1s[Rows::kBytes];
+    __shared__ __attribute__((aligned(1024))) char d1s[Rows::kBytes];
+    // l and D of the tiles' rows (64 of each, whatever BQ)
+    __shared__ __attribute__((aligned(1024))) float l0s[2 * kWave];
+    __shared__ __attribute__((aligned(1024))) float l1s[2 * kWave];
+
+    const int id = xcd_run(blockIdx.x, gridDim.x);
+    const int per_head = p.sink_blocks * p.sink_parts + (p.blocks - p.sink_blocks) * p.near_parts;
+    const int bh = id / per_head, slot = id - bh * per_head;
+    const int hk = bh % p.s.kv_heads, b = bh / p.s.kv_heads;
+    const bool sink = slot < p.sink_blocks * p.sink_parts;
+    const int parts = sink ? p.sink_parts : p.near_parts;
+    const int local = sink ? slot : slot - p.sink_blocks * p.sink_parts;
+    const int kb = (sink ? 0 : p.sink_blocks) + local / parts, part = local % parts;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int lane = threadIdx.x % kWave, l32 = lane % 32, half = lane / 32;
+    const Sequence seq = sequence_of(p.s, b);
+
+    const int mine = kb * 128 + wave * 32 + l32;  // this lane's key
+    const int last = min(kb * 128 + 128, seq.length) - 1;
+    const int w0 = kb * 128 + wave * 32, w1 = min(w0 + 32, seq.length) - 1;
+    // queries that see a key of the block: from the block's first key on, to
+    // the window's end behind its last one or, of first tokens, to the end
+    const int64_t reach = kb * 128 < p.s.rule.sinks ? int64_t{kNoWindow} : int64_t{last} + p.s.rule.window - 1;
+    const int i0 = max(kb * 128 - seq.start, seq.first);
+    const int i1 = static_cast<int>(min(reach - seq.start, static_cast<int64_t>(seq.end) - 1));
+    const int t0 = i0 / BQ;
+    const int per_query_head = last >= kb * 128 && i0 <= i1 ? i1 / BQ - t0 + 1 : 0;
+    const int64_t all = static_cast<int64_t>(per_query_head) * p.s.group;
+    const int from = static_cast<int>(all * part / parts), to = static_cast<int>(all * (part + 1) / parts);
+
+    f32x16 dk[DT], dv[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d) dk[d] = dv[d] = zeros();
+    if (from < to) {
+        auto keep = [&](int i) { return i >= seq.first && i < seq.end; };
+        auto issue = [&](int it, char* qt, char* dt, float* lt) {
+            const int h = hk * p.s.group + it / per_query_head, r0 = (t0 + it % per_query_head) * BQ;
+            const S* qh = static_cast<const S*>(p.q.data) + b * p.q.batch + h * p.q.head;
+            const S* dh = static_cast<const S*>(p.dout.data) + b * p.dout.batch + h * p.dout.head;
+            Rows::issue(qt, qh, p.q.token, r0, p.s.dim, wave, lane, keep);
+            Rows::issue(dt, dh, p.dout.token, r0, p.s.dim, wave, lane, keep);
+            if (wave < 2) {
+                const float* at = (wave == 0 ? p.lse : p.delta) + (static_cast<int64_t>(b) * p.s.heads + h) * p.s.queries + r0;
+                const Rsrc res = buffer_over(at, BQ * sizeof(float));
+                const uint32_t off = lane < BQ && keep(r0 + lane) ? lane * sizeof(float) : kOutOfRange;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(res, (LdsPtr)(lt + wave * kWave), 4, off, 0, 0, 0);
+            }
+        };
+        issue(from, q0s, d0s, l0s);
+        uint4 kf[Rows::kSteps], vf[Rows::kSteps];
+        {
+            auto rows_of = [&](const TokenRows& t) {
+                const S* at = static_cast<const S*>(t.data) + b * t.batch + hk * t.head + static_cast<int64_t>(kb * 128) * t.token;
+                return buffer_over(at, static_cast<uint32_t>((127 * t.token + p.s.dim) * sizeof(S)));
+            };
+            auto row_bytes = [&](const TokenRows& t) { return static_cast<uint32_t>((wave * 32 + l32) * t.token * sizeof(S)); };
+            const Rsrc rk = rows_of(p.k), rv = rows_of(p.v);
+#pragma unroll
+            for (int s = 0; s < Rows::kSteps; ++s) {
+                kf[s] = load_fragment<T>(rk, mine <= last, row_bytes(p.k), s, half, p.s.dim);
+                vf[s] = load_fragment<T>(rv, mine <= last, row_bytes(p.v), s, half, p.s.dim);
+            }
+        }
+        typename Rows::ByRows rows;
+        typename Rows::Transposed cols;
+        rows.init(lane);
+        cols.init(lane);
+        auto step = [&](int it, const char* qt, const char* dt, const float* lt, char* qn, char* dn, float* ln) {
+            meet();
+            if (it + 1 < to) issue(it + 1, qn, dn, ln);
+            const int r0 = (t0 + it % per_query_head) * BQ;
+            const int p0 = seq.start + max(r0, seq.first), p1 = seq.start + min(r0 + BQ, seq.end) - 1;
+            if (w0 > w1 || !p.s.rule.any_sees(p0, p1, w0, w1)) return;
+            const bool whole = p.s.rule.all_see(p0, p1, w0, w1) && w1 == w0 + 31;
+#pragma unroll
+            for (int u = 0; u < NS; ++u) {
+                f32x16 s = zeros(), ds = zeros();
+#pragma unroll
+                for (int f = 0; f < Rows::kSteps; ++f) {
+                    s = mma<T>(rows.read(qt, u, f), kf[f], s);
+                    ds = mma<T>(rows.read(dt, u, f), vf[f], ds);
+                }
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const int r = 32 * u + row_of(e, half);
+                    const float4 l = *reinterpret_cast<const float4*>(lt + r);
+                    const float4 d = *reinterpret_cast<const float4*>(lt + kWave + r);
+                    const float ls[4] = {l.x, l.y, l.z, l.w}, dd[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        s[e + j] = __builtin_amdgcn_exp2f(fmaf(s[e + j], p.scale2, -ls[j] * kLog2E));
+                        ds[e + j] = s[e + j] * (ds[e + j] - dd[j]);
+                    }
+                }
+                if (!whole) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        if (!p.s.rule.sees(seq.start + r0 + 32 * u + row_of(e, half), mine)) s[e] = ds[e] = 0.0f;
+                    }
+                }
+#pragma unroll
+                for (int f = 0; f < kFragsOf32<T>; ++f) {
+                    const uint4 pf = pack_rows<T>(s, f), sf = pack_rows<T>(ds, f);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) {
+                        dv[d] = mma<T>(cols.read(dt, d, u, f), pf, dv[d]);
+                        dk[d] = mma<T>(cols.read(qt, d, u, f), sf, dk[d]);
+                    }
+                }
+            }
+        };
+        for (int it = from; it < to; it += 2) {
+            step(it, q0s, d0s, l0s, q1s, d1s, l1s);
+            if (it + 1 >= to) break;
+            step(it + 1, q1s, d1s, l1s, q0s, d0s, l0s);
+        }
+    }
+    if (mine >= p.s.keys) return;
+    if (parts > 1) {
+        float* sums = p.part + ((static_cast<int64_t>(bh) * per_head + slot) * 2 * 128 + wave * 32 + l32) * p.s.dim;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int at = 32 * d + row_of(e, half);
+                if (at >= p.s.dim) continue;
+                store4<float>(sums + at, dk[d][e], dk[d][e + 1], dk[d][e + 2], dk[d][e + 3]);
+                store4<float>(sums + 128 * p.s.dim + at, dv[d][e], dv[d][e + 1], dv[d][e + 2], dv[d][e + 3]);
+            }
+        return;
+    }
+    const int64_t at_row = ((static_cast<int64_t>(b) * p.s.keys + mine) * p.s.kv_heads + hk) * p.s.dim;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int at = 32 * d + row_of(e, half);
+            if (at >= p.s.dim) continue;
+            store4<T>(static_cast<S*>(p.dk) + at_row + at, dk[d][e] * p.scale, dk[d][e + 1] * p.scale, dk[d][e + 2] * p.scale,
+                      dk[d][e + 3] * p.scale);
+            store4<T>(static_cast<S*>(p.dv) + at_row + at, dv[d][e], dv[d][e + 1], dv[d][e + 2], dv[d][e + 3]);
+        }
+}
+
+// The parts of a block's sums in order, four elements a thread: blockIdx.x
+// over a block's rows, y over the blocks of a head that were cut (from
+// `first` on), z over batch x key heads.
+constexpr int kJoin = 256;
+
+template <typename T>
+__global__ __launch_bounds__(kJoin) void attention_join_kernel(Backward p, int first) {
+    const int per_head = p.sink_blocks * p.sink_parts + (p.blocks - p.sink_blocks) * p.near_parts;
+    const int kb = first + blockIdx.y, bh = blockIdx.z;
+    const int hk = bh % p.s.kv_heads, b = bh / p.s.kv_heads;
+    const bool sink = kb < p.sink_blocks;
+    const int parts = sink ? p.sink_parts : p.near_parts;
+    const int slot = sink ? kb * p.sink_parts : p.sink_blocks * p.sink_parts + (kb - p.sink_blocks) * p.near_parts;
+    const int quads = p.s.dim / 4, at = blockIdx.x * kJoin + threadIdx.x;
+    const int which = at / (128 * quads), row = at / quads % 128, d = at % quads * 4;
+    if (which > 1 || kb * 128 + row >= p.s.keys) return;
+    const float* from = p.part + (((static_cast<int64_t>(bh) * per_head + slot) * 2 + which) * 128 + row) * p.s.dim + d;
+    float4 t = *reinterpret_cast<const float4*>(from);
+#pragma unroll 4
+    for (int i = 1; i < parts; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(from + static_cast<int64_t>(i) * 2 * 128 * p.s.dim);
+        t.x += x.x;
+        t.y += x.y;
+        t.z += x.z;
+        t.w += x.w;
+    }
+    const float f = which == 0 ? p.scale : 1.0f;
+    S_<T>* out = static_cast<S_<T>*>(which == 0 ? p.dk : p.dv) +
+                 ((static_cast<int64_t>(b) * p.s.keys + kb * 128 + row) * p.s.kv_heads + hk) * p.s.dim + d;
+    store4<T>(out, t.x * f, t.y * f, t.z * f, t.w * f);
+}
+
+template <typename T, int DT>
+void backward_tiles(const AttentionArgs& a, int device) {
+    constexpr int BQ = kRows<T>;
+    Backward p;
+    p.s = shape_of(a);
+    p.q = a.q;
+    p.k = a.k;
+    p.v = a.v;
+    p.o = a.o;
+    p.dout = a.dout;
+    p.lse = a.lse;
+    p.dq = a.dq;
+    p.dk = a.dk;
+    p.dv = a.dv;
+    p.scale = a.scale;
+    p.scale2 = a.scale * kLog2E;
+    const int64_t heads = static_cast<int64_t>(a.batch) * a.kv_heads;
+    const Workspace delta(static_cast<size_t>(a.batch) * a.heads * std::max(a.queries, 1) * sizeof(float), device);
+    p.delta = static_cast<float*>(delta.get());
+    const hipStream_t on = stream(device);
+    if (a.queries > 0) {
+        p.blocks = (a.queries + 127) / 128;
+        const int64_t items = static_cast<int64_t>(a.batch) * a.heads * p.blocks;
+        TP_AMD_CHECK(items < (int64_t{1} << 31), "sliding_window_attention_backward: too many rows");
+        attention_dq_kernel<T, DT><<<static_cast<unsigned>(items), 4 * kWave, 0, on>>>(p);
+        TP_AMD_HIP_CHECK(hipGetLastError());
+    }
+    if (a.keys == 0) return;
+    p.blocks = (a.keys + 127) / 128;
+    // Tiles a walk has at most: of one near block, of one that stays visible.
+    const int64_t group = p.s.group, tiles = (a.queries + BQ - 1) / BQ;
+    const int64_t near = group * std::min<int64_t>(tiles, (128 + int64_t{p.s.rule.window} + BQ - 2) / BQ + 1), sink = group * tiles;
+    p.sink_blocks = std::min(p.blocks, (p.s.rule.sinks + 127) / 128);
+    const int64_t want = 2 * cu_count(device);  // blocks that fill the device once
+    const int64_t near_blocks = heads * (p.blocks - p.sink_blocks);
+    p.near_parts = near_blocks == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min(want / near_blocks, near / 4)));
+    const int64_t piece = std::max<int64_t>(4, near_blocks == 0 ? sink * heads * p.sink_blocks / want : near / p.near_parts);
+    p.sink_parts = p.sink_blocks == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, (sink + piece - 1) / piece));
+    const int64_t items = heads * p.per_head();
+    TP_AMD_CHECK(items < (int64_t{1} << 31), "sliding_window_attention_backward: too many keys");
+    const bool cut = p.near_parts > 1 || p.sink_parts > 1;
+    const Workspace part(cut ? static_cast<size_t>(items) * 2 * 128 * a.dim * sizeof(float) : 0, device);
+    p.part = static_cast<float*>(part.get());
+    attention_dkv_kernel<T, DT><<<static_cast<unsigned>(items), 4 * kWave, 0, on>>>(p);
+    TP_AMD_HIP_CHECK(hipGetLastError());
+    if (!cut) return;
+    const int first = p.sink_parts > 1 ? 0 : p.sink_blocks, end = p.near_parts > 1 ? p.blocks : p.sink_blocks;
+    const unsigned wide = static_cast<unsigned>((2 * 128 * (a.dim / 4) + kJoin - 1) / kJoin);
+    TP_AMD_CHECK(heads < 65536 && end - first < 65536, "sliding_window_attention_backward: too many heads to join");
+    attention_join_kernel<T><<<dim3(wide, static_cast<unsigned>(end - first), static_cast<unsigned>(heads)), kJoin, 0, on>>>(p, first);
+    TP_AMD_HIP_CHECK(hipGetLastError());
+}
+
+template <typename T>
+void backward_typed(const AttentionArgs& a, int device) {
+    switch ((a.dim + 31) / 32) {
+        case 1: return backward_tiles<T, 1>(a, device);
+        case 2: return backward_tiles<T, 2>(a, device);
+        case 3: return backward_tiles<T, 3>(a, device);
+        default: return backward_tiles<T, 4>(a, device);
+    }
+}
+
+}  // namespace
+
+}  // namespace attention
+
+void launch_attention_backward(int dtype, const AttentionArgs& a, int device) {
+    const OnDevice scope(device);
+    switch (dtype) {
+        case TP_AMD_FLOAT32: attention::backward_typed<float>(a, scope.index()); break;
+        case TP_AMD_FLOAT16: attention::backward_typed<f16_t>(a, scope.index()); break;
+        case TP_AMD_BFLOAT16: attention::backward_typed<bf16_t>(a, scope.index()); break;
+        default: TP_AMD_CHECK(false, "unsupported dtype ", dtype_name(dtype));
+    }
+}
+
+}  // namespace tp_amd

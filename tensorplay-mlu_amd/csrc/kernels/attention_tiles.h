@@ -1,0 +1,331 @@
+// Device-side pieces the attention kernels share: which keys a row sees, the
+// matrix instruction on 16-byte fragments, and LDS tiles of keys, values or
+// queries that are read both by rows and transposed.
+//
+// All kernels form scores with the keys (or queries) of an LDS tile as rows
+// and a wave's own 32 queries (or keys) as columns.  A 32 x 32 accumulator
+// gives a lane column lane % 32 and rows 8 g + 4 (lane / 32) + r in element
+// 4 g + r: exactly the rows a fragment of the next product's right operand
+// needs in that lane, if the left operand takes its rows in the same order.
+// So probabilities go from one product to the next in the registers they were
+// formed in, and a column's maximum and sum are a lane's own, but for one
+// exchange between the two halves of the wave.
+#pragma once
+
+#include "attention.h"
+#include "device_common.h"
+
+namespace tp_amd {
+namespace attention {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __attribute__((address_space(3))) void* LdsPtr;
+
+template <typename T>
+using S_ = typename Elem<T>::storage;
+
+// Positions lie under it in magnitude, so differences of them fit an int.
+constexpr int kNoWindow = 1 << 30;
+
+// What a row sees: keys j <= p of which j > p - window or j < sinks.
+struct Rule {
+    int window;  // kNoWindow: every earlier key
+    int sinks;
+    __device__ __forceinline__ bool sees(int p, int j) const { return j <= p && (j > p - window || j < sinks); }
+    // Every row of p0 .. p1 sees all of the keys k0 .. k1.
+    __device__ __forceinline__ bool all_see(int p0, int p1, int k0, int k1) const {
+        return k1 <= p0 && (k0 > p1 - window || k1 < sinks);
+    }
+    // Some row of p0 .. p1 sees some key of k0 .. k1.
+    __device__ __forceinline__ bool any_sees(int p0, int p1, int k0, int k1) const {
+        return p0 <= p1 && k0 <= p1 && (k1 > p0 - window || k0 < sinks);
+    }
+};
+
+// A sequence of the batch: query i stands at position start + i and is alive
+// when that lies in [0, length).
+struct Sequence {
+    int length, start;
+    int first, end;  // its alive queries
+};
+
+struct Shape {
+    int queries, keys, heads, kv_heads, group, dim;
+    Rule rule;
+    const void *lengths, *starts;
+    bool wide_lengths, wide_starts;
+    int64_t lengths_step, starts_step;
+};
+
+__device__ __forceinline__ int64_t read_index(const void* p, bool wide, int64_t at) {
+    return wide ? static_cast<const int64_t*>(p)[at] : static_cast<const int32_t*>(p)[at];
+}
+
+// Lengths past the keys count as all keys, negative ones as none; a start
+// that leaves no query alive is held to one that fits 32 bits and does too.
+__device__ __forceinline__ Sequence sequence_of(const Shape& s, int b) {
+    Sequence q;
+    int64_t length = s.keys;
+    if (s.lengths != nullptr) {
+        length = read_index(s.lengths, s.wide_lengths, b * s.lengths_step);
+        length = length < 0 ? 0 : length > s.keys ? s.keys : length;
+    }
+    int64_t start = length - s.queries;
+    if (s.starts != nullptr) {
+        start = read_index(s.starts, s.wide_starts, b * s.starts_step);
+        start = start < -s.queries ? -s.queries : start > s.keys ? s.keys : start;
+    }
+    q.length = __builtin_amdgcn_readfirstlane(static_cast<int>(length));
+    q.start = __builtin_amdgcn_readfirstlane(static_cast<int>(start));
+    q.first = q.start < 0 ? -q.start : 0;
+    q.end = q.length - q.start < s.queries ? q.length - q.start : s.queries;
+    return q;
+}
+
+// The key tiles of BK that rows p0 .. p1 (alive, p0 <= p1) see: `sinks` tiles
+// from key 0 on, then `count - sinks` from tile `low` on.
+struct KeyTiles {
+    int sinks, low, count;
+    int low_key;  // the window's first key
+    __device__ __forceinline__ KeyTiles(const Rule& r, int p0, int p1, int bk) {
+        low_key = p0 - r.window + 1 > 0 ? p0 - r.window + 1 : 0;
+        low = low_key / bk;
+        const int s = r.sinks < p1 + 1 ? r.sinks : p1 + 1;
+        sinks = (s + bk - 1) / bk;
+        if (sinks > low) sinks = low;
+        const int near = p1 / bk - low + 1;
+        count = sinks + (near > 0 ? near : 0);
+    }
+    __device__ __forceinline__ int at(int i) const { return i < sinks ? i : low + i - sinks; }
+};
+
+// ---- matrix instruction ---------------------------------------------------------
+
+// C += A B on fragments of 16 bytes a lane: 16 steps of the inner axis for
+// 16-bit types, 8 for float32 (lane half h holds 4 h .. 4 h + 3 of them).
+template <typename T>
+__device__ __forceinline__ f32x16 mma(const uint4& a, const uint4& b, f32x16 c) {
+    if constexpr (std::is_same_v<T, float>) {
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.x), __uint_as_float(b.x), c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.y), __uint_as_float(b.y), c, 0, 0, 0);
+        c = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.z), __uint_as_float(b.z), c, 0, 0, 0);
+        return __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a.w), __uint_as_float(b.w), c, 0, 0, 0);
+    } else if constexpr (std::is_same_v<T, bf16_t>) {
+        typedef __bf16 V __attribute__((ext_vector_type(8)));
+        V x, y;
+        __builtin_memcpy(&x, &a, 16);
+        __builtin_memcpy(&y, &b, 16);
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, c, 0, 0, 0);
+    } else {
+        typedef _Float16 V __attribute__((ext_vector_type(8)));
+        V x, y;
+        __builtin_memcpy(&x, &a, 16);
+        __builtin_memcpy(&y, &b, 16);
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(x, y, c, 0, 0, 0);
+    }
+}
+
+// Row that element e of a 32 x 32 accumulator holds.
+__device__ __forceinline__ int row_of(int e, int half) { return 8 * (e / 4) + 4 * half + e % 4; }
+
+__device__ __forceinline__ f32x16 zeros() {
+    f32x16 z;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) z[e] = 0.0f;
+    return z;
+}
+
+// Fragments in which one 32 x 32 accumulator's rows feed the next product.
+template <typename T>
+constexpr int kFragsOf32 = sizeof(S_<T>) == 4 ? 4 : 2;
+
+// Fragment f of them, rounded to T (float32: as it is).
+template <typename T>
+__device__ __forceinline__ uint4 pack_rows(const f32x16& s, int f) {
+    constexpr int N = Packet<T>::N;
+    float v[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = s[N * f + j];
+    return pack<T>(v);
+}
+
+// op over the two lanes of a column (the halves of the wave), in both.
+template <typename Op>
+__device__ __forceinline__ float both_halves(float v, Op op) {
+    const uint32_t u = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);  // {low, low}, {high, high}
+    return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+struct MaxOf {
+    __device__ __forceinline__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct SumOf {
+    __device__ __forceinline__ float operator()(float a, float b) const { return a + b; }
+};
+
+// ---- LDS tiles ---------------------------------------------------------------------
+
+// R token rows of DT x 32 elements, filled by W waves with loads straight
+// into LDS (16 bytes a lane).  Rows are padded to a power of two bytes, and the
+// 16-byte chunk c of row r lies at slot c ^ swizzle(r): 16 rows at one chunk
+// (a fragment read by rows) take 16 different sixteenths of LDS's 256 bytes a
+// clock, and 4 consecutive rows at 64 bytes (half a transposed read) its four
+// quarters.
+template <typename T, int DT, int R, int W>
+struct Tile {
+    using S = S_<T>;
+    static constexpr int E = sizeof(S);
+    static constexpr int kUsed = DT * 32 * E;
+    static constexpr int kRow = kUsed <= 64 ? 64 : kUsed <= 128 ? 128 : kUsed <= 256 ? 256 : 512;
+    static constexpr int kChunks = kRow / 16;
+    static constexpr int kBytes = R * kRow;
+    static constexpr int kPerLoad = 1024 / kRow;  // rows a load instruction fills
+    static constexpr int kIssue = kBytes / 1024 / W;
+    static constexpr int kSteps = kUsed / 32;  // fragments along a row
+    static_assert(kIssue * 1024 * W == kBytes, "the waves share a tile's loads evenly");
+
+    static __device__ __forceinline__ int swizzle(int r) {
+        if constexpr (kRow == 64) return (r >> 2) & 3;
+        else if constexpr (kRow == 128) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+        else return ((r & 3) << 2) | ((r >> 2) & 3);
+    }
+
+    // Loads of rows r0 .. r0 + R - 1 (token rows `step` elements apart from
+    // `head` on) into `tile`; of them row r is read if keep(r), else zeros.
+    template <typename Keep>
+    static __device__ __forceinline__ void issue(char* tile, const S* head, int64_t step, int r0, int dim, int wave, int lane,
+                                                 Keep&& keep) {
+        const Rsrc res = buffer_over(head + r0 * step, static_cast<uint32_t>(((R - 1) * step + dim) * E));
+        const uint32_t step_bytes = static_cast<uint32_t>(step * E);
+#pragma unroll
+        for (int i = 0; i < kIssue; ++i) {
+            const int row = (i * W + wave) * kPerLoad + lane / kChunks;
+            const int chunk = (lane % kChunks) ^ swizzle(row);
+            const bool in = keep(r0 + row) && chunk * 16 < dim * E;
+            const uint32_t at = in ? row * step_bytes + chunk * 16 : kOutOfRange;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(res, (LdsPtr)(tile + (i * W + wave) * 1024), 16, at, 0, 0, 0);
+        }
+    }
+
+    // A lane's offsets for reading 32 rows (lane % 32) at fragment s of them.
+    struct ByRows {
+        int off[kSteps];
+        __device__ __forceinline__ void init(int lane) {
+            const int l32 = lane % 32, half = lane / 32;
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) off[s] = l32 * kRow + (((2 * s + half) ^ swizzle(l32)) << 4);
+        }
+        // rows 32 u ..
+        __device__ __forceinline__ uint4 read(const char* tile, int u, int s) const {
+            return *reinterpret_cast<const uint4*>(tile + 32 * u * kRow + off[s]);
+        }
+    };
+
+    // Transposed: 32 columns (32 t + lane % 32) by fragment f of rows 32 u ..
+    // in the order pack_rows has them.
+    struct Transposed {
+        int lo[DT];
+        __device__ __forceinline__ void init(int lane) {
+            const int l32 = lane % 32, half = lane / 32;
+#pragma unroll
+            for (int t = 0; t < DT; ++t) {
+                if constexpr (E == 2) {
+                    // lane p of a 16-lane group addresses row p / 4 of four
+                    // and 8 bytes of it; it gets column p of the four rows
+                    const int p = lane % 16, row = 4 * half + p / 4, col = 32 * t + (lane & 16) + 4 * (p % 4);
+                    lo[t] = row * kRow + (((col / 8) ^ swizzle(row)) << 4) + (col % 8) * 2;
+                } else {
+                    const int row = 4 * half, col = 32 * t + l32;
+                    lo[t] = row * kRow + (((col / 4) ^ swizzle(row)) << 4) + (col % 4) * 4;
+                }
+            }
+        }
+        __device__ __forceinline__ uint4 read(const char* tile, int t, int u, int f) const {
+            uint4 v;
+            if constexpr (E == 2) {
+                typedef short short4_t __attribute__((ext_vector_type(4)));
+                typedef __attribute__((address_space(3))) short4_t* Ptr;
+                const char* q = tile + (32 * u + 16 * f) * kRow;
+                // eight rows on, bit 1 of the swizzle turns
+                const short4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(q + lo[t]));
+                const short4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(q + 8 * kRow + (lo[t] ^ 32)));
+                __builtin_memcpy(&v, &a, 8);
+                __builtin_memcpy(reinterpret_cast<char*>(&v) + 8, &b, 8);
+            } else {
+                // row 8 f + 4 half + j: bits 0 and 1 turn chunk bits 2 and 3
+                // (wide rows) or bit 1 turns chunk bit 2, bit 3 chunk bit 1
+                const char* q = tile + (32 * u + 8 * f) * kRow;
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int turn = (swizzle(8 * f + j) ^ swizzle(0)) << 4;
+                    w[j] = *reinterpret_cast<const uint32_t*>(q + j * kRow + (lo[t] ^ turn));
+                }
+                v = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            return v;
+        }
+    };
+};
+
+// 16 bytes a lane of a wave's own 32 rows, straight from memory: fragment s of
+// row `row` (zeros when not `in`).
+template <typename T>
+__device__ __forceinline__ uint4 load_fragment(Rsrc res, bool in, uint32_t row_bytes, int s, int half, int dim) {
+    constexpr int E = sizeof(S_<T>);
+    const uint32_t at = (2 * s + half) * 16;
+    return buffer_load16_cached(res, in && at < static_cast<uint32_t>(dim * E) ? row_bytes + at : kOutOfRange);
+}
+
+// Four consecutive elements of a dense row.
+template <typename T>
+__device__ __forceinline__ void store4(S_<T>* at, float a, float b, float c, float d) {
+    const S_<T> v[4] = {Elem<T>::store(a), Elem<T>::store(b), Elem<T>::store(c), Elem<T>::store(d)};
+    if constexpr (sizeof(v) == 8) *reinterpret_cast<uint2*>(at) = __builtin_bit_cast(uint2, v);
+    else *reinterpret_cast<uint4*>(at) = __builtin_bit_cast(uint4, v);
+}
+
+// Waits until this wave's loads have landed and its LDS reads are done, then
+// meets the block's other waves.  (Not __syncthreads(): the compiler would
+// place the wait where it likes among the loads into LDS.)
+__device__ __forceinline__ void meet() {
+    __builtin_amdgcn_s_waitcnt(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// Work item `id` of `total` for block `bid`: each XCD (blocks are dealt over
+// the 8 in turn) takes a run of neighbouring items, which share keys and
+// values in its L2.
+__device__ __forceinline__ int xcd_run(int bid, int total) {
+    const int xcd = bid % 8, q = total / 8, rest = total % 8;
+    return xcd * q + (xcd < rest ? xcd : rest) + bid / 8;
+}
+
+constexpr float kLog2E = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+inline Shape shape_of(const AttentionArgs& a) {
+    Shape s;
+    s.queries = a.queries;
+    s.keys = a.keys;
+    s.heads = a.heads;
+    s.kv_heads = a.kv_heads;
+    s.group = a.heads / a.kv_heads;
+    s.dim = a.dim;
+    // a window that reaches every key is none
+    s.rule.window = a.window < 0 || a.window >= static_cast<int64_t>(a.keys) + a.queries ? kNoWindow : static_cast<int>(a.window);
+    s.rule.sinks = s.rule.window == kNoWindow ? 0 : static_cast<int>(a.sinks < a.keys ? a.sinks : a.keys);
+    s.lengths = a.lengths;
+    s.starts = a.starts;
+    s.wide_lengths = a.wide_lengths;
+    s.wide_starts = a.wide_starts;
+    s.lengths_step = a.lengths_step;
+    s.starts_step = a.starts_step;
+    return s;
+}
+
+}  // namespace attention
+}  // namespace tp_amd

@@ -422,6 +422,58 @@ def nll_loss_backward(grad_output, self, target, weight, reduction, ignore_index
                         _ref(weight), int(reduction), int(ignore_index), _ref(total_weight))
 
 
+# ---- the attention layer (no registration of the reference's) -------------------
+
+
+def qk_norm_rope(query, key, table, positions, query_weight=None, key_weight=None, eps=1e-6,
+                 interleaved=False):
+    """(query_out, key_out, query_rstd, key_rstd): each head's row of query
+    [tokens..., Hq, D] and key [tokens..., Hk, D] normed (root mean square,
+    times its weight [D]) and the first R elements rotated by the token's
+    position; ``table`` float32 [P, R] holds R / 2 cosines, then R / 2 sines
+    of each position."""
+    return _call_results(L().tp_amd_qk_norm_rope, _ref(query), _ref(key), _ref(table),
+                         _ref(positions), _ref(query_weight), _ref(key_weight), float(eps),
+                         int(bool(interleaved)), count=4)
+
+
+def qk_norm_rope_backward(grad_query, grad_key, query, key, table, positions, query_rstd, key_rstd,
+                          query_weight=None, key_weight=None, interleaved=False,
+                          output_mask=(True, True, True, True)):
+    """(dquery, dkey, dquery_weight, dkey_weight), None where output_mask is
+    False."""
+    mask = (C.c_int * 4)(*[int(bool(m)) for m in output_mask])
+    return _call_results(L().tp_amd_qk_norm_rope_backward, _ref(grad_query), _ref(grad_key),
+                         _ref(query), _ref(key), _ref(table), _ref(positions), _ref(query_rstd),
+                         _ref(key_rstd), _ref(query_weight), _ref(key_weight),
+                         int(bool(interleaved)), mask, count=4)
+
+
+def _attention_scale(query, scale):
+    return float(scale) if scale is not None else max(query.shape[-1], 1) ** -0.5
+
+
+def sliding_window_attention(query, key, value, window=-1, sinks=0, scale=None, lengths=None,
+                             starts=None):
+    """(out, lse): causal attention of query [B, Tq, Hq, D] over key and value
+    [B, Tk, Hk, D].  The query at position p sees key j if j <= p and
+    (j > p - window or j < sinks); window < 0 is none.  ``lengths`` [B]: the
+    keys each sequence holds (None: Tk); ``starts`` [B]: the position of its
+    first query (None: the queries are its last tokens).  lse [B, Hq, Tq] is
+    float32, -inf for a query that sees nothing, whose row of out is zeros."""
+    return _call_results(L().tp_amd_sliding_window_attention, _ref(query), _ref(key), _ref(value),
+                         int(window), int(sinks), _attention_scale(query, scale), _ref(lengths),
+                         _ref(starts), count=2)
+
+
+def sliding_window_attention_backward(grad_out, query, key, value, out, lse, window=-1, sinks=0,
+                                      scale=None, lengths=None, starts=None):
+    """(dquery, dkey, dvalue) from the forward's operands and results."""
+    return _call_results(L().tp_amd_sliding_window_attention_backward, _ref(grad_out), _ref(query),
+                         _ref(key), _ref(value), _ref(out), _ref(lse), int(window), int(sinks),
+                         _attention_scale(query, scale), _ref(lengths), _ref(starts), count=3)
+
+
 #: The 72 operator names of the reference's registrations (64 on the hot
 #: path, 8 neural-network layers) and the function here that serves each.
 REGISTRATIONS = {
