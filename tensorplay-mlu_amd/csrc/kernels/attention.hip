@@ -27,6 +27,12 @@ namespace attention {
 namespace {
 
 constexpr float kSlack = 8.0f;
+#include <cstdlib>
+static int64_t envi(const char* n, int64_t d) { const char* e = getenv(n); return e ? atoll(e) : d; }
+#define SPLIT_ROUNDS envi("SPLIT_ROUNDS", 8)
+#define SPLIT_LONG envi("SPLIT_LONG", 32)
+#define SPLIT_ROWS envi("SPLIT_ROWS", 64)
+#define SPLIT_NT envi("SPLIT_NT", 128)
 
 struct Forward {
     Shape s;
@@ -78,6 +84,38 @@ struct Columns {
     }
 };
 
+// A lane's share of query `mine` of head h: out and l from the sums on bound m.
+template <typename T, int DT>
+__device__ __forceinline__ void finish_row(const Forward& p, int b, int h, int mine, int half, bool alive, float m, float t,
+                                           const Columns<DT>& col) {
+    const bool any = alive && t != 0.0f;
+    const float inv = any ? 1.0f / t : 0.0f;
+    if (half == 0) {
+        p.lse[(static_cast<int64_t>(b) * p.s.heads + h) * p.s.queries + mine] = any ? fmaf(m, kLn2, logf(t)) : -INFINITY;
+    }
+    S_<T>* out = static_cast<S_<T>*>(p.out) + ((static_cast<int64_t>(b) * p.s.queries + mine) * p.s.heads + h) * p.s.dim;
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int at = 32 * d + row_of(e, half);
+            if (at >= p.s.dim) continue;
+            const auto value = [&](int j) { return any ? col.o[d][e + j] * inv : 0.0f; };
+            store4<T>(out + at, value(0), value(1), value(2), value(3));
+        }
+}
+
+// Four elements of query i of head h, and l with the first.
+template <typename T>
+__device__ __forceinline__ void finish4(const Forward& p, int64_t b, int i, int h, int at, float m, float t, const float (&o)[4]) {
+    const bool any = t != 0.0f;
+    const float inv = any ? 1.0f / t : 0.0f;
+    if (at == 0) p.lse[(b * p.s.heads + h) * p.s.queries + i] = any ? fmaf(m, kLn2, logf(t)) : -INFINITY;
+    S_<T>* out = static_cast<S_<T>*>(p.out) + ((b * p.s.queries + i) * p.s.heads + h) * p.s.dim + at;
+    const auto value = [&](int j) { return any ? o[j] * inv : 0.0f; };
+    store4<T>(out, value(0), value(1), value(2), value(3));
+}
+
 template <typename T, int DT, int BK>
 __global__ __launch_bounds__(4 * kWave, 2) void attention_kernel(Forward p) {
     using S = S_<T>;
@@ -114,11 +152,15 @@ __global__ __launch_bounds__(4 * kWave, 2) void attention_kernel(Forward p) {
         const KeyTiles tiles(p.s.rule, p0, p1, BK);
         const S* kh = static_cast<const S*>(p.k.data) + b * p.k.batch + hk * p.k.head;
         const S* vh = static_cast<const S*>(p.v.data) + b * p.v.batch + hk * p.v.head;
-        auto keep = [&](int j) { return j <= p1 && (j >= tiles.low_key || j < p.s.rule.sinks); };
+        const KeysSeen keep(p.s.rule, tiles, p1);
+        typename Keys::Loads k_loads, v_loads;
+        k_loads.init(kh, p.k.token, p.s.dim, wave, lane);
+        v_loads.init(vh, p.v.token, p.s.dim, wave, lane);
         auto issue = [&](int i, char* kt, char* vt) {
             const int r0 = tiles.at(i) * BK;
-            Keys::issue(kt, kh, p.k.token, r0, p.s.dim, wave, lane, keep);
-            Keys::issue(vt, vh, p.v.token, r0, p.s.dim, wave, lane, keep);
+            const bool whole = keep.all(r0, r0 + BK - 1);
+            k_loads.issue(kt, r0, wave, whole, keep);
+            v_loads.issue(vt, r0, wave, whole, keep);
         };
         if (tiles.count > 0) issue(0, k0s, v0s);
         uint4 qf[Keys::kSteps];
@@ -171,27 +213,263 @@ __global__ __launch_bounds__(4 * kWave, 2) void attention_kernel(Forward p) {
         }
     }
     if (mine >= p.s.queries) return;
-    const float total = both_halves(col.t, SumOf{});
-    const bool any = alive && total != 0.0f;
-    const float inv = any ? 1.0f / total : 0.0f;
-    if (half == 0) {
-        p.lse[(static_cast<int64_t>(b) * p.s.heads + h) * p.s.queries + mine] = any ? fmaf(col.m, kLn2, logf(total)) : -INFINITY;
-    }
-    S* out = static_cast<S*>(p.out) + ((static_cast<int64_t>(b) * p.s.queries + mine) * p.s.heads + h) * p.s.dim;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int at = 32 * d + row_of(e, half);
-            if (at >= p.s.dim) continue;
-            const auto value = [&](int j) { return any ? col.o[d][e + j] * inv : 0.0f; };
-            store4<T>(out + at, value(0), value(1), value(2), value(3));
-        }
+    finish_row<T, DT>(p, b, h, mine, half, alive, col.m, both_halves(col.t, SumOf{}), col);
 }
 
+// ---- few queries over many keys -------------------------------------------------
+
+struct Split {
+    Forward f;
+    int rows, row_tiles;  // packed rows (queries x group) of a key head, tiles of 32 of them
+    int tile_rows;        // rows of a tile, but for a key head's last one: fewer
+    int splits;
+    FastDiv by_splits, by_row_tiles, by_kv_heads, by_group, by_workers;
+    // of item i (batch x key head x row tile): m and t, and the sums
+    float* stat;  // [items][splits][tile_rows][2]
+    float* part;  // [items][splits][tile_rows][dim]
+};
+
+// One arrival counter for each item that is split, on a 128-byte line of its
+// own (atomics on one line serialize); zero between launches.  A device's
+// launches are all on one stream.
+constexpr int kCounterStride = 32, kMaxSplitItems = 4096;
+__device__ unsigned int split_counters[kMaxSplitItems * kCounterStride];
+
+// Two floats written through to, and read from, the level all XCDs share.
+// Relaxed agent-scope stores are acknowledged there before s_waitcnt vmcnt(0)
+// returns, so they precede the arrival that is counted after it.
+__device__ __forceinline__ void store_shared(float* at, float a, float b) {
+    const uint64_t v = static_cast<uint64_t>(__float_as_uint(b)) << 32 | __float_as_uint(a);
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(at), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_shared(const float* at) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(at), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
+}
+
+// A state (bound m, sum t, four outputs x) added to one on bound `top`.
+__device__ __forceinline__ void add_state(float m, float t, const float4& x, float top, float& total, float (&o)[4]) {
+    if (m == -INFINITY) return;  // it met no key
+    const float turn = __builtin_amdgcn_exp2f(m - top);
+    total = fmaf(t, turn, total);
+    o[0] = fmaf(x.x, turn, o[0]);
+    o[1] = fmaf(x.y, turn, o[1]);
+    o[2] = fmaf(x.z, turn, o[2]);
+    o[3] = fmaf(x.w, turn, o[3]);
+}
+
+// Waves a block: what their private tiles (keys and values, two stages) leave
+// room for in LDS.
 template <typename T, int DT>
-void forward_tiles(const AttentionArgs& a, int device) {
-    constexpr int BK = sizeof(S_<T>) == 2 ? 64 : 32;
+constexpr int kSplitWaves = Tile<T, DT, 32, 1>::kRow == 512 ? 2 : 4;
+
+// A block owns 32 packed rows of a key head -- all query heads of the group
+// and all queries together, so the cache is read once -- and one split of the
+// keys they see.  Bound by the cache's bytes: every wave walks a run of 32-key
+// tiles of its own, loaded straight into its own part of LDS with the next
+// tile's loads always in flight, and meets the others only at the end.  The
+// item's last block to arrive adds the splits up, in their order: a second
+// launch for it cost 3.9 us where the walk itself takes 7.
+template <typename T, int DT, int AUX>
+__global__ __launch_bounds__((kSplitWaves<T, DT> * kWave), 1) void attention_split_kernel(Split q) {
+    using S = S_<T>;
+    using Keys = Tile<T, DT, 32, 1, AUX>;
+    constexpr int W = kSplitWaves<T, DT>;
+    __shared__ __attribute__((aligned(1024))) char k0s[W * Keys::kBytes];
+    __shared__ __attribute__((aligned(1024))) char v0s[W * Keys::kBytes];
+    __shared__ __attribute__((aligned(1024))) char k1s[W * Keys::kBytes];
+    __shared__ __attribute__((aligned(1024))) char v1s[W * Keys::kBytes];
+    __shared__ float ms[W][32], ts[W][32];
+    __shared__ int last;
+    const Forward& p = q.f;
+
+    // items: batch, key head, row tile, split
+    const uint32_t id = xcd_run(blockIdx.x, gridDim.x);
+    const uint32_t tile = fastdiv(id, q.by_splits), split = id - tile * q.splits;
+    const uint32_t bh = fastdiv(tile, q.by_row_tiles), rt = tile - bh * q.row_tiles;
+    const uint32_t b = fastdiv(bh, q.by_kv_heads), hk = bh - b * p.s.kv_heads;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int lane = threadIdx.x % kWave, l32 = lane % 32, half = lane / 32;
+
+    const int packed = rt * 32 + l32;
+    const int mine = fastdiv(packed, q.by_group), h = hk * p.s.group + packed - mine * p.s.group;
+    // The queries, on their way while the sequence's length is.
+    uint4 qf[Keys::kSteps];
+    {
+        const S* from_row = static_cast<const S*>(p.q.data) + b * p.q.batch + mine * p.q.token + h * p.q.head;
+#pragma unroll
+        for (int s = 0; s < Keys::kSteps; ++s) {
+            const int e = (2 * s + half) * Packet<T>::N;
+            qf[s] = packed < q.rows && e < p.s.dim ? *reinterpret_cast<const uint4*>(from_row + e) : make_uint4(0, 0, 0, 0);
+        }
+    }
+    const Sequence seq = sequence_of(p.s, b);
+    const bool alive = packed < q.rows && mine >= seq.first && mine < seq.end;
+    const int row = seq.start + mine;
+    const int packed_end = min(static_cast<int>(rt) * 32 + 32, q.rows);
+    const int b0 = max(static_cast<int>(fastdiv(rt * 32, q.by_group)), seq.first);
+    const int b1 = min(static_cast<int>(fastdiv(packed_end - 1, q.by_group)), seq.end - 1);
+
+    Columns<DT> col;
+    col.clear();
+    if (b0 <= b1) {
+        const int p0 = seq.start + b0, p1 = seq.start + b1;
+        const KeyTiles tiles(p.s.rule, p0, p1, 32);
+        const int run = fastdiv(tiles.count + q.splits * W - 1, q.by_workers);
+        const int from = min(static_cast<int>(split * W + wave) * run, tiles.count), to = min(from + run, tiles.count);
+        if (from < to) {
+            const S* kh = static_cast<const S*>(p.k.data) + b * p.k.batch + hk * p.k.head;
+            const S* vh = static_cast<const S*>(p.v.data) + b * p.v.batch + hk * p.v.head;
+            const KeysSeen keep(p.s.rule, tiles, p1);
+            const int at = wave * Keys::kBytes;
+            typename Keys::Loads k_loads, v_loads;
+            k_loads.init(kh, p.k.token, p.s.dim, 0, lane);
+            v_loads.init(vh, p.v.token, p.s.dim, 0, lane);
+            auto issue = [&](int i, char* kt, char* vt) {
+                const int r0 = tiles.at(i) * 32;
+                const bool whole = keep.all(r0, r0 + 31);
+                k_loads.issue(kt + at, r0, 0, whole, keep);
+                v_loads.issue(vt + at, r0, 0, whole, keep);
+            };
+            issue(from, k0s, v0s);
+#pragma unroll
+            for (int s = 0; s < Keys::kSteps; ++s) qf[s] = alive ? qf[s] : make_uint4(0, 0, 0, 0);
+            typename Keys::ByRows rows;
+            typename Keys::Transposed cols;
+            rows.init(lane);
+            cols.init(lane);
+            auto step = [&](int i, const char* kt, const char* vt, char* kn, char* vn) {
+                const bool more = i + 1 < to;
+                if (more) {
+                    reads_done();
+                    issue(i + 1, kn, vn);
+                    wait_but<3 * Keys::kIssue>();  // this tile's keys are there
+                } else {
+                    wait_but<Keys::kIssue>();
+                }
+                const int j0 = tiles.at(i) * 32;
+                f32x16 s[1] = {zeros()};
+#pragma unroll
+                for (int f = 0; f < Keys::kSteps; ++f) s[0] = mma<T>(rows.read(kt + at, 0, f), qf[f], s[0]);
+                if (!p.s.rule.all_see(p0, p1, j0, j0 + 31)) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        if (!p.s.rule.sees(row, j0 + row_of(e, half))) s[0][e] = -INFINITY;
+                    }
+                }
+                col.template absorb<1>(s, p.scale);
+                if (more) wait_but<2 * Keys::kIssue>();  // and its values
+                else wait_but<0>();
+#pragma unroll
+                for (int f = 0; f < kFragsOf32<T>; ++f) {
+                    const uint4 pf = pack_rows<T>(s[0], f);
+#pragma unroll
+                    for (int d = 0; d < DT; ++d) col.o[d] = mma<T>(cols.read(vt + at, d, 0, f), pf, col.o[d]);
+                }
+            };
+            for (int i = from; i < to; i += 2) {
+                step(i, k0s, v0s, k1s, v1s);
+                if (i + 1 >= to) break;
+                step(i + 1, k1s, v1s, k0s, v0s);
+            }
+        }
+    }
+    // The waves' sums in LDS, where their tiles were; then all threads add
+    // them up on one bound, a thread four elements of a row, wave 0's first.
+    const float t = both_halves(col.t, SumOf{});
+    if (half == 0) {
+        ms[wave][l32] = alive ? col.m : -INFINITY;
+        ts[wave][l32] = alive ? t : 0.0f;
+    }
+    // Rows of the sums: 32 lanes store at one column of 32 rows, so a row's
+    // 16-byte pieces are turned by its number (24 of them: padded instead).
+    constexpr int kLine = DT == 3 ? 100 : DT * 32, kSums = 32 * kLine;  // floats a row, a wave
+    static_assert(2 * W * Keys::kBytes >= W * kSums * 4, "half of the waves' sums fit where the keys, half where the values were");
+    auto piece = [](int r, int quad) { return r * kLine + 4 * (DT == 3 ? quad : quad ^ (r & (DT * 8 - 1))); };
+    auto sums_of = [&](int w) { return reinterpret_cast<float*>(w < W / 2 ? k0s : v0s) + w % (W / 2) * kSums; };
+    // a wave's tiles may still be read by no one but itself, but its sums lie
+    // where others' tiles were
+    __syncthreads();
+    if (packed < q.rows) {
+        float* const at = sums_of(wave);
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                store4<float>(at + piece(l32, (32 * d + row_of(e, half)) / 4), col.o[d][e], col.o[d][e + 1], col.o[d][e + 2],
+                              col.o[d][e + 3]);
+            }
+    }
+    __syncthreads();
+    const int quads = p.s.dim / 4, rows_here = packed_end - rt * 32;
+    float* const stat = q.stat + (static_cast<int64_t>(tile) * q.splits + split) * q.tile_rows * 2;
+    for (int at = threadIdx.x; at < rows_here * DT * 8; at += W * kWave) {
+        const int r = at / (DT * 8), quad = at % (DT * 8);
+        if (quad >= quads) continue;
+        float m = ms[0][r];
+#pragma unroll
+        for (int w = 1; w < W; ++w) m = fmaxf(m, ms[w][r]);
+        float total = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const float4 x = *reinterpret_cast<const float4*>(sums_of(w) + piece(r, quad));
+            add_state(ms[w][r], ts[w][r], x, m, total, o);
+        }
+        if (q.splits == 1) {
+            const int packed_r = rt * 32 + r, i = fastdiv(packed_r, q.by_group);
+            finish4<T>(p, b, i, hk * p.s.group + packed_r - i * p.s.group, 4 * quad, m, total, o);
+            continue;
+        }
+        if (quad == 0) store_shared(stat + 2 * r, m, total);
+        float* part = q.part + ((static_cast<int64_t>(tile) * q.splits + split) * q.tile_rows + r) * p.s.dim + 4 * quad;
+        store_shared(part, o[0], o[1]);
+        store_shared(part + 2, o[2], o[3]);
+    }
+    if (q.splits == 1) return;
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        unsigned int* counter = &split_counters[tile * kCounterStride];
+        last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == q.splits - 1u;
+        if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+    __syncthreads();
+    if (!last) return;
+    // All splits' m and t where the sums were.
+    float2* const stats = reinterpret_cast<float2*>(k0s);
+    const float* all = q.stat + static_cast<int64_t>(tile) * q.splits * q.tile_rows * 2;
+    for (int at = threadIdx.x; at < q.splits * q.tile_rows; at += W * kWave) stats[at] = load_shared(all + 2 * at);
+    __syncthreads();
+    for (int at = threadIdx.x; at < rows_here * DT * 8; at += W * kWave) {
+        const int r = at / (DT * 8), quad = at % (DT * 8);
+        if (quad >= quads) continue;
+        const int64_t step = static_cast<int64_t>(q.tile_rows) * p.s.dim;
+        const float* part = q.part + static_cast<int64_t>(tile) * q.splits * step + r * p.s.dim + 4 * quad;
+        float m = -INFINITY;
+        for (int s = 0; s < q.splits; ++s) m = fmaxf(m, stats[s * q.tile_rows + r].x);
+        float total = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        constexpr int kAhead = 8;  // splits whose loads go out together
+        for (int s0 = 0; s0 < q.splits; s0 += kAhead) {
+            float2 lo[kAhead], hi[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                const int s = s0 + k < q.splits ? s0 + k : q.splits - 1;
+                lo[k] = load_shared(part + s * step);
+                hi[k] = load_shared(part + s * step + 2);
+            }
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) {
+                if (s0 + k >= q.splits) break;
+                const float2 x = stats[(s0 + k) * q.tile_rows + r];
+                add_state(x.x, x.y, make_float4(lo[k].x, lo[k].y, hi[k].x, hi[k].y), m, total, o);
+            }
+        }
+        const int packed_r = rt * 32 + r, i = fastdiv(packed_r, q.by_group);
+        finish4<T>(p, b, i, hk * p.s.group + packed_r - i * p.s.group, 4 * quad, m, total, o);
+    }
+}
+
+Forward forward_of(const AttentionArgs& a) {
     Forward p;
     p.s = shape_of(a);
     p.q = a.q;
@@ -201,6 +479,55 @@ void forward_tiles(const AttentionArgs& a, int device) {
     p.lse = a.lse;
     p.scale = a.scale * kLog2E;
     p.blocks = (a.queries + 127) / 128;
+    return p;
+}
+
+template <typename T, int DT>
+void split_tiles(const AttentionArgs& a, int device) {
+    Split q;
+    q.f = forward_of(a);
+    const Rule& rule = q.f.s.rule;
+    q.rows = a.queries * q.f.s.group;
+    q.row_tiles = (q.rows + 31) / 32;
+    q.tile_rows = std::min(q.rows, 32);
+    // Tiles of 32 keys that a row tile sees at most (32 packed rows are at most
+    // 32 queries), and blocks that fill the device.
+    const int64_t near = std::min<int64_t>(a.keys, int64_t{rule.window} + 31) + 31, sinks = std::min(rule.sinks, a.keys) + 31;
+    const int64_t tiles = std::min<int64_t>((a.keys + 31) / 32, near / 32 + 1 + sinks / 32);
+    const int64_t items = static_cast<int64_t>(a.batch) * a.kv_heads * q.row_tiles;
+    constexpr int W = kSplitWaves<T, DT>;
+    const int64_t cus = cu_count(device), here = q.tile_rows;
+    const int64_t rounds = tiles * items >= SPLIT_LONG * W * cus ? SPLIT_ROUNDS : 1;
+    // The last block reads every split's sums back: no more splits than make
+    // that as long as a split's own walk; and their m and t fit in LDS.
+    const int64_t walk = tiles * 64 * sizeof(S_<T>), back = here * sizeof(float);
+    int64_t splits = std::min({rounds * cus / items, (tiles + W - 1) / W, int64_t(W) * Tile<T, DT, 32, 1>::kBytes / 8 / here});
+    while (splits > 1 && splits * splits * back > walk) --splits;
+    q.splits = items > kMaxSplitItems ? 1 : static_cast<int>(std::max<int64_t>(1, splits));
+    TP_AMD_CHECK(items * q.splits < (int64_t{1} << 30), "sliding_window_attention: too many rows");
+    q.by_splits = make_fastdiv(static_cast<uint32_t>(q.splits));
+    q.by_row_tiles = make_fastdiv(static_cast<uint32_t>(q.row_tiles));
+    q.by_kv_heads = make_fastdiv(static_cast<uint32_t>(a.kv_heads));
+    q.by_group = make_fastdiv(static_cast<uint32_t>(q.f.s.group));
+    q.by_workers = make_fastdiv(static_cast<uint32_t>(q.splits * W));
+    Workspace part;
+    if (q.splits > 1) {
+        const int64_t slots = items * q.splits * here;
+        part = Workspace(static_cast<size_t>(slots * (a.dim + 2)) * sizeof(float), device);
+        q.part = static_cast<float*>(part.get());
+        q.stat = q.part + slots * a.dim;
+    }
+    const int64_t bytes = 2 * int64_t{32} * tiles * a.batch * a.kv_heads * a.dim * sizeof(S_<T>);
+    auto* kernel = q.row_tiles == 1 && bytes > (SPLIT_NT << 20) ? attention_split_kernel<T, DT, kNt> : attention_split_kernel<T, DT, 0>;
+    kernel<<<static_cast<unsigned>(items * q.splits), W * kWave, 0, stream(device)>>>(q);
+    TP_AMD_HIP_CHECK(hipGetLastError());
+}
+
+template <typename T, int DT>
+void forward_tiles(const AttentionArgs& a, int device) {
+    constexpr int BK = sizeof(S_<T>) == 2 ? 64 : 32;
+    if (static_cast<int64_t>(a.queries) * (a.heads / a.kv_heads) <= SPLIT_ROWS) return split_tiles<T, DT>(a, device);
+    const Forward p = forward_of(a);
     const int64_t items = static_cast<int64_t>(a.batch) * a.heads * p.blocks;
     TP_AMD_CHECK(items < (int64_t{1} << 31), "sliding_window_attention: too many rows");
     attention_kernel<T, DT, BK><<<static_cast<unsigned>(items), 4 * kWave, 0, stream(device)>>>(p);

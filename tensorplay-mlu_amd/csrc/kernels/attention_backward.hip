@@ -82,11 +82,15 @@ __global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 && DT == 4 ? 1 : 2) v
         const KeyTiles tiles(p.s.rule, p0, p1, BK);
         const S* kh = static_cast<const S*>(p.k.data) + b * p.k.batch + hk * p.k.head;
         const S* vh = static_cast<const S*>(p.v.data) + b * p.v.batch + hk * p.v.head;
-        auto keep = [&](int j) { return j <= p1 && (j >= tiles.low_key || j < p.s.rule.sinks); };
+        const KeysSeen keep(p.s.rule, tiles, p1);
+        typename Keys::Loads k_loads, v_loads;
+        k_loads.init(kh, p.k.token, p.s.dim, wave, lane);
+        v_loads.init(vh, p.v.token, p.s.dim, wave, lane);
         auto issue = [&](int i, char* kt, char* vt) {
             const int r0 = tiles.at(i) * BK;
-            Keys::issue(kt, kh, p.k.token, r0, p.s.dim, wave, lane, keep);
-            Keys::issue(vt, vh, p.v.token, r0, p.s.dim, wave, lane, keep);
+            const bool whole = keep.all(r0, r0 + BK - 1);
+            k_loads.issue(kt, r0, wave, whole, keep);
+            v_loads.issue(vt, r0, wave, whole, keep);
         };
         if (tiles.count > 0) issue(0, k0s, v0s);
         uint4 qf[Keys::kSteps], df[Keys::kSteps];
@@ -213,12 +217,18 @@ __global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 ? 1 : 2) void attenti
     for (int d = 0; d < DT; ++d) dk[d] = dv[d] = zeros();
     if (from < to) {
         auto keep = [&](int i) { return i >= seq.first && i < seq.end; };
+        typename Rows::Loads q_loads, d_loads;
+        q_loads.init(static_cast<const S*>(p.q.data) + b * p.q.batch, p.q.token, p.s.dim, wave, lane);
+        d_loads.init(static_cast<const S*>(p.dout.data) + b * p.dout.batch, p.dout.token, p.s.dim, wave, lane);
+        const S* const q_all = q_loads.head;
+        const S* const d_all = d_loads.head;
         auto issue = [&](int it, char* qt, char* dt, float* lt) {
             const int h = hk * p.s.group + it / per_query_head, r0 = (t0 + it % per_query_head) * BQ;
-            const S* qh = static_cast<const S*>(p.q.data) + b * p.q.batch + h * p.q.head;
-            const S* dh = static_cast<const S*>(p.dout.data) + b * p.dout.batch + h * p.dout.head;
-            Rows::issue(qt, qh, p.q.token, r0, p.s.dim, wave, lane, keep);
-            Rows::issue(dt, dh, p.dout.token, r0, p.s.dim, wave, lane, keep);
+            q_loads.head = q_all + h * p.q.head;
+            d_loads.head = d_all + h * p.dout.head;
+            const bool whole = r0 >= seq.first && r0 + BQ <= seq.end;
+            q_loads.issue(qt, r0, wave, whole, keep);
+            d_loads.issue(dt, r0, wave, whole, keep);
             if (wave < 2) {
                 const float* at = (wave == 0 ? p.lse : p.delta) + (static_cast<int64_t>(b) * p.s.heads + h) * p.s.queries + r0;
                 const Rsrc res = buffer_over(at, BQ * sizeof(float));

@@ -99,6 +99,15 @@ struct KeyTiles {
     __device__ __forceinline__ int at(int i) const { return i < sinks ? i : low + i - sinks; }
 };
 
+// Keys that some row of a block sees, which are the ones it reads: up to the
+// last row's position, from the first row's window on or among the first.
+struct KeysSeen {
+    int last, low_key, sinks;
+    __device__ __forceinline__ KeysSeen(const Rule& r, const KeyTiles& t, int p1) : last(p1), low_key(t.low_key), sinks(r.sinks) {}
+    __device__ __forceinline__ bool operator()(int j) const { return j <= last && (j >= low_key || j < sinks); }
+    __device__ __forceinline__ bool all(int k0, int k1) const { return k1 <= last && (k0 >= low_key || k1 < sinks); }
+};
+
 // ---- matrix instruction ---------------------------------------------------------
 
 // C += A B on fragments of 16 bytes a lane: 16 steps of the inner axis for
@@ -167,12 +176,12 @@ struct SumOf {
 // ---- LDS tiles ---------------------------------------------------------------------
 
 // R token rows of DT x 32 elements, filled by W waves with loads straight
-// into LDS (16 bytes a lane).  Rows are padded to a power of two bytes, and the
+// into LDS (16 bytes a lane, cache policy AUX).  Rows are padded to a power of two bytes, and the
 // 16-byte chunk c of row r lies at slot c ^ swizzle(r): 16 rows at one chunk
 // (a fragment read by rows) take 16 different sixteenths of LDS's 256 bytes a
 // clock, and 4 consecutive rows at 64 bytes (half a transposed read) its four
 // quarters.
-template <typename T, int DT, int R, int W>
+template <typename T, int DT, int R, int W, int AUX = 0>
 struct Tile {
     using S = S_<T>;
     static constexpr int E = sizeof(S);
@@ -191,22 +200,47 @@ struct Tile {
         else return ((r & 3) << 2) | ((r >> 2) & 3);
     }
 
-    // Loads of rows r0 .. r0 + R - 1 (token rows `step` elements apart from
-    // `head` on) into `tile`; of them row r is read if keep(r), else zeros.
-    template <typename Keep>
-    static __device__ __forceinline__ void issue(char* tile, const S* head, int64_t step, int r0, int dim, int wave, int lane,
-                                                 Keep&& keep) {
-        const Rsrc res = buffer_over(head + r0 * step, static_cast<uint32_t>(((R - 1) * step + dim) * E));
-        const uint32_t step_bytes = static_cast<uint32_t>(step * E);
+    // A wave's loads of tiles of one tensor, whose token rows lie `step`
+    // elements apart from `head` on.
+    struct Loads {
+        // the swizzle repeats every 16 rows
+        static constexpr int kPeriod = kPerLoad * W >= 16 ? 1 : 16 / (kPerLoad * W);
+        const S* head;
+        int64_t step;
+        uint32_t records;       // bytes from a load's first row to its last one's end
+        uint32_t off[kPeriod];  // a lane's place in the rows of load i % kPeriod
+        int row;                // and its row in load 0
+
+        __device__ __forceinline__ void init(const S* first, int64_t step_, int dim, int wave, int lane) {
+            step = step_;
+            head = first + wave * kPerLoad * step;
+            records = static_cast<uint32_t>(((kPerLoad - 1) * step + dim) * E);
+            row = wave * kPerLoad + lane / kChunks;
 #pragma unroll
-        for (int i = 0; i < kIssue; ++i) {
-            const int row = (i * W + wave) * kPerLoad + lane / kChunks;
-            const int chunk = (lane % kChunks) ^ swizzle(row);
-            const bool in = keep(r0 + row) && chunk * 16 < dim * E;
-            const uint32_t at = in ? row * step_bytes + chunk * 16 : kOutOfRange;
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(res, (LdsPtr)(tile + (i * W + wave) * 1024), 16, at, 0, 0, 0);
+            for (int i = 0; i < kPeriod; ++i) {
+                const int chunk = (lane % kChunks) ^ swizzle(i * W * kPerLoad + row);
+                off[i] = chunk * 16 < dim * E ? static_cast<uint32_t>(lane / kChunks * step * E) + chunk * 16 : kOutOfRange;
+            }
         }
-    }
+
+        // Rows r0 .. r0 + R - 1 into `tile`: all of them if `whole`, else row r
+        // if keep(r), the others as zeros.
+        template <typename Keep>
+        __device__ __forceinline__ void issue(char* tile, int r0, int wave, bool whole, Keep&& keep) const {
+            const S* from = head + r0 * step;
+            auto load = [&](int i, uint32_t at) {
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer_over(from + i * W * kPerLoad * step, records),
+                                                         (LdsPtr)(tile + (i * W + wave) * 1024), 16, at, 0, 0, AUX);
+            };
+            if (whole) {
+#pragma unroll
+                for (int i = 0; i < kIssue; ++i) load(i, off[i % kPeriod]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kIssue; ++i) load(i, keep(r0 + row + i * W * kPerLoad) ? off[i % kPeriod] : kOutOfRange);
+            }
+        }
+    };
 
     // A lane's offsets for reading 32 rows (lane % 32) at fragment s of them.
     struct ByRows {
@@ -293,6 +327,19 @@ __device__ __forceinline__ void meet() {
     __builtin_amdgcn_s_waitcnt(0);
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// This wave's LDS reads are done: what they read may be filled again.
+__device__ __forceinline__ void reads_done() {
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+}
+
+// The same as meet() for one wave's own tile, its N latest loads left in flight.
+template <int N>
+__device__ __forceinline__ void wait_but() {
+    __builtin_amdgcn_s_waitcnt((N & 15) | (7 << 4) | ((N >> 4) << 14));  // vmcnt(N) lgkmcnt(0)
     asm volatile("" ::: "memory");
 }
 

@@ -140,11 +140,11 @@ class DeviceTensor:
 
     @property
     def shape(self) -> tuple[int, ...]:
-        return tuple(self._ref.sizes[i] for i in range(self._ref.ndim))
+        return tuple(self._ref.sizes[: self._ref.ndim])
 
     @property
     def strides(self) -> tuple[int, ...]:
-        return tuple(self._ref.strides[i] for i in range(self._ref.ndim))
+        return tuple(self._ref.strides[: self._ref.ndim])
 
     @property
     def dtype(self) -> int:
