@@ -27,12 +27,6 @@ namespace attention {
 namespace {
 
 constexpr float kSlack = 8.0f;
-#include <cstdlib>
-static int64_t envi(const char* n, int64_t d) { const char* e = getenv(n); return e ? atoll(e) : d; }
-#define SPLIT_ROUNDS envi("SPLIT_ROUNDS", 8)
-#define SPLIT_LONG envi("SPLIT_LONG", 32)
-#define SPLIT_ROWS envi("SPLIT_ROWS", 64)
-#define SPLIT_NT envi("SPLIT_NT", 128)
 
 struct Forward {
     Shape s;
@@ -41,6 +35,7 @@ struct Forward {
     float* lse;
     float scale;  // scale log2 e
     int blocks;   // of 128 queries a head
+    int pairs;    // batch x key heads
 };
 
 // The running state of a wave's 32 columns (queries).
@@ -116,34 +111,36 @@ __device__ __forceinline__ void finish4(const Forward& p, int64_t b, int i, int 
     store4<T>(out, value(0), value(1), value(2), value(3));
 }
 
-template <typename T, int DT, int BK>
-__global__ __launch_bounds__(4 * kWave, 2) void attention_kernel(Forward p) {
+template <typename T, int DT>
+__global__ __launch_bounds__(kWide* kWave, sizeof(S_<T>) == 4 && DT == 4 ? 1 : 2) void attention_kernel(Forward p) {
     using S = S_<T>;
-    using Keys = Tile<T, DT, BK, 4>;
-    constexpr int NS = BK / 32;
+    constexpr int BK = sizeof(S) == 2 ? 64 : 32, NS = BK / 32, RB = 32 * kWide;
+    using Keys = Tile<T, DT, BK, kWide>;
     __shared__ __attribute__((aligned(1024))) char k0s[Keys::kBytes];
     __shared__ __attribute__((aligned(1024))) char v0s[Keys::kBytes];
     __shared__ __attribute__((aligned(1024))) char k1s[Keys::kBytes];
     __shared__ __attribute__((aligned(1024))) char v1s[Keys::kBytes];
 
-    // items: batch, key head, blocks of queries from the last (which sees the
-    // most keys) to the first, query head of the group
-    const int id = xcd_run(blockIdx.x, gridDim.x);
-    const int g = id % p.s.group, rest = id / p.s.group;
-    const int qb = p.blocks - 1 - rest % p.blocks, bh = rest / p.blocks;
+    // Blocks of queries from the last, which sees the most keys, to the first,
+    // query heads of the group, then batch and key heads innermost: blocks are
+    // dealt over the 8 XCDs in turn, so with a multiple of 8 of those each XCD
+    // keeps its own keys and values in its L2, and the short walks come last,
+    // where they fill the gaps.
+    const int bh = blockIdx.x % p.pairs, rest = blockIdx.x / p.pairs;
+    const int g = rest % p.s.group, qb = p.blocks - 1 - rest / p.s.group;
     const int hk = bh % p.s.kv_heads, b = bh / p.s.kv_heads;
     const int h = hk * p.s.group + g;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave, l32 = lane % 32, half = lane / 32;
     const Sequence seq = sequence_of(p.s, b);
 
-    const int mine = qb * 128 + wave * 32 + l32;  // this lane's query
+    const int mine = qb * RB + wave * 32 + l32;  // this lane's query
     const bool alive = mine >= seq.first && mine < seq.end;
     const int row = seq.start + mine;
     // the alive rows of the block, and of the wave
-    const int b0 = max(qb * 128, seq.first), b1 = min(qb * 128 + 128, seq.end) - 1;
-    const int w0 = seq.start + max(qb * 128 + wave * 32, seq.first);
-    const int w1 = seq.start + min(qb * 128 + wave * 32 + 32, seq.end) - 1;
+    const int b0 = max(qb * RB, seq.first), b1 = min(qb * RB + RB, seq.end) - 1;
+    const int w0 = seq.start + max(qb * RB + wave * 32, seq.first);
+    const int w1 = seq.start + min(qb * RB + wave * 32 + 32, seq.end) - 1;
 
     Columns<DT> col;
     col.clear();
@@ -165,8 +162,8 @@ __global__ __launch_bounds__(4 * kWave, 2) void attention_kernel(Forward p) {
         if (tiles.count > 0) issue(0, k0s, v0s);
         uint4 qf[Keys::kSteps];
         {
-            const S* qh = static_cast<const S*>(p.q.data) + b * p.q.batch + h * p.q.head + static_cast<int64_t>(qb * 128) * p.q.token;
-            const Rsrc res = buffer_over(qh, static_cast<uint32_t>((127 * p.q.token + p.s.dim) * sizeof(S)));
+            const S* qh = static_cast<const S*>(p.q.data) + b * p.q.batch + h * p.q.head + static_cast<int64_t>(qb * RB) * p.q.token;
+            const Rsrc res = buffer_over(qh, static_cast<uint32_t>(((RB - 1) * p.q.token + p.s.dim) * sizeof(S)));
 #pragma unroll
             for (int s = 0; s < Keys::kSteps; ++s) {
                 qf[s] = load_fragment<T>(res, alive, static_cast<uint32_t>((wave * 32 + l32) * p.q.token * sizeof(S)), s, half, p.s.dim);
@@ -478,7 +475,8 @@ Forward forward_of(const AttentionArgs& a) {
     p.out = a.out;
     p.lse = a.lse;
     p.scale = a.scale * kLog2E;
-    p.blocks = (a.queries + 127) / 128;
+    TP_AMD_CHECK(static_cast<int64_t>(a.batch) * a.kv_heads < (int64_t{1} << 31), "sliding_window_attention: too many heads");
+    p.pairs = static_cast<int>(static_cast<int64_t>(a.batch) * a.kv_heads);
     return p;
 }
 
@@ -497,7 +495,11 @@ void split_tiles(const AttentionArgs& a, int device) {
     const int64_t items = static_cast<int64_t>(a.batch) * a.kv_heads * q.row_tiles;
     constexpr int W = kSplitWaves<T, DT>;
     const int64_t cus = cu_count(device), here = q.tile_rows;
-    const int64_t rounds = tiles * items >= SPLIT_LONG * W * cus ? SPLIT_ROUNDS : 1;
+    // Long walks (32 tiles and more a wave) in eight rounds of blocks, which
+    // evens out sequences of different lengths: 64 x 16384 keys 546 us against
+    // 570 in one; short ones in one, a block costs some 8 us besides its walk:
+    // 16 x 2000 keys 17 us against 23 in two.
+    const int64_t rounds = tiles * items >= 32 * W * cus ? 8 : 1;
     // The last block reads every split's sums back: no more splits than make
     // that as long as a split's own walk; and their m and t fit in LDS.
     const int64_t walk = tiles * 64 * sizeof(S_<T>), back = here * sizeof(float);
@@ -517,20 +519,37 @@ void split_tiles(const AttentionArgs& a, int device) {
         q.part = static_cast<float*>(part.get());
         q.stat = q.part + slots * a.dim;
     }
+    // A cache larger than the Infinity Cache is half full of, read once, passes
+    // by it: 64 x 16384 keys 558 us against 611; a small one comes from it
+    // again (16 x 2000 keys 20.1 us non-temporal, 19.4 so).
     const int64_t bytes = 2 * int64_t{32} * tiles * a.batch * a.kv_heads * a.dim * sizeof(S_<T>);
-    auto* kernel = q.row_tiles == 1 && bytes > (SPLIT_NT << 20) ? attention_split_kernel<T, DT, kNt> : attention_split_kernel<T, DT, 0>;
+    auto* kernel = q.row_tiles == 1 && bytes > (int64_t{128} << 20) ? attention_split_kernel<T, DT, kNt> : attention_split_kernel<T, DT, 0>;
     kernel<<<static_cast<unsigned>(items * q.splits), W * kWave, 0, stream(device)>>>(q);
     TP_AMD_HIP_CHECK(hipGetLastError());
 }
 
+// The split kernel also takes more packed rows than one tile of 32 where the
+// wide blocks are few and a round of its own blocks, one a CU, is enough
+// (float32, bound by its products: two rounds).  bf16, 32 heads of 128 on 8 key
+// heads over a window of 1024: 64 queries 15.9 us against 27.7 in wide blocks,
+// 256 (256 row tiles) 18.0 and 31.0, 512 33.4 and 31.3; float32, 12 heads of 64,
+// 1000 queries (384 row tiles) 26.3 and 37.1.  Up to 64 packed rows (two
+// tiles) it takes any batch: wide blocks would hold mostly padding.
+template <typename T>
+bool takes_split(const AttentionArgs& a, int device) {
+    const int64_t rows = static_cast<int64_t>(a.queries) * (a.heads / a.kv_heads), cus = cu_count(device);
+    const int64_t tiles = static_cast<int64_t>(a.batch) * a.kv_heads * ((rows + 31) / 32);
+    return rows <= 64 || tiles <= (sizeof(S_<T>) == 4 ? 2 : 1) * cus;
+}
+
 template <typename T, int DT>
 void forward_tiles(const AttentionArgs& a, int device) {
-    constexpr int BK = sizeof(S_<T>) == 2 ? 64 : 32;
-    if (static_cast<int64_t>(a.queries) * (a.heads / a.kv_heads) <= SPLIT_ROWS) return split_tiles<T, DT>(a, device);
-    const Forward p = forward_of(a);
-    const int64_t items = static_cast<int64_t>(a.batch) * a.heads * p.blocks;
+    if (takes_split<T>(a, device)) return split_tiles<T, DT>(a, device);
+    Forward p = forward_of(a);
+    p.blocks = (a.queries + 32 * kWide - 1) / (32 * kWide);
+    const int64_t items = static_cast<int64_t>(p.pairs) * p.s.group * p.blocks;
     TP_AMD_CHECK(items < (int64_t{1} << 31), "sliding_window_attention: too many rows");
-    attention_kernel<T, DT, BK><<<static_cast<unsigned>(items), 4 * kWave, 0, stream(device)>>>(p);
+    attention_kernel<T, DT><<<static_cast<unsigned>(items), kWide * kWave, 0, stream(device)>>>(p);
     TP_AMD_HIP_CHECK(hipGetLastError());
 }
 

@@ -34,45 +34,45 @@ struct Backward {
     Shape s;
     TokenRows q, k, v, o, dout;
     const float* lse;
-    float* delta;  // [batch][heads][queries]
+    // what the first kernel finds of every query for the second one: -l log2 e
+    // and D, [batch][heads][queries] each
+    float *bias, *delta;
     void *dq, *dk, *dv;
     float scale, scale2;  // scale2: times log2 e
-    int blocks;           // of 128 queries (dq) or keys (dk, dv) a head
+    int blocks;           // of 32 W queries (dq) or keys (dk, dv) a head
+    int pairs;            // batch x key heads
     // dk, dv: the first sink_blocks blocks of a head walk in sink_parts parts,
     // the others in near_parts; parts of more than one leave float32 sums.
     int sink_blocks, sink_parts, near_parts;
-    float* part;  // [head][part][2][128][dim]
+    float* part;  // [head][part][2][rows][dim]
     int per_head() const { return sink_blocks * sink_parts + (blocks - sink_blocks) * near_parts; }
 };
 
-template <typename T>
-constexpr int kRows = sizeof(S_<T>) == 2 ? 64 : 32;  // of an LDS tile
-
-template <typename T, int DT>
-__global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 && DT == 4 ? 1 : 2) void attention_dq_kernel(Backward p) {
+template <typename T, int DT, int BK, int W>
+__global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4) ? 1 : 2) void attention_dq_kernel(Backward p) {
     using S = S_<T>;
-    constexpr int BK = kRows<T>, NS = BK / 32;
-    using Keys = Tile<T, DT, BK, 4>;
+    constexpr int NS = BK / 32, RB = 32 * W;
+    using Keys = Tile<T, DT, BK, W>;
     __shared__ __attribute__((aligned(1024))) char k0s[Keys::kBytes];
     __shared__ __attribute__((aligned(1024))) char v0s[Keys::kBytes];
     __shared__ __attribute__((aligned(1024))) char k1s[Keys::kBytes];
     __shared__ __attribute__((aligned(1024))) char v1s[Keys::kBytes];
 
-    const int id = xcd_run(blockIdx.x, gridDim.x);
-    const int g = id % p.s.group, rest = id / p.s.group;
-    const int qb = p.blocks - 1 - rest % p.blocks, bh = rest / p.blocks;
+    // as in the forward: long walks first, batch and key heads innermost
+    const int bh = blockIdx.x % p.pairs, rest = blockIdx.x / p.pairs;
+    const int g = rest % p.s.group, qb = p.blocks - 1 - rest / p.s.group;
     const int hk = bh % p.s.kv_heads, b = bh / p.s.kv_heads;
     const int h = hk * p.s.group + g;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave, l32 = lane % 32, half = lane / 32;
     const Sequence seq = sequence_of(p.s, b);
 
-    const int mine = qb * 128 + wave * 32 + l32;
+    const int mine = qb * RB + wave * 32 + l32;
     const bool alive = mine >= seq.first && mine < seq.end;
     const int row = seq.start + mine;
-    const int b0 = max(qb * 128, seq.first), b1 = min(qb * 128 + 128, seq.end) - 1;
-    const int w0 = seq.start + max(qb * 128 + wave * 32, seq.first);
-    const int w1 = seq.start + min(qb * 128 + wave * 32 + 32, seq.end) - 1;
+    const int b0 = max(qb * RB, seq.first), b1 = min(qb * RB + RB, seq.end) - 1;
+    const int w0 = seq.start + max(qb * RB + wave * 32, seq.first);
+    const int w1 = seq.start + min(qb * RB + wave * 32 + 32, seq.end) - 1;
 
     f32x16 dq[DT];
 #pragma unroll
@@ -97,8 +97,8 @@ __global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 && DT == 4 ? 1 : 2) v
         float delta = 0.0f;
         {
             auto rows_of = [&](const TokenRows& t) {
-                const S* at = static_cast<const S*>(t.data) + b * t.batch + h * t.head + static_cast<int64_t>(qb * 128) * t.token;
-                return buffer_over(at, static_cast<uint32_t>((127 * t.token + p.s.dim) * sizeof(S)));
+                const S* at = static_cast<const S*>(t.data) + b * t.batch + h * t.head + static_cast<int64_t>(qb * RB) * t.token;
+                return buffer_over(at, static_cast<uint32_t>(((RB - 1) * t.token + p.s.dim) * sizeof(S)));
             };
             auto row_bytes = [&](const TokenRows& t) { return static_cast<uint32_t>((wave * 32 + l32) * t.token * sizeof(S)); };
             const Rsrc rq = rows_of(p.q), rd = rows_of(p.dout), ro = rows_of(p.o);
@@ -119,13 +119,15 @@ __global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 && DT == 4 ? 1 : 2) v
         float bias = 0.0f;
         if (alive) {
             bias = -p.lse[stat] * kLog2E;
-            if (half == 0) p.delta[stat] = delta;
         }
         typename Keys::ByRows rows;
         typename Keys::Transposed cols;
         rows.init(lane);
         cols.init(lane);
-        auto step = [&](int i, const char* kt, const char* vt, char* kn, char* vn) {
+        // `sums` false: only D, as the sum of P dP, into `exact`
+        float exact = 0.0f;
+        auto step = [&](auto sums_, int i, const char* kt, const char* vt, char* kn, char* vn) __attribute__((always_inline)) {
+            constexpr bool sums = decltype(sums_)::value;
             meet();
             if (i + 1 < tiles.count) issue(i + 1, kn, vn);
             const int j0 = tiles.at(i) * BK;
@@ -140,12 +142,17 @@ __global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 && DT == 4 ? 1 : 2) v
                     ds = mma<T>(rows.read(vt, u, f), df[f], ds);
                 }
 #pragma unroll
-                for (int e = 0; e < 16; ++e) ds[e] = __builtin_amdgcn_exp2f(fmaf(s[e], p.scale2, bias)) * (ds[e] - delta);
+                for (int e = 0; e < 16; ++e) ds[e] = __builtin_amdgcn_exp2f(fmaf(s[e], p.scale2, bias)) * (sums ? ds[e] - delta : ds[e]);
                 if (!whole) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         if (!p.s.rule.sees(row, j0 + 32 * u + row_of(e, half))) ds[e] = 0.0f;
                     }
+                }
+                if constexpr (!sums) {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) exact += ds[e];
+                    continue;
                 }
 #pragma unroll
                 for (int f = 0; f < kFragsOf32<T>; ++f) {
@@ -155,11 +162,27 @@ __global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 && DT == 4 ? 1 : 2) v
                 }
             }
         };
-        for (int i = 0; i < tiles.count; i += 2) {
-            step(i, k0s, v0s, k1s, v1s);
-            if (i + 1 >= tiles.count) break;
-            step(i + 1, k1s, v1s, k0s, v0s);
+        auto walk = [&](auto sums) __attribute__((always_inline)) {
+            for (int i = 0; i < tiles.count; i += 2) {
+                step(sums, i, k0s, v0s, k1s, v1s);
+                if (i + 1 >= tiles.count) break;
+                step(sums, i + 1, k1s, v1s, k0s, v0s);
+            }
+        };
+        // Rows of few keys have the largest gradients, and the rounding of
+        // their out in D is as large there as that of dS: their D is summed
+        // up from P and dP, in a walk of its own over at most 128 keys.
+        if (sizeof(S) == 2 && tiles.count * BK <= 128) {
+            walk(std::false_type{});
+            delta = both_halves(exact, SumOf{});
+            meet();
+            if (tiles.count > 0) issue(0, k0s, v0s);
         }
+        if (alive && half == 0) {
+            p.bias[stat] = bias;
+            p.delta[stat] = delta;
+        }
+        walk(std::true_type{});
     }
     if (mine >= p.s.queries) return;
     S* out = static_cast<S*>(p.dq) + ((static_cast<int64_t>(b) * p.s.queries + mine) * p.s.heads + h) * p.s.dim;
@@ -174,22 +197,21 @@ __global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 && DT == 4 ? 1 : 2) v
         }
 }
 
-template <typename T, int DT>
-__global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 ? 1 : 2) void attention_dkv_kernel(Backward p) {
+template <typename T, int DT, int BQ, int W>
+__global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) void attention_dkv_kernel(Backward p) {
     using S = S_<T>;
-    constexpr int BQ = kRows<T>, NS = BQ / 32;
-    using Rows = Tile<T, DT, BQ, 4>;
+    constexpr int NS = BQ / 32, RB = 32 * W;
+    using Rows = Tile<T, DT, BQ, W>;
     __shared__ __attribute__((aligned(1024))) char q0s[Rows::kBytes];
     __shared__ __attribute__((aligned(1024))) char d0s[Rows::kBytes];
     __shared__ __attribute__((aligned(1024))) char q1s[Rows::kBytes];
     __shared__ __attribute__((aligned(1024))) char d1s[Rows::kBytes];
-    // l and D of the tiles' rows (64 of each, whatever BQ)
+    // -l log2 e and D of the tiles' rows (64 of each, whatever BQ)
     __shared__ __attribute__((aligned(1024))) float l0s[2 * kWave];
     __shared__ __attribute__((aligned(1024))) float l1s[2 * kWave];
 
-    const int id = xcd_run(blockIdx.x, gridDim.x);
     const int per_head = p.sink_blocks * p.sink_parts + (p.blocks - p.sink_blocks) * p.near_parts;
-    const int bh = id / per_head, slot = id - bh * per_head;
+    const int bh = blockIdx.x % p.pairs, slot = blockIdx.x / p.pairs;
     const int hk = bh % p.s.kv_heads, b = bh / p.s.kv_heads;
     const bool sink = slot < p.sink_blocks * p.sink_parts;
     const int parts = sink ? p.sink_parts : p.near_parts;
@@ -199,16 +221,16 @@ __global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 ? 1 : 2) void attenti
     const int lane = threadIdx.x % kWave, l32 = lane % 32, half = lane / 32;
     const Sequence seq = sequence_of(p.s, b);
 
-    const int mine = kb * 128 + wave * 32 + l32;  // this lane's key
-    const int last = min(kb * 128 + 128, seq.length) - 1;
-    const int w0 = kb * 128 + wave * 32, w1 = min(w0 + 32, seq.length) - 1;
+    const int mine = kb * RB + wave * 32 + l32;  // this lane's key
+    const int last = min(kb * RB + RB, seq.length) - 1;
+    const int w0 = kb * RB + wave * 32, w1 = min(w0 + 32, seq.length) - 1;
     // queries that see a key of the block: from the block's first key on, to
     // the window's end behind its last one or, of first tokens, to the end
-    const int64_t reach = kb * 128 < p.s.rule.sinks ? int64_t{kNoWindow} : int64_t{last} + p.s.rule.window - 1;
-    const int i0 = max(kb * 128 - seq.start, seq.first);
+    const int64_t reach = kb * RB < p.s.rule.sinks ? int64_t{kNoWindow} : int64_t{last} + p.s.rule.window - 1;
+    const int i0 = max(kb * RB - seq.start, seq.first);
     const int i1 = static_cast<int>(min(reach - seq.start, static_cast<int64_t>(seq.end) - 1));
     const int t0 = i0 / BQ;
-    const int per_query_head = last >= kb * 128 && i0 <= i1 ? i1 / BQ - t0 + 1 : 0;
+    const int per_query_head = last >= kb * RB && i0 <= i1 ? i1 / BQ - t0 + 1 : 0;
     const int64_t all = static_cast<int64_t>(per_query_head) * p.s.group;
     const int from = static_cast<int>(all * part / parts), to = static_cast<int>(all * (part + 1) / parts);
 
@@ -222,26 +244,40 @@ __global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 ? 1 : 2) void attenti
         d_loads.init(static_cast<const S*>(p.dout.data) + b * p.dout.batch, p.dout.token, p.s.dim, wave, lane);
         const S* const q_all = q_loads.head;
         const S* const d_all = d_loads.head;
-        auto issue = [&](int it, char* qt, char* dt, float* lt) {
-            const int h = hk * p.s.group + it / per_query_head, r0 = (t0 + it % per_query_head) * BQ;
+        // the walk's next tile to load: query head and first row
+        int next_h = hk * p.s.group + from / per_query_head, next_row = (t0 + from % per_query_head) * BQ;
+        const int end_row = (t0 + per_query_head) * BQ;
+        auto issue = [&](char* qt, char* dt, float* lt) {
+            const int h = next_h, r0 = next_row;
+            next_row += BQ;
+            if (next_row == end_row) {
+                next_row = t0 * BQ;
+                ++next_h;
+            }
             q_loads.head = q_all + h * p.q.head;
             d_loads.head = d_all + h * p.dout.head;
             const bool whole = r0 >= seq.first && r0 + BQ <= seq.end;
             q_loads.issue(qt, r0, wave, whole, keep);
             d_loads.issue(dt, r0, wave, whole, keep);
-            if (wave < 2) {
-                const float* at = (wave == 0 ? p.lse : p.delta) + (static_cast<int64_t>(b) * p.s.heads + h) * p.s.queries + r0;
-                const Rsrc res = buffer_over(at, BQ * sizeof(float));
+            auto load_stat = [&](int w) {
+                const float* at = (w == 0 ? p.bias : p.delta) + (static_cast<int64_t>(b) * p.s.heads + h) * p.s.queries + r0;
                 const uint32_t off = lane < BQ && keep(r0 + lane) ? lane * sizeof(float) : kOutOfRange;
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(res, (LdsPtr)(lt + wave * kWave), 4, off, 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer_over(at, BQ * sizeof(float)), (LdsPtr)(lt + w * kWave), 4, off, 0, 0, 0);
+            };
+            if (W > 1) {
+                if (wave < 2) load_stat(wave);
+            } else {
+                load_stat(0);
+                load_stat(1);
             }
         };
-        issue(from, q0s, d0s, l0s);
+        int row0 = next_row;  // of the tile at hand
+        issue(q0s, d0s, l0s);
         uint4 kf[Rows::kSteps], vf[Rows::kSteps];
         {
             auto rows_of = [&](const TokenRows& t) {
-                const S* at = static_cast<const S*>(t.data) + b * t.batch + hk * t.head + static_cast<int64_t>(kb * 128) * t.token;
-                return buffer_over(at, static_cast<uint32_t>((127 * t.token + p.s.dim) * sizeof(S)));
+                const S* at = static_cast<const S*>(t.data) + b * t.batch + hk * t.head + static_cast<int64_t>(kb * RB) * t.token;
+                return buffer_over(at, static_cast<uint32_t>(((RB - 1) * t.token + p.s.dim) * sizeof(S)));
             };
             auto row_bytes = [&](const TokenRows& t) { return static_cast<uint32_t>((wave * 32 + l32) * t.token * sizeof(S)); };
             const Rsrc rk = rows_of(p.k), rv = rows_of(p.v);
@@ -255,10 +291,13 @@ __global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 ? 1 : 2) void attenti
         typename Rows::Transposed cols;
         rows.init(lane);
         cols.init(lane);
+        // how far this lane's key is seen; a first token to the end
+        const unsigned reach_of_mine = mine < p.s.rule.sinks ? kNoWindow : p.s.rule.window;
         auto step = [&](int it, const char* qt, const char* dt, const float* lt, char* qn, char* dn, float* ln) {
             meet();
-            if (it + 1 < to) issue(it + 1, qn, dn, ln);
-            const int r0 = (t0 + it % per_query_head) * BQ;
+            const int r0 = row0;
+            row0 = next_row;
+            if (it + 1 < to) issue(qn, dn, ln);
             const int p0 = seq.start + max(r0, seq.first), p1 = seq.start + min(r0 + BQ, seq.end) - 1;
             if (w0 > w1 || !p.s.rule.any_sees(p0, p1, w0, w1)) return;
             const bool whole = p.s.rule.all_see(p0, p1, w0, w1) && w1 == w0 + 31;
@@ -278,14 +317,16 @@ __global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 ? 1 : 2) void attenti
                     const float ls[4] = {l.x, l.y, l.z, l.w}, dd[4] = {d.x, d.y, d.z, d.w};
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        s[e + j] = __builtin_amdgcn_exp2f(fmaf(s[e + j], p.scale2, -ls[j] * kLog2E));
+                        s[e + j] = __builtin_amdgcn_exp2f(fmaf(s[e + j], p.scale2, ls[j]));
                         ds[e + j] = s[e + j] * (ds[e + j] - dd[j]);
                     }
                 }
                 if (!whole) {
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        if (!p.s.rule.sees(seq.start + r0 + 32 * u + row_of(e, half), mine)) s[e] = ds[e] = 0.0f;
+                        // (unsigned: rows before the key are out of reach too)
+                        const unsigned behind = seq.start + r0 + 32 * u + row_of(e, half) - mine;
+                        if (behind >= reach_of_mine) s[e] = ds[e] = 0.0f;
                     }
                 }
 #pragma unroll
@@ -307,7 +348,7 @@ __global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 ? 1 : 2) void attenti
     }
     if (mine >= p.s.keys) return;
     if (parts > 1) {
-        float* sums = p.part + ((static_cast<int64_t>(bh) * per_head + slot) * 2 * 128 + wave * 32 + l32) * p.s.dim;
+        float* sums = p.part + ((static_cast<int64_t>(bh) * per_head + slot) * 2 * RB + wave * 32 + l32) * p.s.dim;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -315,7 +356,7 @@ __global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 ? 1 : 2) void attenti
                 const int at = 32 * d + row_of(e, half);
                 if (at >= p.s.dim) continue;
                 store4<float>(sums + at, dk[d][e], dk[d][e + 1], dk[d][e + 2], dk[d][e + 3]);
-                store4<float>(sums + 128 * p.s.dim + at, dv[d][e], dv[d][e + 1], dv[d][e + 2], dv[d][e + 3]);
+                store4<float>(sums + RB * p.s.dim + at, dv[d][e], dv[d][e + 1], dv[d][e + 2], dv[d][e + 3]);
             }
         return;
     }
@@ -337,7 +378,7 @@ __global__ __launch_bounds__(4 * kWave, sizeof(S_<T>) == 4 ? 1 : 2) void attenti
 // `first` on), z over batch x key heads.
 constexpr int kJoin = 256;
 
-template <typename T>
+template <typename T, int RB>
 __global__ __launch_bounds__(kJoin) void attention_join_kernel(Backward p, int first) {
     const int per_head = p.sink_blocks * p.sink_parts + (p.blocks - p.sink_blocks) * p.near_parts;
     const int kb = first + blockIdx.y, bh = blockIdx.z;
@@ -346,13 +387,13 @@ __global__ __launch_bounds__(kJoin) void attention_join_kernel(Backward p, int f
     const int parts = sink ? p.sink_parts : p.near_parts;
     const int slot = sink ? kb * p.sink_parts : p.sink_blocks * p.sink_parts + (kb - p.sink_blocks) * p.near_parts;
     const int quads = p.s.dim / 4, at = blockIdx.x * kJoin + threadIdx.x;
-    const int which = at / (128 * quads), row = at / quads % 128, d = at % quads * 4;
-    if (which > 1 || kb * 128 + row >= p.s.keys) return;
-    const float* from = p.part + (((static_cast<int64_t>(bh) * per_head + slot) * 2 + which) * 128 + row) * p.s.dim + d;
+    const int which = at / (RB * quads), row = at / quads % RB, d = at % quads * 4;
+    if (which > 1 || kb * RB + row >= p.s.keys) return;
+    const float* from = p.part + (((static_cast<int64_t>(bh) * per_head + slot) * 2 + which) * RB + row) * p.s.dim + d;
     float4 t = *reinterpret_cast<const float4*>(from);
 #pragma unroll 4
     for (int i = 1; i < parts; ++i) {
-        const float4 x = *reinterpret_cast<const float4*>(from + static_cast<int64_t>(i) * 2 * 128 * p.s.dim);
+        const float4 x = *reinterpret_cast<const float4*>(from + static_cast<int64_t>(i) * 2 * RB * p.s.dim);
         t.x += x.x;
         t.y += x.y;
         t.z += x.z;
@@ -360,13 +401,51 @@ __global__ __launch_bounds__(kJoin) void attention_join_kernel(Backward p, int f
     }
     const float f = which == 0 ? p.scale : 1.0f;
     S_<T>* out = static_cast<S_<T>*>(which == 0 ? p.dk : p.dv) +
-                 ((static_cast<int64_t>(b) * p.s.keys + kb * 128 + row) * p.s.kv_heads + hk) * p.s.dim + d;
+                 ((static_cast<int64_t>(b) * p.s.keys + kb * RB + row) * p.s.kv_heads + hk) * p.s.dim + d;
     store4<T>(out, t.x * f, t.y * f, t.z * f, t.w * f);
+}
+
+template <typename T, int DT, int R, int W>
+void dq_blocks(Backward p, const AttentionArgs& a, hipStream_t on) {
+    p.blocks = (a.queries + 32 * W - 1) / (32 * W);
+    const int64_t items = static_cast<int64_t>(a.batch) * a.heads * p.blocks;
+    TP_AMD_CHECK(items < (int64_t{1} << 31), "sliding_window_attention_backward: too many rows");
+    attention_dq_kernel<T, DT, R, W><<<static_cast<unsigned>(items), W * kWave, 0, on>>>(p);
+    TP_AMD_HIP_CHECK(hipGetLastError());
+}
+
+template <typename T, int DT, int R, int W>
+void dkv_blocks(Backward p, const AttentionArgs& a, int device, hipStream_t on) {
+    constexpr int RB = 32 * W;
+    const int64_t pairs = p.pairs;
+    p.blocks = (a.keys + RB - 1) / RB;
+    // Tiles a walk has at most: of one near block, of one that stays visible.
+    const int64_t group = p.s.group, tiles = (a.queries + R - 1) / R;
+    const int64_t near = group * std::min<int64_t>(tiles, (RB + int64_t{p.s.rule.window} + R - 2) / R + 1), sink = group * tiles;
+    p.sink_blocks = std::min(p.blocks, (p.s.rule.sinks + RB - 1) / RB);
+    const int64_t want = (W == kWide ? 2 : 4) * cu_count(device);  // blocks that fill the device once
+    const int64_t near_blocks = pairs * (p.blocks - p.sink_blocks);
+    p.near_parts = near_blocks == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min(want / near_blocks, near / 4)));
+    const int64_t piece = std::max<int64_t>(4, near_blocks == 0 ? sink * pairs * p.sink_blocks / want : near / p.near_parts);
+    p.sink_parts = p.sink_blocks == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, (sink + piece - 1) / piece));
+    const int64_t items = pairs * p.per_head();
+    TP_AMD_CHECK(items < (int64_t{1} << 31), "sliding_window_attention_backward: too many keys");
+    const bool cut = p.near_parts > 1 || p.sink_parts > 1;
+    const Workspace part(cut ? static_cast<size_t>(items) * 2 * RB * a.dim * sizeof(float) : 0, device);
+    p.part = static_cast<float*>(part.get());
+    attention_dkv_kernel<T, DT, R, W><<<static_cast<unsigned>(items), W * kWave, 0, on>>>(p);
+    TP_AMD_HIP_CHECK(hipGetLastError());
+    if (!cut) return;
+    const int first = p.sink_parts > 1 ? 0 : p.sink_blocks, end = p.near_parts > 1 ? p.blocks : p.sink_blocks;
+    const unsigned wide = static_cast<unsigned>((2 * RB * (a.dim / 4) + kJoin - 1) / kJoin);
+    TP_AMD_CHECK(pairs < 65536 && end - first < 65536, "sliding_window_attention_backward: too many heads to join");
+    attention_join_kernel<T, RB><<<dim3(wide, static_cast<unsigned>(end - first), static_cast<unsigned>(pairs)), kJoin, 0, on>>>(p, first);
+    TP_AMD_HIP_CHECK(hipGetLastError());
 }
 
 template <typename T, int DT>
 void backward_tiles(const AttentionArgs& a, int device) {
-    constexpr int BQ = kRows<T>;
+    constexpr int R = sizeof(S_<T>) == 2 ? 64 : 32;
     Backward p;
     p.s = shape_of(a);
     p.q = a.q;
@@ -380,41 +459,33 @@ void backward_tiles(const AttentionArgs& a, int device) {
     p.dv = a.dv;
     p.scale = a.scale;
     p.scale2 = a.scale * kLog2E;
-    const int64_t heads = static_cast<int64_t>(a.batch) * a.kv_heads;
-    const Workspace delta(static_cast<size_t>(a.batch) * a.heads * std::max(a.queries, 1) * sizeof(float), device);
-    p.delta = static_cast<float*>(delta.get());
+    const int64_t pairs = static_cast<int64_t>(a.batch) * a.kv_heads;
+    TP_AMD_CHECK(pairs < (int64_t{1} << 31), "sliding_window_attention_backward: too many heads");
+    p.pairs = static_cast<int>(pairs);
+    const size_t stats = static_cast<size_t>(a.batch) * a.heads * std::max(a.queries, 1);
+    const Workspace found(2 * stats * sizeof(float), device);
+    p.bias = static_cast<float*>(found.get());
+    p.delta = p.bias + stats;
     const hipStream_t on = stream(device);
+    const int64_t cus = cu_count(device), group = p.s.group;
     if (a.queries > 0) {
-        p.blocks = (a.queries + 127) / 128;
-        const int64_t items = static_cast<int64_t>(a.batch) * a.heads * p.blocks;
-        TP_AMD_CHECK(items < (int64_t{1} << 31), "sliding_window_attention_backward: too many rows");
-        attention_dq_kernel<T, DT><<<static_cast<unsigned>(items), 4 * kWave, 0, on>>>(p);
-        TP_AMD_HIP_CHECK(hipGetLastError());
+        // float32, bound by its products, fills more CUs with blocks of one
+        // wave: 2 x 1000 queries, 12 heads of 64 (192 wide blocks) 9 us less.
+        // 16-bit does not gain: 32 heads x 512 (128) 2.5 us more, x 1024 8 more.
+        if (sizeof(S_<T>) == 2 || wide_blocks(a.batch, a.heads, a.queries) >= cus) dq_blocks<T, DT, R, kWide>(p, a, on);
+        else if constexpr (sizeof(S_<T>) == 4) dq_blocks<T, DT, 32, 1>(p, a, on);
     }
     if (a.keys == 0) return;
-    p.blocks = (a.keys + 127) / 128;
-    // Tiles a walk has at most: of one near block, of one that stays visible.
-    const int64_t group = p.s.group, tiles = (a.queries + BQ - 1) / BQ;
-    const int64_t near = group * std::min<int64_t>(tiles, (128 + int64_t{p.s.rule.window} + BQ - 2) / BQ + 1), sink = group * tiles;
-    p.sink_blocks = std::min(p.blocks, (p.s.rule.sinks + 127) / 128);
-    const int64_t want = 2 * cu_count(device);  // blocks that fill the device once
-    const int64_t near_blocks = heads * (p.blocks - p.sink_blocks);
-    p.near_parts = near_blocks == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min(want / near_blocks, near / 4)));
-    const int64_t piece = std::max<int64_t>(4, near_blocks == 0 ? sink * heads * p.sink_blocks / want : near / p.near_parts);
-    p.sink_parts = p.sink_blocks == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, (sink + piece - 1) / piece));
-    const int64_t items = heads * p.per_head();
-    TP_AMD_CHECK(items < (int64_t{1} << 31), "sliding_window_attention_backward: too many keys");
-    const bool cut = p.near_parts > 1 || p.sink_parts > 1;
-    const Workspace part(cut ? static_cast<size_t>(items) * 2 * 128 * a.dim * sizeof(float) : 0, device);
-    p.part = static_cast<float*>(part.get());
-    attention_dkv_kernel<T, DT><<<static_cast<unsigned>(items), 4 * kWave, 0, on>>>(p);
-    TP_AMD_HIP_CHECK(hipGetLastError());
-    if (!cut) return;
-    const int first = p.sink_parts > 1 ? 0 : p.sink_blocks, end = p.near_parts > 1 ? p.blocks : p.sink_blocks;
-    const unsigned wide = static_cast<unsigned>((2 * 128 * (a.dim / 4) + kJoin - 1) / kJoin);
-    TP_AMD_CHECK(heads < 65536 && end - first < 65536, "sliding_window_attention_backward: too many heads to join");
-    attention_join_kernel<T><<<dim3(wide, static_cast<unsigned>(end - first), static_cast<unsigned>(heads)), kJoin, 0, on>>>(p, first);
-    TP_AMD_HIP_CHECK(hipGetLastError());
+    // Few key blocks: their walks are cut by query heads and rows, and the
+    // parts joined; where that leaves fewer than two wide blocks a CU but there
+    // are waves enough, blocks of one wave need no parts.  Whole backward, us,
+    // wide and one wave: 64 heads x 512 keys (256 wide blocks, no groups) 84
+    // and 79, 32 x 512 75 and 73, 16 x 2048 under a window of 512 61 and 56;
+    // float32 12 heads x 1000 139 and 113; 8 key heads of four each x 1024 (64)
+    // 115 and 130, 4 x 8 x 512 (128) 108 and 119.
+    const int64_t waves = pairs * ((a.keys + 31) / 32);
+    if (wide_blocks(a.batch, a.kv_heads, a.keys) * group >= 2 * cus || 2 * waves < 3 * cus) dkv_blocks<T, DT, R, kWide>(p, a, device, on);
+    else dkv_blocks<T, DT, 32, 1>(p, a, device, on);
 }
 
 template <typename T>

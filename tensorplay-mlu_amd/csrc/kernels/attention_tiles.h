@@ -12,6 +12,9 @@
 // exchange between the two halves of the wave.
 #pragma once
 
+#include <type_traits>
+#include <utility>
+
 #include "attention.h"
 #include "device_common.h"
 
@@ -20,6 +23,12 @@ namespace attention {
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef __attribute__((address_space(3))) void* LdsPtr;
+
+// f(0), f(1), ... with compile-time arguments.
+template <typename F, int... N>
+__device__ __forceinline__ void unrolled(const F& f, std::integer_sequence<int, N...>) {
+    (f(std::integral_constant<int, N>{}), ...);
+}
 
 template <typename T>
 using S_ = typename Elem<T>::storage;
@@ -32,6 +41,8 @@ struct Rule {
     int window;  // kNoWindow: every earlier key
     int sinks;
     __device__ __forceinline__ bool sees(int p, int j) const { return j <= p && (j > p - window || j < sinks); }
+    // The same for keys behind the first tokens: one unsigned comparison.
+    __device__ __forceinline__ bool near(int p, int j) const { return static_cast<unsigned>(p - j) < static_cast<unsigned>(window); }
     // Every row of p0 .. p1 sees all of the keys k0 .. k1.
     __device__ __forceinline__ bool all_see(int p0, int p1, int k0, int k1) const {
         return k1 <= p0 && (k0 > p1 - window || k1 < sinks);
@@ -216,29 +227,29 @@ struct Tile {
             head = first + wave * kPerLoad * step;
             records = static_cast<uint32_t>(((kPerLoad - 1) * step + dim) * E);
             row = wave * kPerLoad + lane / kChunks;
-#pragma unroll
-            for (int i = 0; i < kPeriod; ++i) {
+            unrolled([&](auto i) {
                 const int chunk = (lane % kChunks) ^ swizzle(i * W * kPerLoad + row);
                 off[i] = chunk * 16 < dim * E ? static_cast<uint32_t>(lane / kChunks * step * E) + chunk * 16 : kOutOfRange;
-            }
+            }, std::make_integer_sequence<int, kPeriod>{});
         }
 
         // Rows r0 .. r0 + R - 1 into `tile`: all of them if `whole`, else row r
         // if keep(r), the others as zeros.
         template <typename Keep>
-        __device__ __forceinline__ void issue(char* tile, int r0, int wave, bool whole, Keep&& keep) const {
+        __device__ __forceinline__ void issue(char* tile, int r0, int wave, bool whole, const Keep& keep) const {
             const S* from = head + r0 * step;
-            auto load = [&](int i, uint32_t at) {
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer_over(from + i * W * kPerLoad * step, records),
-                                                         (LdsPtr)(tile + (i * W + wave) * 1024), 16, at, 0, 0, AUX);
-            };
             if (whole) {
-#pragma unroll
-                for (int i = 0; i < kIssue; ++i) load(i, off[i % kPeriod]);
+                unrolled([&](auto i) { load(i, tile, from, wave, off[i % kPeriod]); }, std::make_integer_sequence<int, kIssue>{});
             } else {
-#pragma unroll
-                for (int i = 0; i < kIssue; ++i) load(i, keep(r0 + row + i * W * kPerLoad) ? off[i % kPeriod] : kOutOfRange);
+                unrolled([&](auto i) { load(i, tile, from, wave, keep(r0 + row + i * W * kPerLoad) ? off[i % kPeriod] : kOutOfRange); },
+                         std::make_integer_sequence<int, kIssue>{});
             }
+        }
+
+    private:
+        __device__ __forceinline__ void load(int i, char* tile, const S* from, int wave, uint32_t at) const {
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer_over(from + i * W * kPerLoad * step, records),
+                                                     (LdsPtr)(tile + (i * W + wave) * 1024), 16, at, 0, 0, AUX);
         }
     };
 
@@ -353,6 +364,14 @@ __device__ __forceinline__ int xcd_run(int bid, int total) {
 
 constexpr float kLog2E = 1.44269504088896340736f;
 constexpr float kLn2 = 0.69314718055994530942f;
+
+// Blocks own 32 rows a wave: of kWide waves where those are enough to give the
+// CUs work, else of one.
+constexpr int kWide = 4;
+
+inline int64_t wide_blocks(int64_t batch, int64_t heads, int64_t rows) {
+    return batch * heads * ((rows + 32 * kWide - 1) / (32 * kWide));
+}
 
 inline Shape shape_of(const AttentionArgs& a) {
     Shape s;
