@@ -278,8 +278,10 @@ int tp_amd_sliding_window_attention(const tp_amd_tensor* query, const tp_amd_ten
                                     const tp_amd_tensor* starts, tp_amd_tensor* out, tp_amd_tensor* lse);
 /* sliding_window_attention_backward: dquery, dkey and dvalue from the
  * forward's operands and results.  Key heads' gradients sum over their query
- * heads; rows of queries and keys outside their sequence get zeros.  Sums in
- * a fixed order. */
+ * heads; rows of queries and keys outside their sequence get zeros, as does a
+ * query whose lse is -inf.  Rows outside a sequence are not read; a value that
+ * is not finite reaches its block's neighbours as in the forward.  Sums in a
+ * fixed order. */
 int tp_amd_sliding_window_attention_backward(const tp_amd_tensor* grad_out, const tp_amd_tensor* query, const tp_amd_tensor* key,
                                              const tp_amd_tensor* value, const tp_amd_tensor* out, const tp_amd_tensor* lse,
                                              int64_t window, int64_t sinks, double scale, const tp_amd_tensor* lengths,

@@ -322,7 +322,7 @@ __global__ __launch_bounds__((kSplitWaves<T, DT> * kWave), 1) void attention_spl
             typename Keys::Loads k_loads, v_loads;
             k_loads.init(kh, p.k.token, p.s.dim, 0, lane);
             v_loads.init(vh, p.v.token, p.s.dim, 0, lane);
-            auto issue = [&](int i, char* kt, char* vt) {
+            auto issue = [&](int i, char* kt, char* vt) __attribute__((always_inline)) {
                 const int r0 = tiles.at(i) * 32;
                 const bool whole = keep.all(r0, r0 + 31);
                 k_loads.issue(kt + at, r0, 0, whole, keep);
@@ -335,7 +335,7 @@ __global__ __launch_bounds__((kSplitWaves<T, DT> * kWave), 1) void attention_spl
             typename Keys::Transposed cols;
             rows.init(lane);
             cols.init(lane);
-            auto step = [&](int i, const char* kt, const char* vt, char* kn, char* vn) {
+            auto step = [&](int i, const char* kt, const char* vt, char* kn, char* vn) __attribute__((always_inline)) {
                 const bool more = i + 1 < to;
                 if (more) {
                     reads_done();

@@ -86,7 +86,7 @@ __global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4)
         typename Keys::Loads k_loads, v_loads;
         k_loads.init(kh, p.k.token, p.s.dim, wave, lane);
         v_loads.init(vh, p.v.token, p.s.dim, wave, lane);
-        auto issue = [&](int i, char* kt, char* vt) {
+        auto issue = [&](int i, char* kt, char* vt) __attribute__((always_inline)) {
             const int r0 = tiles.at(i) * BK;
             const bool whole = keep.all(r0, r0 + BK - 1);
             k_loads.issue(kt, r0, wave, whole, keep);
@@ -118,7 +118,9 @@ __global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4)
         const int64_t stat = (static_cast<int64_t>(b) * p.s.heads + h) * p.s.queries + mine;
         float bias = 0.0f;
         if (alive) {
-            bias = -p.lse[stat] * kLog2E;
+            // (a row whose sum is 0 has no probabilities, whatever its scores)
+            const float l = p.lse[stat];
+            bias = l == -INFINITY ? -INFINITY : -l * kLog2E;
         }
         typename Keys::ByRows rows;
         typename Keys::Transposed cols;
@@ -247,7 +249,7 @@ __global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) voi
         // the walk's next tile to load: query head and first row
         int next_h = hk * p.s.group + from / per_query_head, next_row = (t0 + from % per_query_head) * BQ;
         const int end_row = (t0 + per_query_head) * BQ;
-        auto issue = [&](char* qt, char* dt, float* lt) {
+        auto issue = [&](char* qt, char* dt, float* lt) __attribute__((always_inline)) {
             const int h = next_h, r0 = next_row;
             next_row += BQ;
             if (next_row == end_row) {
@@ -292,15 +294,18 @@ __global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) voi
         rows.init(lane);
         cols.init(lane);
         // how far this lane's key is seen; a first token to the end
-        const unsigned reach_of_mine = mine < p.s.rule.sinks ? kNoWindow : p.s.rule.window;
-        auto step = [&](int it, const char* qt, const char* dt, const float* lt, char* qn, char* dn, float* ln) {
+        const int reach_of_mine = mine < p.s.rule.sinks ? kNoWindow : p.s.rule.window;
+        auto step = [&](int it, const char* qt, const char* dt, const float* lt, char* qn, char* dn, float* ln) __attribute__((always_inline)) {
             meet();
             const int r0 = row0;
             row0 = next_row;
             if (it + 1 < to) issue(qn, dn, ln);
             const int p0 = seq.start + max(r0, seq.first), p1 = seq.start + min(r0 + BQ, seq.end) - 1;
             if (w0 > w1 || !p.s.rule.any_sees(p0, p1, w0, w1)) return;
-            const bool whole = p.s.rule.all_see(p0, p1, w0, w1) && w1 == w0 + 31;
+            // (rows outside the sequence are zeros here, whose scores with an
+            // infinite key are no number: they are masked too)
+            const bool whole = p1 - p0 == BQ - 1 && p.s.rule.all_see(p0, p1, w0, w1) && w1 == w0 + 31;
+            const unsigned limit = max(min(reach_of_mine, p1 - mine + 1), 0);
 #pragma unroll
             for (int u = 0; u < NS; ++u) {
                 f32x16 s = zeros(), ds = zeros();
@@ -326,7 +331,7 @@ __global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) voi
                     for (int e = 0; e < 16; ++e) {
                         // (unsigned: rows before the key are out of reach too)
                         const unsigned behind = seq.start + r0 + 32 * u + row_of(e, half) - mine;
-                        if (behind >= reach_of_mine) s[e] = ds[e] = 0.0f;
+                        if (behind >= limit) s[e] = ds[e] = 0.0f;
                     }
                 }
 #pragma unroll
@@ -422,6 +427,7 @@ void dkv_blocks(Backward p, const AttentionArgs& a, int device, hipStream_t on) 
     // Tiles a walk has at most: of one near block, of one that stays visible.
     const int64_t group = p.s.group, tiles = (a.queries + R - 1) / R;
     const int64_t near = group * std::min<int64_t>(tiles, (RB + int64_t{p.s.rule.window} + R - 2) / R + 1), sink = group * tiles;
+    TP_AMD_CHECK(sink < (int64_t{1} << 31), "sliding_window_attention_backward: too many queries of one key head");
     p.sink_blocks = std::min(p.blocks, (p.s.rule.sinks + RB - 1) / RB);
     const int64_t want = (W == kWide ? 2 : 4) * cu_count(device);  // blocks that fill the device once
     const int64_t near_blocks = pairs * (p.blocks - p.sink_blocks);

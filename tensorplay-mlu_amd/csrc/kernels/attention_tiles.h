@@ -227,7 +227,7 @@ struct Tile {
             head = first + wave * kPerLoad * step;
             records = static_cast<uint32_t>(((kPerLoad - 1) * step + dim) * E);
             row = wave * kPerLoad + lane / kChunks;
-            unrolled([&](auto i) {
+            unrolled([&](auto i) __attribute__((always_inline)) {
                 const int chunk = (lane % kChunks) ^ swizzle(i * W * kPerLoad + row);
                 off[i] = chunk * 16 < dim * E ? static_cast<uint32_t>(lane / kChunks * step * E) + chunk * 16 : kOutOfRange;
             }, std::make_integer_sequence<int, kPeriod>{});
@@ -239,9 +239,9 @@ struct Tile {
         __device__ __forceinline__ void issue(char* tile, int r0, int wave, bool whole, const Keep& keep) const {
             const S* from = head + r0 * step;
             if (whole) {
-                unrolled([&](auto i) { load(i, tile, from, wave, off[i % kPeriod]); }, std::make_integer_sequence<int, kIssue>{});
+                unrolled([&](auto i) __attribute__((always_inline)) { load(i, tile, from, wave, off[i % kPeriod]); }, std::make_integer_sequence<int, kIssue>{});
             } else {
-                unrolled([&](auto i) { load(i, tile, from, wave, keep(r0 + row + i * W * kPerLoad) ? off[i % kPeriod] : kOutOfRange); },
+                unrolled([&](auto i) __attribute__((always_inline)) { load(i, tile, from, wave, keep(r0 + row + i * W * kPerLoad) ? off[i % kPeriod] : kOutOfRange); },
                          std::make_integer_sequence<int, kIssue>{});
             }
         }

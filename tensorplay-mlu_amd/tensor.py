@@ -106,9 +106,13 @@ class DeviceTensor:
     @staticmethod
     def from_result(ref: _abi.Tensor, base: "DeviceTensor | None" = None) -> "DeviceTensor":
         """Wrap a result an entry point wrote; a NULL ctx means a view of ``base``."""
-        if ref.ctx:
-            return DeviceTensor(ref)
-        return DeviceTensor(ref, base._owner if base is not None else None)
+        ctx = ref.ctx
+        if not ctx:
+            return DeviceTensor(ref, base._owner if base is not None else None)
+        tensor = DeviceTensor.__new__(DeviceTensor)  # as __init__ would, without its tests
+        tensor._ref, tensor._owner = ref, _Block(ctx)
+        ref.ctx = None
+        return tensor
 
     @staticmethod
     def empty(shape, dtype="float32", device: int = 0) -> "DeviceTensor":

@@ -285,3 +285,37 @@ def test_a_layer_recorded_and_replayed(dev, ops):
     a = Attention(BF16, wide(qr.numpy(), BF16), wide(kr.numpy(), BF16), wide(heads(packed, h + hk, hk).numpy(), BF16), **rule)
     assert_within(out.numpy(), a.tokens(a.out), a.tokens(a.out_bound), BF16, "out")
     assert_within(eager[11].numpy(), a.tokens(a.out)[:, -1:], a.tokens(a.out_bound)[:, -1:], BF16, "one token")
+
+
+@pytest.mark.parametrize("tq", [1, 130], ids=["split", "wide"])
+def test_offsets_past_32_bits(dev, ops, tq):
+    """A cache of more than 2^31 elements: the first tokens and the window's
+    are at its two ends."""
+    h, d, tk = 64, 128, 270000
+    k, v = ops.empty((1, tk, h, d), "bfloat16"), ops.empty((1, tk, h, d), "bfloat16")
+    assert k.numel() > 2 ** 31
+    near, sinks, window = 260, 3, 100
+    q, *tail = make(BF16, 1, tq, near, h, h, d, 120)[:3]
+    head = make(BF16, 1, 1, sinks, h, h, d, 130)[1:3]
+    for cache, a, b in zip((k, v), head, tail):
+        ops.zero_(cache)
+        ops.copy_(cache[:, :sinks], put(a, BF16))
+        ops.copy_(cache[:, tk - near:], put(b, BF16))
+    out, lse = ops.sliding_window_attention(put(q, BF16), k, v, window, sinks)
+    # the same rows with what lies between left out: nobody sees it
+    short = [np.concatenate([a, b], 1) for a, b in zip(head, tail)]
+    a = Attention(BF16, wide(q, BF16), *[wide(x, BF16) for x in short], window=window, sinks=sinks)
+    assert_within(out.numpy(), a.tokens(a.out), a.tokens(a.out_bound), BF16, "out")
+    assert_within(lse.numpy(), a.lse, a.lse_bound, F32, "lse")
+
+
+@pytest.mark.parametrize("tq", [1, 200])
+def test_scores_of_minus_infinity_only(dev, ops, tq):
+    """A row whose every score is -inf has no sum: zeros, -inf, no gradient."""
+    q, k, v, do = make(F32, 1, tq, 200, 1, 1, 16, 140)
+    q[:, :, :, 3], k[0, :, 0, 3] = 1.0, -np.inf
+    q, k, v, do = (put(x) for x in (q, k, v, do))
+    out, lse = ops.sliding_window_attention(q, k, v)
+    assert (out.numpy() == 0).all() and (lse.numpy() == -np.inf).all()
+    dv = ops.sliding_window_attention_backward(do, q, k, v, out, lse)[2]
+    assert (dv.numpy() == 0).all()
