@@ -203,6 +203,11 @@ template <typename T, int DT, int BQ, int W>
 __global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) void attention_dkv_kernel(Backward p) {
     using S = S_<T>;
     constexpr int NS = BQ / 32, RB = 32 * W;
+    // A lone wave has the registers to read all fragments of 32 rows before
+    // their products, and the transposed ones between these, where a CU's other
+    // waves do not hide the reads: 64 heads of 128 x 512, whole backward, 6 us
+    // less (float32, whose products take longer, does not gain).
+    constexpr bool kAhead = W == 1 && sizeof(S) == 2;
     using Rows = Tile<T, DT, BQ, W>;
     __shared__ __attribute__((aligned(1024))) char q0s[Rows::kBytes];
     __shared__ __attribute__((aligned(1024))) char d0s[Rows::kBytes];
@@ -309,10 +314,29 @@ __global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) voi
 #pragma unroll
             for (int u = 0; u < NS; ++u) {
                 f32x16 s = zeros(), ds = zeros();
+                uint4 qc[kAhead ? Rows::kSteps : 1], dc[kAhead ? Rows::kSteps : 1];
+                if constexpr (kAhead) {
+                    uint4 qr[Rows::kSteps], dr[Rows::kSteps];
 #pragma unroll
-                for (int f = 0; f < Rows::kSteps; ++f) {
-                    s = mma<T>(rows.read(qt, u, f), kf[f], s);
-                    ds = mma<T>(rows.read(dt, u, f), vf[f], ds);
+                    for (int f = 0; f < Rows::kSteps; ++f) {
+                        qr[f] = rows.read(qt, u, f);
+                        dr[f] = rows.read(dt, u, f);
+                    }
+#pragma unroll
+                    for (int f = 0; f < Rows::kSteps; ++f) {
+                        __builtin_amdgcn_sched_barrier(0);
+                        s = mma<T>(qr[f], kf[f], s);
+                        ds = mma<T>(dr[f], vf[f], ds);
+                        qc[f] = cols.read(qt, f % DT, u, f / DT);
+                        dc[f] = cols.read(dt, f % DT, u, f / DT);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                } else {
+#pragma unroll
+                    for (int f = 0; f < Rows::kSteps; ++f) {
+                        s = mma<T>(rows.read(qt, u, f), kf[f], s);
+                        ds = mma<T>(rows.read(dt, u, f), vf[f], ds);
+                    }
                 }
 #pragma unroll
                 for (int e = 0; e < 16; e += 4) {
@@ -339,8 +363,8 @@ __global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) voi
                     const uint4 pf = pack_rows<T>(s, f), sf = pack_rows<T>(ds, f);
 #pragma unroll
                     for (int d = 0; d < DT; ++d) {
-                        dv[d] = mma<T>(cols.read(dt, d, u, f), pf, dv[d]);
-                        dk[d] = mma<T>(cols.read(qt, d, u, f), sf, dk[d]);
+                        dv[d] = mma<T>(kAhead ? dc[f * DT + d] : cols.read(dt, d, u, f), pf, dv[d]);
+                        dk[d] = mma<T>(kAhead ? qc[f * DT + d] : cols.read(qt, d, u, f), sf, dk[d]);
                     }
                 }
             }
@@ -483,14 +507,15 @@ void backward_tiles(const AttentionArgs& a, int device) {
     }
     if (a.keys == 0) return;
     // Few key blocks: their walks are cut by query heads and rows, and the
-    // parts joined; where that leaves fewer than two wide blocks a CU but there
-    // are waves enough, blocks of one wave need no parts.  Whole backward, us,
-    // wide and one wave: 64 heads x 512 keys (256 wide blocks, no groups) 84
-    // and 79, 32 x 512 75 and 73, 16 x 2048 under a window of 512 61 and 56;
-    // float32 12 heads x 1000 139 and 113; 8 key heads of four each x 1024 (64)
-    // 115 and 130, 4 x 8 x 512 (128) 108 and 119.
-    const int64_t waves = pairs * ((a.keys + 31) / 32);
-    if (wide_blocks(a.batch, a.kv_heads, a.keys) * group >= 2 * cus || 2 * waves < 3 * cus) dkv_blocks<T, DT, R, kWide>(p, a, device, on);
+    // parts joined.  Blocks of one wave find more room on the CUs, and four
+    // waves that share what they load are ahead where there are wide blocks
+    // enough or the walks are long.  Whole backward, us, wide and one wave:
+    // 64 heads x 512 keys 82 and 70, 8 x 256 47 and 41, 2 x 32 x 768 109 and 99,
+    // 2 key heads of 4 each x 4096 under a window of 512 100 and 91; float32
+    // 12 x 1000 128 and 111; and 8 key heads of 4 each x 1024 114 and 120, 4 x 32
+    // x 1024 233 and 242, 1 key head of 4 x 8192 596 and 726.
+    const int64_t walk = group * std::min(a.queries, p.s.rule.window);
+    if (wide_blocks(a.batch, a.kv_heads, a.keys) * group >= 2 * cus || walk >= 4096) dkv_blocks<T, DT, R, kWide>(p, a, device, on);
     else dkv_blocks<T, DT, 32, 1>(p, a, device, on);
 }
 

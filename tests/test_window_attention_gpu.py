@@ -216,6 +216,26 @@ def test_walks_in_parts(dev, ops, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("rule", RULES, ids=str)
+def test_many_heads(dev, ops, dtype, rule):
+    """Work enough for blocks of several waves on every kernel's side, of heads
+    that share keys and of heads that do not."""
+    check(ops, dtype, make(dtype, 2, 131, 131, 128, 32, 40, 150), rule)
+    check(ops, dtype, make(dtype, 2, 70, 140, 128, 128, 24, 160), rule)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("tq,dim", [(150, 64), (290, 128)])
+def test_many_heads_padded(dev, ops, dtype, tq, dim):
+    """The same, and long walks in parts, over sequences of every length."""
+    lengths, starts = np.array([290, 130, 0, 1]), np.array([140, -3, 0, 289 - tq])
+    for heads, kv in ((32, 32), (32, 1)):
+        host = make(dtype, 4, tq, 290, heads, kv, dim, 170)
+        check(ops, dtype, host, dict(lengths=lengths, starts=starts))
+        check(ops, dtype, host, dict(window=129, sinks=5, lengths=lengths))
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("batch,tq,heads,kv", [(1, 1, 8, 8), (1, 1, 8, 1), (3, 2, 6, 2), (5, 9, 8, 2), (64, 1, 4, 2), (2, 33, 4, 1)])
 def test_long_caches(dev, ops, dtype, batch, tq, heads, kv):
     """A few queries over a long cache: the keys are split over blocks."""
