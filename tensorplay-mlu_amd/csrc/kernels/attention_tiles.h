@@ -41,8 +41,6 @@ struct Rule {
     int window;  // kNoWindow: every earlier key
     int sinks;
     __device__ __forceinline__ bool sees(int p, int j) const { return j <= p && (j > p - window || j < sinks); }
-    // The same for keys behind the first tokens: one unsigned comparison.
-    __device__ __forceinline__ bool near(int p, int j) const { return static_cast<unsigned>(p - j) < static_cast<unsigned>(window); }
     // Every row of p0 .. p1 sees all of the keys k0 .. k1.
     __device__ __forceinline__ bool all_see(int p0, int p1, int k0, int k1) const {
         return k1 <= p0 && (k0 > p1 - window || k1 < sinks);

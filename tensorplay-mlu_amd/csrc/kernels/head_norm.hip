@@ -17,6 +17,11 @@
 // element, unaligned 16-byte loads cost nothing here), else single elements.
 // A group takes ROWS heads of one token in a row: their loads go out together
 // and the table's row, as many bytes as a 16-bit head, is read once for all.
+//
+// bf16, 40 heads of 128: 8192 tokens forward 31.5 us, 5.5 TB/s; 4 x 2048 backward
+// 45 us, 5.6 TB/s, and 4 us for the weights' sums over blocks (2 GiB read and
+// written by a plain elementwise pass: 6.35 TB/s).  8 tokens 3.7 us, a launch's
+// own time.
 
 #include <algorithm>
 #include <type_traits>
