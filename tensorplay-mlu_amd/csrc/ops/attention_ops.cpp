@@ -60,6 +60,7 @@ bool axes_merge(const TensorRef& t, int n, int64_t& step) {
 struct Tokens {
     Sizes shape;
     int64_t outer = 1, inner = 1;
+    Tokens() = default;
     explicit Tokens(const TensorRef& t) {
         for (int d = 0; d + 2 < t.ndim; ++d) shape.push_back(t.sizes[d]);
         for (size_t d = 0; d + 1 < shape.size(); ++d) outer *= shape[d];
@@ -95,8 +96,7 @@ struct HeadNorm {
     MaybeOwned hold_q, hold_k, hold_table, hold_pos, hold_w[2];
 
     HeadNorm(const TensorRef& q, const TensorRef& k, const TensorRef& table, const TensorRef& positions,
-             const tp_amd_tensor* qw, const tp_amd_tensor* kw, int interleaved)
-        : tokens(q.ndim >= 2 ? q : TensorRef{}) {
+             const tp_amd_tensor* qw, const tp_amd_tensor* kw, int interleaved) {
         check_view(q, "query");
         check_view(k, "key");
         check_view(table, "table");
@@ -107,6 +107,7 @@ struct HeadNorm {
         }
         const int64_t dim = q.sizes[q.ndim - 1], rotary = table.sizes[1];
         if (dim > kHeadNormMaxDim) TP_AMD_DECLINE("qk_norm_rope: heads wider than the device kernels take");
+        tokens = Tokens(q);
         const Tokens key_tokens(k);
         TP_AMD_CHECK(k.sizes[k.ndim - 1] == dim && key_tokens.shape == tokens.shape,
                      "qk_norm_rope: queries and keys differ in their tokens or head size");

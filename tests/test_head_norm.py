@@ -88,3 +88,11 @@ def test_backward_refused(ops, change, error):
 def test_null_operand(ops):
     with pytest.raises(mod("tensor").DeviceError, match="null"):
         call(ops, table=None)
+
+
+def test_more_axes_than_a_tensor_has(ops):
+    """Refused before an axis past the last one is looked at."""
+    query = fake((2, 5, 4, 16))
+    query._ref.ndim = 10 ** 9
+    with pytest.raises(mod("tensor").DeviceError, match="dimensions"):
+        call(ops, query=query)
