@@ -467,7 +467,11 @@ void dkv_blocks(Backward p, const AttentionArgs& a, int device, hipStream_t on) 
     const int64_t want = (W == kWide ? 2 : 4) * cu_count(device);  // blocks that fill the device once
     const int64_t near_blocks = pairs * (p.blocks - p.sink_blocks);
     p.near_parts = near_blocks == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, std::min(want / near_blocks, near / 4)));
-    const int64_t piece = std::max<int64_t>(4, near_blocks == 0 ? sink * pairs * p.sink_blocks / want : near / p.near_parts);
+    // Parts as long as the other walks, and no more than four rounds of them:
+    // each leaves 2 RB rows of sums (4 heads of 128 x 8192 under 4096 first
+    // tokens and a window of 1: 160 MB, where parts of 4 tiles took 1.1 GB).
+    const int64_t even = sink * pairs * p.sink_blocks / want;
+    const int64_t piece = std::max({int64_t{4}, even / 4, near_blocks == 0 ? even : near / p.near_parts});
     p.sink_parts = p.sink_blocks == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, (sink + piece - 1) / piece));
     const int64_t items = pairs * p.per_head();
     TP_AMD_CHECK(items < (int64_t{1} << 31), "sliding_window_attention_backward: too many keys");

@@ -215,6 +215,30 @@ def test_walks_in_parts(dev, ops, dtype):
     check(ops, dtype, host, dict())
 
 
+def test_sums_of_many_first_tokens_stay_small(dev, ops):
+    """Thousands of first tokens beside a short window: the parts of their
+    walks are bounded by the device's blocks, not by the walks' length."""
+    runtime = mod("runtime")
+    t, h, d = 8192, 4, 128
+    q, k, v, do = (put(x, BF16) for x in make(BF16, 1, t, t, h, h, d, 180))
+    out, lse = ops.sliding_window_attention(q, k, v, 1, 4096)
+    runtime.synchronize()
+    runtime.reset_peak_memory_stats()
+    before = runtime.memory_allocated()
+    dq, dk, dv = ops.sliding_window_attention_backward(do, q, k, v, out, lse, 1, 4096)
+    runtime.synchronize()
+    # parts: at most 4 rounds of 4 blocks a CU and one more a block of first
+    # tokens, of 2 x 32 rows of float32; results and statistics beside them
+    blocks = 16 * runtime.compute_units() + h * 4096 // 32
+    bound = blocks * 2 * 32 * d * 4 + 3 * t * h * d * 2 + 2 * t * h * 4
+    assert runtime.max_memory_allocated() - before <= 1.1 * bound
+    # the rows of dv add up to do: every row of P adds up to 1 (each P rounded
+    # to bf16, 8192 rows of do's size, and dv's own rounding)
+    d64 = wide(do.numpy(), BF16)[0].sum(0)
+    v64 = wide(dv.numpy(), BF16)[0]
+    assert (np.abs(v64.sum(0) - d64) <= 2.0 ** -8 * (np.abs(wide(do.numpy(), BF16)[0]).sum(0) + np.abs(v64).sum(0)) + 1e-2).all()
+
+
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("rule", RULES, ids=str)
 def test_many_heads(dev, ops, dtype, rule):
