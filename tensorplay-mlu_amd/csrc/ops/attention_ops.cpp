@@ -1,15 +1,15 @@
 // The attention layer's operators: the norm and position rotation of each
 // head's query and key (kernels/head_norm.hip), and causal attention with a
 // sliding window and first tokens that stay visible (kernels/attention.hip,
-// kernels/attention_backward.hip), forward and backward.  The reference has no counterpart; entries follow the neural-network layers'
-// conventions: device float tensors of one dtype or the call is declined,
-// shapes that contradict each other are errors, operands are read where they
-// lie and copied only when the kernels cannot address them.
+// kernels/attention_backward.hip), forward and backward.  The reference has no
+// counterpart; entries follow the neural-network layers' conventions: device
+// float tensors of one dtype or the call is declined, shapes that contradict
+// each other are errors, operands are read where they lie and copied only when
+// the kernels cannot address them.
 
 #include <initializer_list>
 
 #include "../kernels/attention.h"
-#include "../runtime.h"
 #include "tensor.h"
 #include "tp_amd_ops.h"
 
@@ -231,7 +231,8 @@ struct Attention {
                      " query heads cannot share ", k.sizes[2], " key heads");
         TP_AMD_CHECK(sinks >= 0, "sliding_window_attention: negative sinks");
         const float s = static_cast<float>(scale);
-        TP_AMD_CHECK(s > 0.0f && s <= 3.4028234663852886e38f, "sliding_window_attention: the scale has to be positive and finite");
+        // (also times log2 e, as the kernels' powers of two have it)
+        TP_AMD_CHECK(s > 0.0f && s < 2.3e38f, "sliding_window_attention: the scale has to be positive and finite");
         TP_AMD_CHECK(q.sizes[1] + k.sizes[1] < (int64_t{1} << 30) && b < (int64_t{1} << 30) && q.sizes[2] < (int64_t{1} << 30),
                      "sliding_window_attention: sizes past 2^30");
         per_sequence(lengths, "lengths", b, q.device, args.lengths, args.wide_lengths, args.lengths_step);

@@ -91,7 +91,7 @@ def test_declined(ops, change):
     ({"key": fake((2, 7, 0, 16)), "value": fake((2, 7, 0, 16))}, "share"),
     ({"sinks": -1}, "sinks"),
     ({"scale": 0.0}, "scale"), ({"scale": -1.0}, "scale"), ({"scale": float("nan")}, "scale"),
-    ({"scale": float("inf")}, "scale"), ({"scale": 1e-60}, "scale"),
+    ({"scale": float("inf")}, "scale"), ({"scale": 3e38}, "scale"), ({"scale": 1e-60}, "scale"),
     ({"lengths": fake((3,), "int32")}, "lengths"),
     ({"starts": fake((2, 1), "int32")}, "starts"),
     ({"key": fake((2, 1 << 30, 2, 16)), "value": fake((2, 1 << 30, 2, 16))}, "2\\^30"),
