@@ -8,7 +8,15 @@
 
 #include <cstdint>
 
+#include "../common.h"
+
 namespace tp_amd {
+
+// Blocks of a launch, whose threads are counted in 32 bits.
+inline unsigned grid_of(int64_t blocks, int threads, const char* op) {
+    TP_AMD_CHECK(blocks * threads < (int64_t{1} << 32), op, ": too many rows for one launch");
+    return static_cast<unsigned>(blocks);
+}
 
 // Rows [outer][inner][head][D] of one tensor, the last axis dense.
 struct HeadRows {

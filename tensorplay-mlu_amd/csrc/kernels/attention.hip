@@ -523,7 +523,7 @@ void split_tiles(const AttentionArgs& a, int device) {
     int64_t splits = std::min({rounds * cus / items, (tiles + W - 1) / W, int64_t(W) * Tile<T, DT, 32, 1>::kBytes / 8 / here});
     while (splits > 1 && splits * splits * back > walk) --splits;
     q.splits = items > kMaxSplitItems ? 1 : static_cast<int>(std::max<int64_t>(1, splits));
-    TP_AMD_CHECK(items * q.splits < (int64_t{1} << 30), "sliding_window_attention: too many rows");
+    const unsigned grid = grid_of(items * q.splits, W * kWave, "sliding_window_attention");
     q.by_splits = make_fastdiv(static_cast<uint32_t>(q.splits));
     q.by_row_tiles = make_fastdiv(static_cast<uint32_t>(q.row_tiles));
     q.by_kv_heads = make_fastdiv(static_cast<uint32_t>(a.kv_heads));
@@ -541,7 +541,7 @@ void split_tiles(const AttentionArgs& a, int device) {
     // again (16 x 2000 keys 20.1 us non-temporal, 19.4 so).
     const int64_t bytes = 2 * int64_t{32} * tiles * a.batch * a.kv_heads * a.dim * sizeof(S_<T>);
     auto* kernel = q.row_tiles == 1 && bytes > (int64_t{128} << 20) ? attention_split_kernel<T, DT, kNt> : attention_split_kernel<T, DT, 0>;
-    kernel<<<static_cast<unsigned>(items * q.splits), W * kWave, 0, stream(device)>>>(q);
+    kernel<<<grid, W * kWave, 0, stream(device)>>>(q);
     TP_AMD_HIP_CHECK(hipGetLastError());
 }
 
@@ -565,8 +565,8 @@ void forward_tiles(const AttentionArgs& a, int device) {
     Forward p = forward_of(a);
     p.blocks = (a.queries + 32 * kWide - 1) / (32 * kWide);
     const int64_t items = static_cast<int64_t>(p.pairs) * p.s.group * p.blocks;
-    TP_AMD_CHECK(items < (int64_t{1} << 31), "sliding_window_attention: too many rows");
-    attention_kernel<T, DT><<<static_cast<unsigned>(items), kWide * kWave, 0, stream(device)>>>(p);
+    const unsigned grid = grid_of(items, kWide * kWave, "sliding_window_attention");
+    attention_kernel<T, DT><<<grid, kWide * kWave, 0, stream(device)>>>(p);
     TP_AMD_HIP_CHECK(hipGetLastError());
 }
 

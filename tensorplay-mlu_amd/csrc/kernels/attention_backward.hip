@@ -449,8 +449,8 @@ template <typename T, int DT, int R, int W>
 void dq_blocks(Backward p, const AttentionArgs& a, hipStream_t on) {
     p.blocks = (a.queries + 32 * W - 1) / (32 * W);
     const int64_t items = static_cast<int64_t>(a.batch) * a.heads * p.blocks;
-    TP_AMD_CHECK(items < (int64_t{1} << 31), "sliding_window_attention_backward: too many rows");
-    attention_dq_kernel<T, DT, R, W><<<static_cast<unsigned>(items), W * kWave, 0, on>>>(p);
+    const unsigned grid = grid_of(items, W * kWave, "sliding_window_attention_backward");
+    attention_dq_kernel<T, DT, R, W><<<grid, W * kWave, 0, on>>>(p);
     TP_AMD_HIP_CHECK(hipGetLastError());
 }
 
@@ -474,16 +474,16 @@ void dkv_blocks(Backward p, const AttentionArgs& a, int device, hipStream_t on) 
     const int64_t piece = std::max({int64_t{4}, even / 4, near_blocks == 0 ? even : near / p.near_parts});
     p.sink_parts = p.sink_blocks == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, (sink + piece - 1) / piece));
     const int64_t items = pairs * p.per_head();
-    TP_AMD_CHECK(items < (int64_t{1} << 31), "sliding_window_attention_backward: too many keys");
+    const unsigned grid = grid_of(items, W * kWave, "sliding_window_attention_backward");
     const bool cut = p.near_parts > 1 || p.sink_parts > 1;
     const Workspace part(cut ? static_cast<size_t>(items) * 2 * RB * a.dim * sizeof(float) : 0, device);
     p.part = static_cast<float*>(part.get());
-    attention_dkv_kernel<T, DT, R, W><<<static_cast<unsigned>(items), W * kWave, 0, on>>>(p);
+    attention_dkv_kernel<T, DT, R, W><<<grid, W * kWave, 0, on>>>(p);
     TP_AMD_HIP_CHECK(hipGetLastError());
     if (!cut) return;
     const int first = p.sink_parts > 1 ? 0 : p.sink_blocks, end = p.near_parts > 1 ? p.blocks : p.sink_blocks;
     const unsigned wide = static_cast<unsigned>((2 * RB * (a.dim / 4) + kJoin - 1) / kJoin);
-    TP_AMD_CHECK(pairs < 65536 && end - first < 65536, "sliding_window_attention_backward: too many heads to join");
+    // (walks are cut only where blocks are few: both are far below 2^16)
     attention_join_kernel<T, RB><<<dim3(wide, static_cast<unsigned>(end - first), static_cast<unsigned>(pairs)), kJoin, 0, on>>>(p, first);
     TP_AMD_HIP_CHECK(hipGetLastError());
 }

@@ -370,7 +370,7 @@ template <typename T, int V, int UPL, int ROWS>
 void forward_rows(const HeadNormArgs& p, int device) {
     const HeadNormPlan w = plan_of(p, V, ROWS);
     const uint64_t groups = static_cast<uint64_t>(w.tokens) * w.slots;
-    const unsigned blocks = static_cast<unsigned>((groups * w.lanes + kBlock - 1) / kBlock);
+    const unsigned blocks = grid_of(static_cast<int64_t>((groups * w.lanes + kBlock - 1) / kBlock), kBlock, "qk_norm_rope");
     auto* kernel = p.interleaved ? head_norm_kernel<T, V, UPL, true, ROWS> : head_norm_kernel<T, V, UPL, false, ROWS>;
     kernel<<<blocks, kBlock, 0, stream(device)>>>(w);
     TP_AMD_HIP_CHECK(hipGetLastError());
@@ -407,8 +407,8 @@ void backward_units(const HeadNormArgs& p, int device) {
     TP_AMD_HIP_CHECK(hipGetLastError());
 }
 
-// Indices are 32 bits: a row is one of fewer than 2^31, of at most 64 lanes
-// each (groups past the last row's block reach fewer than 2^31 as well).
+// Rows and groups of lanes are counted in 32 bits, those past the last row's
+// in its block among them.
 void check_extent(const HeadNormArgs& p) {
     const int64_t rows = p.outer * p.inner * (static_cast<int64_t>(p.side[0].heads) + p.side[1].heads);
     TP_AMD_CHECK(p.dim > 0 && p.dim <= kHeadNormMaxDim && p.rotary >= 0 && p.rotary <= p.dim && p.rotary % 2 == 0,

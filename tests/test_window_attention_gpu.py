@@ -353,6 +353,13 @@ def test_offsets_past_32_bits(dev, ops, tq):
     assert_within(lse.numpy(), a.lse, a.lse_bound, F32, "lse")
 
 
+def test_more_rows_than_a_launch_has(dev, ops):
+    """2^24 sequences' blocks of 256 threads are 2^32 threads: refused."""
+    one = put(np.zeros((1, 1, 1, 8), np.float16)).expand(1 << 24, 1, 1, 8)
+    with pytest.raises(mod("tensor").DeviceError, match="too many rows"):
+        ops.sliding_window_attention(one, one, one)
+
+
 @pytest.mark.parametrize("tq", [1, 200])
 def test_scores_of_minus_infinity_only(dev, ops, tq):
     """A row whose every score is -inf has no sum: zeros, -inf, no gradient."""
