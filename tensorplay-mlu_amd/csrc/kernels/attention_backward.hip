@@ -524,13 +524,16 @@ void backward_tiles(const AttentionArgs& a, int device) {
     // Few key blocks: their walks are cut by query heads and rows, and the
     // parts joined.  Blocks of one wave find more room on the CUs, and four
     // waves that share what they load are ahead where there are wide blocks
-    // enough or the walks are long.  Whole backward, us, wide and one wave:
-    // 64 heads x 512 keys 82 and 70, 8 x 256 47 and 41, 2 x 32 x 768 109 and 99,
-    // 2 key heads of 4 each x 4096 under a window of 512 100 and 91; float32
-    // 12 x 1000 128 and 111; and 8 key heads of 4 each x 1024 114 and 120, 4 x 32
-    // x 1024 233 and 242, 1 key head of 4 x 8192 596 and 726.
+    // enough or the walks are long; without a window, where they are of every
+    // length and parts even them out, sooner.  Whole backward, us, wide and one
+    // wave: 64 heads x 512 keys 82 and 70, 8 x 256 47 and 41, 2 x 32 x 768 109
+    // and 99, 8 x 1024 80 and 76, 2 key heads of 4 each x 4096 under a window of
+    // 512 100 and 91; and 16 x 2000 181 and 195, 8 key heads of 4 each x 1024 114
+    // and 120, 4 x 32 x 1024 233 and 242, 8 x 4096 190 and 257; float32 12 x 1000
+    // under 256 128 and 111, 8 key heads of 4 each x 1024 281 and 338.
+    const bool even = p.s.rule.window < a.queries;
     const int64_t walk = group * std::min(a.queries, p.s.rule.window);
-    if (wide_blocks(a.batch, a.kv_heads, a.keys) * group >= 2 * cus || walk >= 4096) dkv_blocks<T, DT, R, kWide>(p, a, device, on);
+    if (wide_blocks(a.batch, a.kv_heads, a.keys) * group >= 2 * cus || walk >= (even ? 4096 : 1536)) dkv_blocks<T, DT, R, kWide>(p, a, device, on);
     else dkv_blocks<T, DT, 32, 1>(p, a, device, on);
 }
 
