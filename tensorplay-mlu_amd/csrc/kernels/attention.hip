@@ -258,9 +258,11 @@ __device__ __forceinline__ float2 load_shared(const float* at) {
     return make_float2(__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32)));
 }
 
-// A state (bound m, sum t, four outputs x) added to one on bound `top`.
+// A state (bound m, sum t, four outputs x) added to one on bound `top`.  (A
+// bound is a maximum, which passes over NaN: a state that met nothing but NaN
+// has m = -inf, as one that met no key, but a sum of NaN.)
 __device__ __forceinline__ void add_state(float m, float t, const float4& x, float top, float& total, float (&o)[4]) {
-    if (m == -INFINITY) return;  // it met no key
+    if (t == 0.0f) return;  // it met no key
     const float turn = __builtin_amdgcn_exp2f(m - top);
     total = fmaf(t, turn, total);
     o[0] = fmaf(x.x, turn, o[0]);
