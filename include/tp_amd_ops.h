@@ -281,7 +281,9 @@ int tp_amd_sliding_window_attention(const tp_amd_tensor* query, const tp_amd_ten
  * heads; rows of queries and keys outside their sequence get zeros, as does a
  * query whose lse is -inf.  Rows outside a sequence are not read; a value that
  * is not finite reaches its block's neighbours as in the forward.  Sums in a
- * fixed order. */
+ * fixed order, float32; the probabilities P and dS = P (dP - D) are rounded to
+ * the operands' dtype, in float16 at a power of two times their size, so that
+ * gradients of any size that dtype holds keep its precision. */
 int tp_amd_sliding_window_attention_backward(const tp_amd_tensor* grad_out, const tp_amd_tensor* query, const tp_amd_tensor* key,
                                              const tp_amd_tensor* value, const tp_amd_tensor* out, const tp_amd_tensor* lse,
                                              int64_t window, int64_t sinks, double scale, const tp_amd_tensor* lengths,

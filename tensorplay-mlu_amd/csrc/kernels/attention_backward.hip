@@ -16,7 +16,10 @@
 // than the others: their walks are cut into parts of about the others' length,
 // and with few blocks all walks are, the parts' float32 sums joined in order by
 // a third kernel.  P and dS are rounded to the operands' type for the matrix
-// instruction; sums are float32.
+// instruction; sums are float32.  float16 does not hold every dS: it has the
+// gradients' size, 1 / scale times what dq needs and 1 / keys of it.  So there
+// dS is rounded at a power of two times its size that each sum keeps for itself
+// (ColumnScale), and P at 2^12 times.
 //
 // Bound by the instructions that share a wave's issue: matrix products, and
 // beside them an exponential, two products and two roundings an element and
@@ -46,7 +49,7 @@ struct Backward {
     TokenRows q, k, v, o, dout;
     const float* lse;
     // what the first kernel finds of every query for the second one: -l log2 e
-    // and D, [batch][heads][queries] each
+    // (and the bits P is scaled by) and D, [batch][heads][queries] each
     float *bias, *delta;
     void *dq, *dk, *dv;
     float scale, scale2;  // scale2: times log2 e
@@ -57,6 +60,50 @@ struct Backward {
     int sink_blocks, sink_parts, near_parts;
     float* part;  // [head][part][2][rows][dim]
     int per_head() const { return sink_blocks * sink_parts + (blocks - sink_blocks) * near_parts; }
+};
+
+// P is rounded at this power of two times its size.  float16 is full down to
+// 2^-14 and steps by 2^-24 below, less than the P of 2^14 keys and more; P itself
+// is at most 1 but for the rounding of s - l, which has 2^4 left.
+template <typename T>
+constexpr int kProbabilityBits = std::is_same_v<T, f16_t> ? 12 : 0;
+
+// The power of two that the dS of a lane's column are multiplied with before
+// float16 rounds them: the first that are not 0, and any that would pass 2^15,
+// are brought to 2^7 .. 2^8, and the column's sums with them.  So an element is off
+// by its half step or by 2^-32 of the column's largest so far.  (Other types have
+// float32's exponents and leave dS as it is.)  The maximum and the products are
+// 3 % of forward and backward of 2 x 4096 tokens, 32 heads of 128 under a window
+// of 1024 (706 us without, 728 with), 11 % of 64 heads x 512 (68 and 75).
+template <typename T>
+struct ColumnScale {
+    static constexpr bool kOn = std::is_same_v<T, f16_t>;
+    float up = 0x1p60f;
+
+    template <int DT>
+    __device__ __forceinline__ void apply(f32x16& ds, f32x16 (&sums)[DT]) {
+        if constexpr (kOn) {
+            float top = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(ds[e]));
+            top = both_halves(top, MaxOf{});
+            const bool past = top * up > 0x1p15f;
+            if (__any(past)) {
+                // 2^(7 - exponent of top), for an infinite one too
+                const float next = past ? __uint_as_float((261u << 23) - (__float_as_uint(top) & 0x7f800000u)) : up;
+                const float turn = next * down();
+                up = next;
+#pragma unroll
+                for (int d = 0; d < DT; ++d)
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) sums[d][e] *= turn;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) ds[e] *= up;
+        }
+    }
+    // What the sums are multiplied with in the end.
+    __device__ __forceinline__ float down() const { return kOn ? __uint_as_float((254u << 23) - __float_as_uint(up)) : 1.0f; }
 };
 
 template <typename T, int DT, int BK, int W>
@@ -88,6 +135,7 @@ __global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4)
     f32x16 dq[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) dq[d] = zeros();
+    ColumnScale<T> scaled;
     if (b0 <= b1) {
         const int p0 = seq.start + b0, p1 = seq.start + b1;
         const KeyTiles tiles(p.s.rule, p0, p1, BK);
@@ -167,6 +215,7 @@ __global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4)
                     for (int e = 0; e < 16; ++e) exact += ds[e];
                     continue;
                 }
+                scaled.apply(ds, dq);
 #pragma unroll
                 for (int f = 0; f < kFragsOf32<T>; ++f) {
                     const uint4 sf = pack_rows<T>(ds, f);
@@ -192,7 +241,7 @@ __global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4)
             if (tiles.count > 0) issue(0, k0s, v0s);
         }
         if (alive && half == 0) {
-            p.bias[stat] = bias;
+            p.bias[stat] = bias + kProbabilityBits<T>;
             p.delta[stat] = delta;
         }
         walk(std::true_type{});
@@ -205,7 +254,7 @@ __global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4)
         for (int e = 0; e < 16; e += 4) {
             const int at = 32 * d + row_of(e, half);
             if (at >= p.s.dim) continue;
-            const auto value = [&](int j) { return alive ? dq[d][e + j] * p.scale : 0.0f; };
+            const auto value = [&](int j) { return alive ? dq[d][e + j] * scaled.down() * p.scale : 0.0f; };
             store4<T>(out + at, value(0), value(1), value(2), value(3));
         }
 }
@@ -224,7 +273,7 @@ __global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) voi
     __shared__ __attribute__((aligned(1024))) char d0s[Rows::kBytes];
     __shared__ __attribute__((aligned(1024))) char q1s[Rows::kBytes];
     __shared__ __attribute__((aligned(1024))) char d1s[Rows::kBytes];
-    // -l log2 e and D of the tiles' rows (64 of each, whatever BQ)
+    // bias and D of the tiles' rows (64 of each, whatever BQ)
     __shared__ __attribute__((aligned(1024))) float l0s[2 * kWave];
     __shared__ __attribute__((aligned(1024))) float l1s[2 * kWave];
 
@@ -255,6 +304,7 @@ __global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) voi
     f32x16 dk[DT], dv[DT];
 #pragma unroll
     for (int d = 0; d < DT; ++d) dk[d] = dv[d] = zeros();
+    ColumnScale<T> scaled;
     if (from < to) {
         auto keep = [&](int i) { return i >= seq.first && i < seq.end; };
         typename Rows::Loads q_loads, d_loads;
@@ -369,6 +419,7 @@ __global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) voi
                         if (behind >= limit) s[e] = ds[e] = 0.0f;
                     }
                 }
+                scaled.apply(ds, dk);
 #pragma unroll
                 for (int f = 0; f < kFragsOf32<T>; ++f) {
                     const uint4 pf = pack_rows<T>(s, f), sf = pack_rows<T>(ds, f);
@@ -387,6 +438,17 @@ __global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) voi
         }
     }
     if (mine >= p.s.keys) return;
+    if constexpr (ColumnScale<T>::kOn) {
+        constexpr float kDown = 1.0f / (1 << kProbabilityBits<T>);
+        const float down = scaled.down() * kDown;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                dk[d][e] *= down;
+                dv[d][e] *= kDown;
+            }
+    }
     if (parts > 1) {
         float* sums = p.part + ((static_cast<int64_t>(bh) * per_head + slot) * 2 * RB + wave * 32 + l32) * p.s.dim;
 #pragma unroll

@@ -8,7 +8,7 @@ it is derived beside the test.
 import numpy as np
 import pytest
 
-from _attention import BF16, F16, F32, Attention, assert_within, put, sample, wide
+from _attention import BF16, F16, F32, HALF, TINY, Attention, assert_within, put, sample, wide
 from oracle import binding as orc
 
 pytestmark = pytest.mark.gpu
@@ -61,3 +61,89 @@ def test_keys_that_are_nan(dev, ops, dtype, tq, tk, first, count):
     assert_within(out.numpy(), want, a.tokens(a.out_bound), dtype, "out")
     struck = struck.transpose(0, 2, 1)
     assert_within(lse.numpy(), np.where(struck, np.nan, a.lse), a.lse_bound, F32, "lse")
+
+
+# ---- gradients of every size in float16 -----------------------------------------
+
+
+def close_bounds(a, do, dtype):
+    """The backward's results and bounds of an ``Attention`` whose dS and P are
+    scaled by powers of two before they are rounded to 16 bits: of dS in a sum
+    the largest so far lies at 2^7 or above, so that an element is off by half a
+    step, relative, and by 2^-25, half of float16's smallest step, over 2^7 of
+    the sum's largest; P is scaled by 2^12."""
+    want, bounds = a.backward(do, dtype)
+    if dtype != F16:
+        return want, bounds
+    do = np.where(~a.see.any(-1)[..., None], 0.0, do.transpose(0, 2, 1, 3))
+    dp = do @ a.v.swapaxes(-1, -2)
+    ds = np.abs(a.p * (dp - (do * a.out).sum(-1, keepdims=True)))
+    see = np.broadcast_to(a.see, a.p.shape)
+    t, k, q = TINY[F16], np.abs(a.k), np.abs(a.q)
+    row = ds.max(-1, keepdims=True) * 2.0 ** -7 - 1.0
+    # a key's sum runs over all query heads that share it
+    b, h, tq, tk = ds.shape
+    column = np.repeat(ds.reshape(b, h // a.group, -1, tk).max(2), a.group, 1)[:, :, None] * 2.0 ** -7 - 1.0
+    more = (a.tokens(a.scale * t * (row * see) @ k), a.shared(a.scale * t * (column * see).swapaxes(-1, -2) @ q),
+            a.shared(t * (2.0 ** -12 - 1.0) * see.swapaxes(-1, -2) @ np.abs(do)))
+    return want, tuple(x + y for x, y in zip(bounds, more))
+
+
+@pytest.mark.parametrize("shape", [(1, 512, 512, 2, 1, 128), (1, 200, 200, 256, 256, 64), (1, 130, 700, 64, 32, 96), (1, 300, 300, 6, 2, 32)], ids=str)
+@pytest.mark.parametrize("size", [1e-5, 1e-4, 1e-3, 1.0, 300.0, 8000.0])
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS[1:])
+def test_gradients_of_every_size(dev, ops, dtype, size, shape):
+    """dS as large as the gradients passes float16's range, and as small falls
+    among its subnormals: neither shows in dq, dk or dv."""
+    host = make(dtype, *shape, 30)
+    # (large ones beside small queries and keys, so that the results stay in range)
+    for i, by in enumerate((0.25, 0.25, 2.0, size) if size > 1000 else (1.0, 1.0, 1.0, size)):
+        host[i] = orc.from_float((wide(host[i], dtype) * by).astype(np.float32), dtype)
+    w = [wide(x, dtype) for x in host]
+    a = Attention(dtype, *w[:3], window=250, sinks=2)
+    want, bounds = close_bounds(a, w[3], dtype)
+    assert all(np.abs(x).max() < 6e4 for x in want), "the results themselves have to be in range"
+    q, k, v, do = (put(x, dtype) for x in host)
+    out, lse = ops.sliding_window_attention(q, k, v, 250, 2)
+    for g, x, bound, name in zip(ops.sliding_window_attention_backward(do, q, k, v, out, lse, 250, 2), want, bounds, ("dq", "dk", "dv")):
+        assert_within(g.numpy(), x, bound, dtype, name)
+
+
+@pytest.mark.parametrize("down", [False, True], ids=["growing", "shrinking"])
+@pytest.mark.parametrize("shape", [(1, 400, 400, 2, 1, 64), (1, 200, 200, 256, 256, 64)], ids=str)
+def test_gradients_that_change_size_along_a_sum(dev, ops, shape, down):
+    """Values grow by 2^20 along the keys and the gradients along the queries:
+    the scale of a sum's dS is left again and again."""
+    host = make(F16, *shape, 40)
+    for i in (2, 3):
+        grow = 2.0 ** np.linspace(-14 + 2 * i, 2 + 2 * i, host[i].shape[1])[:: -1 if down else 1]
+        host[i] = orc.from_float((wide(host[i], F16) * grow[:, None, None]).astype(np.float32), F16)
+    w = [wide(x, F16) for x in host]
+    a = Attention(F16, *w[:3])
+    want, bounds = close_bounds(a, w[3], F16)
+    assert all(np.abs(x).max() < 6e4 for x in want), "the results themselves have to be in range"
+    q, k, v, do = (put(x, F16) for x in host)
+    out, lse = ops.sliding_window_attention(q, k, v)
+    for g, x, bound, name in zip(ops.sliding_window_attention_backward(do, q, k, v, out, lse), want, bounds, ("dq", "dk", "dv")):
+        assert_within(g.numpy(), x, bound, F16, name)
+
+
+def test_dv_of_small_probabilities(dev, ops):
+    """302292 keys of one score: each probability lies midway between two of
+    float16's subnormals.  With keys of zero every sum of exponentials is a
+    whole number under 2^24 and exact; l = ln n is off by 2 u of itself, its
+    product with log2 e by 2 u more and the power by 4 u: under 2^-18 of P
+    together.  A sum of 8 heads' and queries' terms adds 2^-20."""
+    tk, tq, heads, kv, d = 302292, 4, 2, 1, 8
+    q, k, v, do = make(F16, 1, tq, tk, heads, kv, d, 50)
+    k[:] = 0
+    do = orc.from_float(np.sign(wide(do, F16)).astype(np.float32) * 512 + np.abs(wide(do, F16)).astype(np.float32), F16)
+    dq_, dk_, dv_, ddo = (put(x, F16) for x in (q, k, v, do))
+    out, lse = ops.sliding_window_attention(dq_, dk_, dv_)
+    dv = ops.sliding_window_attention_backward(ddo, dq_, dk_, dv_, out, lse)[2].numpy()
+    n = tk - tq + 1 + np.arange(tq)
+    terms = (wide(do, F16)[0] / n[:, None, None]).reshape(tq, kv, heads // kv, d).sum(2)
+    want = np.cumsum(terms[::-1], 0)[::-1]  # key tk - tq + i: by queries i and on
+    want = np.concatenate([np.broadcast_to(want[:1], (tk - tq + 1, kv, d)), want[1:]])
+    size = np.abs(wide(do, F16)[0] / n[:, None, None]).reshape(tq, kv, heads // kv, d).sum((0, 2))
+    assert_within(dv[0], want, (HALF[F16] + 2.0 ** -17) * size, F16, "dv")
