@@ -136,6 +136,7 @@ __global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4)
 #pragma unroll
     for (int d = 0; d < DT; ++d) dq[d] = zeros();
     ColumnScale<T> scaled;
+    float bias = 0.0f;
     if (b0 <= b1) {
         const int p0 = seq.start + b0, p1 = seq.start + b1;
         const KeyTiles tiles(p.s.rule, p0, p1, BK);
@@ -175,9 +176,9 @@ __global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4)
         }
         delta = both_halves(delta, SumOf{});
         const int64_t stat = (static_cast<int64_t>(b) * p.s.heads + h) * p.s.queries + mine;
-        float bias = 0.0f;
         if (alive) {
-            // (a row whose sum is 0 has no probabilities, whatever its scores)
+            // (a row whose sum is 0 has no probabilities, whatever its scores:
+            // dk and dv have them as powers of -inf, and D as 0)
             const float l = p.lse[stat];
             bias = l == -INFINITY ? -INFINITY : -l * kLog2E;
         }
@@ -242,11 +243,14 @@ __global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4)
         }
         if (alive && half == 0) {
             p.bias[stat] = bias + kProbabilityBits<T>;
-            p.delta[stat] = delta;
+            p.delta[stat] = bias == -INFINITY ? 0.0f : delta;
         }
         walk(std::true_type{});
     }
     if (mine >= p.s.queries) return;
+    // A row that is outside its sequence or has no sum, beside keys and values
+    // that may be infinite: zeros by selection.
+    const bool any = alive && bias != -INFINITY;
     S* out = static_cast<S*>(p.dq) + ((static_cast<int64_t>(b) * p.s.queries + mine) * p.s.heads + h) * p.s.dim;
 #pragma unroll
     for (int d = 0; d < DT; ++d)
@@ -254,7 +258,7 @@ __global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4)
         for (int e = 0; e < 16; e += 4) {
             const int at = 32 * d + row_of(e, half);
             if (at >= p.s.dim) continue;
-            const auto value = [&](int j) { return alive ? dq[d][e + j] * scaled.down() * p.scale : 0.0f; };
+            const auto value = [&](int j) { return any ? dq[d][e + j] * scaled.down() * p.scale : 0.0f; };
             store4<T>(out + at, value(0), value(1), value(2), value(3));
         }
 }

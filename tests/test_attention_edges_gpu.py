@@ -147,3 +147,53 @@ def test_dv_of_small_probabilities(dev, ops):
     want = np.concatenate([np.broadcast_to(want[:1], (tk - tq + 1, kv, d)), want[1:]])
     size = np.abs(wide(do, F16)[0] / n[:, None, None]).reshape(tq, kv, heads // kv, d).sum((0, 2))
     assert_within(dv[0], want, (HALF[F16] + 2.0 ** -17) * size, F16, "dv")
+
+
+# ---- rows without a sum -----------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("tq,heads,kv", [(1, 1, 1), (200, 1, 1), (200, 128, 64)])
+def test_rows_whose_scores_are_minus_infinity(dev, ops, dtype, tq, heads, kv):
+    """Sequence 0's keys give every score -inf: zeros, an l of -inf and
+    gradients of zero, and sequence 1 is as ever."""
+    host = make(dtype, 2, tq, 200, heads, kv, 16, 60)
+    host[0][:, :, :, 3] = one(1.0, dtype)
+    w = [wide(x, dtype) for x in host]
+    a = Attention(dtype, *w[:3])
+    want, bounds = a.backward(w[3], dtype)
+    host[1][0, :, :, 3] = one(-np.inf, dtype)
+    q, k, v, do = (put(x, dtype) for x in host)
+    out, lse = ops.sliding_window_attention(q, k, v)
+    grads = ops.sliding_window_attention_backward(do, q, k, v, out, lse)
+    assert (wide(out.numpy(), dtype)[0] == 0).all() and (lse.numpy()[0] == -np.inf).all()
+    for g, x, bound, name in zip(grads, want, bounds, ("dq", "dk", "dv")):
+        x, bound = x.copy(), bound.copy()
+        x[0] = bound[0] = 0.0
+        assert_within(g.numpy(), x, bound, dtype, name)
+        assert (wide(g.numpy(), dtype)[0] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("heads,kv", [(1, 1), (256, 128)])
+@pytest.mark.parametrize("where", ["out"])
+def test_rows_given_as_without_a_sum(dev, ops, dtype, heads, kv, where):
+    """A query whose l is handed in as -inf has no gradient and takes no part
+    in the keys', whatever it, its result and its gradient hold."""
+    host = make(dtype, 1, 150, 150, heads, kv, 32, 65)
+    q, k, v, do = (put(x, dtype) for x in host)
+    out, lse = ops.sliding_window_attention(q, k, v, 60, 1)
+    o, l = out.numpy().copy(), lse.numpy().copy()
+    without = [0, 70, 71, 149]
+    l[:, :, without] = -np.inf
+    clean = [x.numpy() for x in ops.sliding_window_attention_backward(do, q, k, v, put(o, dtype), put(l), 60, 1)]
+    for x in clean:
+        assert np.isfinite(wide(x, dtype)).all()
+    assert (wide(clean[0], dtype)[:, without] == 0).all()
+    struck = {"query": host[0], "gradient": host[3], "out": o}[where]
+    struck[:, without] = one(np.inf, dtype)
+    struck[:, without[1]] = one(np.nan, dtype)
+    q, do = put(host[0], dtype), put(host[3], dtype)
+    for x, y in zip(ops.sliding_window_attention_backward(do, q, k, v, put(o, dtype), put(l), 60, 1), clean):
+        # the rows' part is summed in another order where it is left out
+        assert_within(x.numpy(), wide(y, dtype), 2.0 ** -7 * np.abs(wide(y, dtype)).max(), dtype)
