@@ -56,10 +56,14 @@ struct Backward {
     int blocks;           // of 32 W queries (dq) or keys (dk, dv) a head
     int pairs;            // batch x key heads
     // dk, dv: the first sink_blocks blocks of a head walk in sink_parts parts,
-    // the others in near_parts; parts of more than one leave float32 sums.
+    // the others in near_parts; parts of more than one leave float32 sums, the
+    // first tokens' before the others'.
     int sink_blocks, sink_parts, near_parts;
-    float* part;  // [head][part][2][rows][dim]
-    int per_head() const { return sink_blocks * sink_parts + (blocks - sink_blocks) * near_parts; }
+    float* part;  // [head][part that leaves sums][2][rows][dim]
+    __host__ __device__ int sink_slots() const { return sink_blocks * sink_parts; }
+    __host__ __device__ int near_slots() const { return (blocks - sink_blocks) * near_parts; }
+    __host__ __device__ int sums_of_sinks() const { return sink_parts > 1 ? sink_slots() : 0; }
+    __host__ __device__ int sums() const { return sums_of_sinks() + (near_parts > 1 ? near_slots() : 0); }
 };
 
 // P is rounded at this power of two times its size.  float16 is full down to
@@ -281,12 +285,11 @@ __global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) voi
     __shared__ __attribute__((aligned(1024))) float l0s[2 * kWave];
     __shared__ __attribute__((aligned(1024))) float l1s[2 * kWave];
 
-    const int per_head = p.sink_blocks * p.sink_parts + (p.blocks - p.sink_blocks) * p.near_parts;
     const int bh = blockIdx.x % p.pairs, slot = blockIdx.x / p.pairs;
     const int hk = bh % p.s.kv_heads, b = bh / p.s.kv_heads;
-    const bool sink = slot < p.sink_blocks * p.sink_parts;
+    const bool sink = slot < p.sink_slots();
     const int parts = sink ? p.sink_parts : p.near_parts;
-    const int local = sink ? slot : slot - p.sink_blocks * p.sink_parts;
+    const int local = sink ? slot : slot - p.sink_slots();
     const int kb = (sink ? 0 : p.sink_blocks) + local / parts, part = local % parts;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave, l32 = lane % 32, half = lane / 32;
@@ -454,7 +457,8 @@ __global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) voi
             }
     }
     if (parts > 1) {
-        float* sums = p.part + ((static_cast<int64_t>(bh) * per_head + slot) * 2 * RB + wave * 32 + l32) * p.s.dim;
+        const int64_t at_part = static_cast<int64_t>(bh) * p.sums() + local + (sink ? 0 : p.sums_of_sinks());
+        float* sums = p.part + (at_part * 2 * RB + wave * 32 + l32) * p.s.dim;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -486,16 +490,15 @@ constexpr int kJoin = 256;
 
 template <typename T, int RB>
 __global__ __launch_bounds__(kJoin) void attention_join_kernel(Backward p, int first) {
-    const int per_head = p.sink_blocks * p.sink_parts + (p.blocks - p.sink_blocks) * p.near_parts;
     const int kb = first + blockIdx.y, bh = blockIdx.z;
     const int hk = bh % p.s.kv_heads, b = bh / p.s.kv_heads;
     const bool sink = kb < p.sink_blocks;
     const int parts = sink ? p.sink_parts : p.near_parts;
-    const int slot = sink ? kb * p.sink_parts : p.sink_blocks * p.sink_parts + (kb - p.sink_blocks) * p.near_parts;
+    const int slot = sink ? kb * p.sink_parts : p.sums_of_sinks() + (kb - p.sink_blocks) * p.near_parts;
     const int quads = p.s.dim / 4, at = blockIdx.x * kJoin + threadIdx.x;
     const int which = at / (RB * quads), row = at / quads % RB, d = at % quads * 4;
     if (which > 1 || kb * RB + row >= p.s.keys) return;
-    const float* from = p.part + (((static_cast<int64_t>(bh) * per_head + slot) * 2 + which) * RB + row) * p.s.dim + d;
+    const float* from = p.part + (((static_cast<int64_t>(bh) * p.sums() + slot) * 2 + which) * RB + row) * p.s.dim + d;
     float4 t = *reinterpret_cast<const float4*>(from);
 #pragma unroll 4
     for (int i = 1; i < parts; ++i) {
@@ -539,10 +542,10 @@ void dkv_blocks(Backward p, const AttentionArgs& a, int device, hipStream_t on) 
     const int64_t even = sink * pairs * p.sink_blocks / want;
     const int64_t piece = std::max({int64_t{4}, even / 4, near_blocks == 0 ? even : near / p.near_parts});
     p.sink_parts = p.sink_blocks == 0 ? 1 : static_cast<int>(std::max<int64_t>(1, (sink + piece - 1) / piece));
-    const int64_t items = pairs * p.per_head();
+    const int64_t items = pairs * (p.sink_slots() + p.near_slots());
     const unsigned grid = grid_of(items, W * kWave, "sliding_window_attention_backward");
-    const bool cut = p.near_parts > 1 || p.sink_parts > 1;
-    const Workspace part(cut ? static_cast<size_t>(items) * 2 * RB * a.dim * sizeof(float) : 0, device);
+    const bool cut = p.sums() > 0;
+    const Workspace part(static_cast<size_t>(pairs * p.sums()) * 2 * RB * a.dim * sizeof(float), device);
     p.part = static_cast<float*>(part.get());
     attention_dkv_kernel<T, DT, R, W><<<grid, W * kWave, 0, on>>>(p);
     TP_AMD_HIP_CHECK(hipGetLastError());

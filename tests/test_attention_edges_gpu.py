@@ -8,7 +8,7 @@ it is derived beside the test.
 import numpy as np
 import pytest
 
-from _attention import BF16, F16, F32, HALF, TINY, Attention, assert_within, put, sample, wide
+from _attention import BF16, F16, F32, HALF, TINY, Attention, assert_within, mod, put, sample, wide
 from oracle import binding as orc
 
 pytestmark = pytest.mark.gpu
@@ -197,3 +197,56 @@ def test_rows_given_as_without_a_sum(dev, ops, dtype, heads, kv, where):
     for x, y in zip(ops.sliding_window_attention_backward(do, q, k, v, put(o, dtype), put(l), 60, 1), clean):
         # the rows' part is summed in another order where it is left out
         assert_within(x.numpy(), wide(y, dtype), 2.0 ** -7 * np.abs(wide(y, dtype)).max(), dtype)
+
+
+# ---- memory of the parts ------------------------------------------------------------
+
+
+def test_sums_of_few_first_tokens_beside_many_keys(dev, ops):
+    """Only the first tokens' walks are cut: the keys behind them write their
+    gradients themselves and have no room among the parts."""
+    runtime = mod("runtime")
+    t, h, d, window, sinks = 16384, 8, 64, 256, 4
+    q, k, v, do = (put(x, BF16) for x in make(BF16, 1, t, t, h, h, d, 70))
+    out, lse = ops.sliding_window_attention(q, k, v, window, sinks)
+    runtime.synchronize()
+    runtime.reset_peak_memory_stats()
+    before = runtime.memory_allocated()
+    grads = ops.sliding_window_attention_backward(do, q, k, v, out, lse, window, sinks)
+    runtime.synchronize()
+    # a block of 128 keys walks 64 queries a step: the first block all of
+    # them, in parts no shorter than the others' walk of at least 6 steps
+    parts = h * (t // 64 // 6 + 1)
+    bound = parts * 2 * 128 * d * 4 + 3 * t * h * d * 2 + 2 * t * h * 4
+    assert runtime.max_memory_allocated() - before <= 1.1 * bound
+    # head 3 against float64, a run of keys at either end
+    w = [wide(x.numpy(), BF16)[:, :, 3:4] for x in (q, k, v, do)]
+    n = 700
+    for cut in (slice(0, n), slice(t - n, t)):
+        if cut.start == 0:
+            continue
+        low = t - n - window
+        part = [np.concatenate([x[:, :sinks], x[:, low:]], 1) for x in w[1:3]]
+        a = Attention(BF16, w[0][:, low + window:], *part, window=window, sinks=sinks)
+        want, bounds = a.backward(w[3][:, low + window:], BF16)
+        assert_within(grads[0].numpy()[:, t - n:, 3:4], want[0], bounds[0], BF16, "dq")
+        for i, name in ((1, "dk"), (2, "dv")):
+            last = n - window  # keys whose queries are all among these
+            assert_within(grads[i].numpy()[:, t - last:, 3:4], want[i][:, -last:], bounds[i][:, -last:], BF16, name)
+
+
+@pytest.mark.parametrize("heads,sinks,window", [(256, 2048, 600), (8, 300, 900), (40, 130, 40)])
+def test_which_walks_are_cut(dev, ops, heads, sinks, window):
+    """The first tokens' walks, the others', both: the heads are all one, and
+    each has the gradients that float64 gives it."""
+    t, d = 2176, 8
+    host = make(F32, 1, t, t, 1, 1, d, 75)
+    w = [wide(x, F32) for x in host]
+    a = Attention(F32, *w[:3], window=window, sinks=sinks)
+    want, bounds = a.backward(w[3], F32)
+    q, k, v, do = (put(x).expand(1, t, heads, d) for x in host)
+    out, lse = ops.sliding_window_attention(q, k, v, window, sinks)
+    for g, x, bound, name in zip(ops.sliding_window_attention_backward(do, q, k, v, out, lse, window, sinks), want, bounds, ("dq", "dk", "dv")):
+        g = g.numpy()
+        assert (g == g[:, :, :1]).all(), name
+        assert_within(g[:, :, :1], x, bound, F32, name)
