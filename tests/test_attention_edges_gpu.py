@@ -8,7 +8,7 @@ it is derived beside the test.
 import numpy as np
 import pytest
 
-from _attention import BF16, F16, F32, HALF, TINY, Attention, assert_within, mod, put, sample, wide
+from _attention import BF16, F16, F32, FLUSH, HALF, TINY, U, Attention, assert_within, mod, put, sample, wide
 from oracle import binding as orc
 
 pytestmark = pytest.mark.gpu
@@ -250,3 +250,51 @@ def test_which_walks_are_cut(dev, ops, heads, sinks, window):
         g = g.numpy()
         assert (g == g[:, :, :1]).all(), name
         assert_within(g[:, :, :1], x, bound, F32, name)
+
+
+# ---- D of rows that see few keys ------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=IDS[1:])
+@pytest.mark.parametrize("shape,rule", [
+    ((1, 500, 500, 2, 1, 64), dict(window=16)),
+    ((1, 500, 500, 2, 2, 128), dict(window=100, sinks=28)),
+    ((2, 300, 300, 32, 16, 32), dict(window=33, sinks=3)),
+    ((1, 500, 500, 2, 1, 64), dict(window=0, sinks=128)),
+    ((1, 128, 128, 3, 3, 64), dict()),
+], ids=str)
+def test_gradients_of_rows_that_see_few_keys(dev, ops, dtype, shape, rule):
+    """Values far from zero: D = do . out with out rounded to 16 bits is off by
+    more than what dP - D leaves of it.  Rows of at most 128 keys have it as the
+    sum of P dP, off by eps of P and by dP's own error: the bound here has no
+    rounding of out in it.  (The closer bound of dP - D takes half a step of the
+    difference, not of its two parts.)"""
+    host = make(dtype, *shape, 80)
+    host[2] = orc.from_float((wide(host[2], dtype) + 50.0).astype(np.float32), dtype)
+    w = [wide(x, dtype) for x in host]
+    a = Attention(dtype, *w[:3], **rule)
+    want, _ = a.backward(w[3], dtype)
+    do = w[3].transpose(0, 2, 1, 3)
+    d, n = do.shape[-1], a.see.sum(-1, keepdims=True)
+    assert n.max() <= 128
+    eps = a.eps + a.lse_bound[..., None] + n * U
+    dp = do @ a.v.swapaxes(-1, -2)
+    e_dp = (d + 8) * U * (np.abs(do) @ np.abs(a.v).swapaxes(-1, -2))
+    delta = (a.p * dp).sum(-1, keepdims=True)
+    e_delta = (a.p * (np.abs(dp) * (2 * eps + n * U) + e_dp)).sum(-1, keepdims=True)
+    off = a.p * (np.abs(dp - delta) * (a.h + 2 * eps) + e_dp + e_delta) * (1 + a.h)
+    off = off + FLUSH * a.see * (1 + np.abs(dp) + np.abs(delta))
+    if dtype == F16:  # half of the smallest step, at a scale that leaves the sum's largest at 2^7 or above
+        ds = np.abs(a.p * (dp - delta))
+        b, h, tq, tk = ds.shape
+        column = np.repeat(ds.reshape(b, h // a.group, -1, tk).max(2), a.group, 1)[:, :, None]
+        off = off + TINY[F16] * 2.0 ** -7 * a.see * np.maximum(ds.max(-1, keepdims=True), column)
+    # the sums over a row's keys, and over the queries and heads a key has
+    sums = (2 * n.max() * a.group + 400) * U
+    bq = a.scale * ((off + sums * np.abs(a.p * (dp - delta))) @ np.abs(a.k))
+    bk = a.scale * ((off + sums * np.abs(a.p * (dp - delta))).swapaxes(-1, -2) @ np.abs(a.q))
+    q, k, v, g = (put(x, dtype) for x in host)
+    out, lse = ops.sliding_window_attention(q, k, v, **rule)
+    dq, dk, _ = ops.sliding_window_attention_backward(g, q, k, v, out, lse, **rule)
+    assert_within(dq.numpy(), want[0], a.tokens(bq), dtype, "dq")
+    assert_within(dk.numpy(), want[1], a.shared(bk), dtype, "dk")
