@@ -265,10 +265,10 @@ int tp_amd_qk_norm_rope_backward(const tp_amd_tensor* grad_query, const tp_amd_t
  *   starts [B] (NULL: lengths[b] - Tq): the position of query 0 of sequence b.
  * Query i stands at p = starts[b] + i and sees key j if j <= p and
  * (j > p - window or j < sinks); window < 0 is none.  A query outside
- * 0 <= p < lengths[b] is not read; it, and one that sees no key, gives a row of
- * zeros and an lse of -inf.  Of the other keys a block of
- * neighbouring queries reads those that some query of it sees, so a value that is not
- * finite reaches queries of its block that do not see it, and no others.
+ * 0 <= p < lengths[b] is not used; it, and one that sees no key (or whose every
+ * score is -inf), gives a row of zeros and an lse of -inf.  A key or value that is
+ * not finite reaches the queries that see it and no others; where blocks of
+ * neighbouring queries hold one the call is slower.
  * out [B, Tq, Hq, D] = softmax(scale q.k) v and float32 lse [B, Hq, Tq], the
  * natural logarithm of each row's sum of exponentials; scale > 0.  Scores,
  * statistics and sums are float32, probabilities are rounded to the
@@ -279,9 +279,8 @@ int tp_amd_sliding_window_attention(const tp_amd_tensor* query, const tp_amd_ten
 /* sliding_window_attention_backward: dquery, dkey and dvalue from the
  * forward's operands and results.  Key heads' gradients sum over their query
  * heads; rows of queries and keys outside their sequence get zeros, as does a
- * query whose lse is -inf.  Rows outside a sequence are not read; a value that
- * is not finite reaches its block's neighbours as in the forward.  Sums in a
- * fixed order, float32; the probabilities P and dS = P (dP - D) are rounded to
+ * query whose lse is -inf.  Rows outside a sequence are not used, and what is not
+ * finite reaches those that see it, as in the forward.  Sums in a fixed order, float32; the probabilities P and dS = P (dP - D) are rounded to
  * the operands' dtype, in float16 at a power of two times their size, so that
  * gradients of any size that dtype holds keep its precision. */
 int tp_amd_sliding_window_attention_backward(const tp_amd_tensor* grad_out, const tp_amd_tensor* query, const tp_amd_tensor* key,

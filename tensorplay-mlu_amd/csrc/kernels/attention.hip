@@ -111,6 +111,41 @@ __device__ __forceinline__ void finish4(const Forward& p, int64_t b, int i, int 
     store4<T>(out, value(0), value(1), value(2), value(3));
 }
 
+// Rows of `out` that hold a NaN and are `bad`, each lane's its own (query i of
+// head h at position `row`): see "sums again".
+template <typename T>
+__device__ __attribute__((noinline)) void rows_again(const Forward* launched, int b_, int hk_, int p0, int p1, bool bad, int i, int h, int row) {
+    const int b = shared_by_lanes(b_), hk = shared_by_lanes(hk_);
+    const Forward& p = as_launched(launched);
+    const S_<T>* kh = static_cast<const S_<T>*>(p.k.data) + b * p.k.batch + hk * p.k.head;
+    const S_<T>* vh = static_cast<const S_<T>*>(p.v.data) + b * p.v.batch + hk * p.v.head;
+    for_each_question(only_beside<T>(p.s, vh, p.v.token, shared_by_lanes(p0), shared_by_lanes(p1), bad, row), [&](int lane) __attribute__((always_inline)) {
+        const int iu = __builtin_amdgcn_readlane(i, lane), hu = __builtin_amdgcn_readlane(h, lane);
+        const S_<T>* q = static_cast<const S_<T>*>(p.q.data) + b * p.q.batch + iu * p.q.token + hu * p.q.head;
+        Two o{0.0f, 0.0f};
+        float m = -INFINITY, t = 0.0f;  // t: this lane's share
+        for_seen(p.s.rule, __builtin_amdgcn_readlane(row, lane), [&](int j0, uint64_t seen) __attribute__((always_inline)) {
+            const int mine = threadIdx.x % kWave;
+            const float s = seen >> mine & 1 ? row_product<T>(q, kh + (j0 + mine) * p.k.token, p.s.dim) * p.scale : -INFINITY;
+            const float now = fmaxf(m, over_wave(s, MaxOf{}));
+            if (now == -INFINITY) return;
+            const float turn = __builtin_amdgcn_exp2f(m - now), weight = __builtin_amdgcn_exp2f(s - now);
+            m = now;
+            t = fmaf(t, turn, weight);
+            o.x *= turn;
+            o.y *= turn;
+            add_rows<T>(o, weight, vh + j0 * p.v.token, p.v.token, seen, p.s.dim);
+        });
+        const float inv = 1.0f / over_wave(t, SumOf{});
+        S_<T>* out = static_cast<S_<T>*>(p.out) + ((static_cast<int64_t>(b) * p.s.queries + iu) * p.s.heads + hu) * p.s.dim;
+        store_two<T>(out, p.s.dim, Two{o.x * inv, o.y * inv});
+        return i == iu && h == hu;
+    });
+}
+
+// Whether a row's NaN (if `nan`) is none that its sum has too.
+__device__ __forceinline__ bool unexplained(bool nan, float t) { return nan && t > 0.0f && finite(t); }
+
 // A block of four waves owns 128 queries of a head, a wave 32 of them: scores
 // are formed transposed, S^T = K Q^T, so that a lane's column is its query, the
 // statistics are the lane's own and the probabilities are the next product's
@@ -223,8 +258,10 @@ __global__ __launch_bounds__(kWide* kWave, sizeof(S_<T>) == 4 && DT == 4 ? 1 : 2
             step(i + 1, k1s, v1s, k0s, v0s);
         }
     }
-    if (mine >= p.s.queries) return;
-    finish_row<T, DT>(p, b, h, mine, half, alive, col.m, both_halves(col.t, SumOf{}), col);
+    const float t = both_halves(col.t, SumOf{});
+    if (mine < p.s.queries) finish_row<T, DT>(p, b, h, mine, half, alive, col.m, t, col);
+    const bool bad = unexplained(alive && holds_nan(col.o), t);
+    if (__any(bad)) rows_again<T>(launched_with<Forward>(), b, hk, seq.start + b0, seq.start + b1, bad, mine, h, row);
 }
 
 // ---- few queries over many keys -------------------------------------------------
@@ -418,6 +455,20 @@ __global__ __launch_bounds__((kSplitWaves<T, DT> * kWave), 1) void attention_spl
     }
     __syncthreads();
     const int quads = p.s.dim / 4, rows_here = packed_end - rt * 32;
+    unsigned odd = 0;  // the rounds of the threads in which this one finished a row with a NaN
+    auto finish = [&](int at, int r, int quad, float m, float total, const float (&o)[4]) __attribute__((always_inline)) {
+        const int packed_r = rt * 32 + r, i = fastdiv(packed_r, q.by_group);
+        finish4<T>(p, b, i, hk * p.s.group + packed_r - i * p.s.group, 4 * quad, m, total, o);
+        const float x = (o[0] + o[1]) + (o[2] + o[3]);
+        if (unexplained(x != x, total)) odd |= 1u << at / (W * kWave);
+    };
+    auto again = [&]() __attribute__((always_inline)) {
+        for (int k = 0; __any(odd >> k); ++k) {
+            const int packed_r = rt * 32 + (k * W * kWave + static_cast<int>(threadIdx.x)) / (DT * 8), i = fastdiv(packed_r, q.by_group);
+            rows_again<T>(&launched_with<Split>()->f, b, hk, seq.start + b0, seq.start + b1, odd >> k & 1, i,
+                          hk * p.s.group + packed_r - i * p.s.group, seq.start + i);
+        }
+    };
     float* const stat = q.stat + (static_cast<int64_t>(tile) * q.splits + split) * q.tile_rows * 2;
     for (int at = threadIdx.x; at < rows_here * DT * 8; at += W * kWave) {
         const int r = at / (DT * 8), quad = at % (DT * 8);
@@ -432,8 +483,7 @@ __global__ __launch_bounds__((kSplitWaves<T, DT> * kWave), 1) void attention_spl
             add_state(ms[w][r], ts[w][r], x, m, total, o);
         }
         if (q.splits == 1) {
-            const int packed_r = rt * 32 + r, i = fastdiv(packed_r, q.by_group);
-            finish4<T>(p, b, i, hk * p.s.group + packed_r - i * p.s.group, 4 * quad, m, total, o);
+            finish(at, r, quad, m, total, o);
             continue;
         }
         if (quad == 0) store_shared(stat + 2 * r, m, total);
@@ -441,7 +491,7 @@ __global__ __launch_bounds__((kSplitWaves<T, DT> * kWave), 1) void attention_spl
         store_shared(part, o[0], o[1]);
         store_shared(part + 2, o[2], o[3]);
     }
-    if (q.splits == 1) return;
+    if (q.splits == 1) return again();
     __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -480,9 +530,9 @@ __global__ __launch_bounds__((kSplitWaves<T, DT> * kWave), 1) void attention_spl
                 add_state(x.x, x.y, make_float4(lo[k].x, lo[k].y, hi[k].x, hi[k].y), m, total, o);
             }
         }
-        const int packed_r = rt * 32 + r, i = fastdiv(packed_r, q.by_group);
-        finish4<T>(p, b, i, hk * p.s.group + packed_r - i * p.s.group, 4 * quad, m, total, o);
+        finish(at, r, quad, m, total, o);
     }
+    again();
 }
 
 Forward forward_of(const AttentionArgs& a) {

@@ -110,6 +110,145 @@ struct ColumnScale {
     __device__ __forceinline__ float down() const { return kOn ? __uint_as_float((254u << 23) - __float_as_uint(up)) : 1.0f; }
 };
 
+// Rows of dq that hold a NaN and are `bad`, each lane's its own (query i at
+// position `row`, with its bias and D): see "sums again".
+template <typename T>
+__device__ __attribute__((noinline)) void queries_again(const Backward* launched, int b_, int h_, int p0, int p1, bool bad, int i, int row,
+                                                        float bias, float delta) {
+    const Backward& p = as_launched(launched);
+    const int b = shared_by_lanes(b_), h = shared_by_lanes(h_), hk = h / p.s.group;
+    const S_<T>* kh = static_cast<const S_<T>*>(p.k.data) + b * p.k.batch + hk * p.k.head;
+    const S_<T>* vh = static_cast<const S_<T>*>(p.v.data) + b * p.v.batch + hk * p.v.head;
+    for_each_question(only_beside<T>(p.s, kh, p.k.token, shared_by_lanes(p0), shared_by_lanes(p1), bad, row), [&](int lane) __attribute__((always_inline)) {
+        const int iu = __builtin_amdgcn_readlane(i, lane);
+        const float bu = from_lane(bias, lane), du = from_lane(delta, lane);
+        const S_<T>* q = static_cast<const S_<T>*>(p.q.data) + b * p.q.batch + h * p.q.head + iu * p.q.token;
+        const S_<T>* g = static_cast<const S_<T>*>(p.dout.data) + b * p.dout.batch + h * p.dout.head + iu * p.dout.token;
+        Two o{0.0f, 0.0f};
+        for_seen(p.s.rule, __builtin_amdgcn_readlane(row, lane), [&](int j0, uint64_t seen) __attribute__((always_inline)) {
+            const int mine = threadIdx.x % kWave;
+            float ds = 0.0f;
+            if (seen >> mine & 1) {
+                const float s = row_product<T>(q, kh + (j0 + mine) * p.k.token, p.s.dim);
+                ds = __builtin_amdgcn_exp2f(fmaf(s, p.scale2, bu)) * (row_product<T>(g, vh + (j0 + mine) * p.v.token, p.s.dim) - du);
+            }
+            add_rows<T>(o, ds, kh + j0 * p.k.token, p.k.token, seen, p.s.dim);
+        });
+        S_<T>* out = static_cast<S_<T>*>(p.dq) + ((static_cast<int64_t>(b) * p.s.queries + iu) * p.s.heads + h) * p.s.dim;
+        store_two<T>(out, p.s.dim, Two{o.x * p.scale, o.y * p.scale});
+        return i == iu;
+    });
+}
+
+// What a block of dk and dv walks: keys kb RB .. last of a sequence, tiles
+// from .. to - 1 of BQ queries, per_query_head of them from tile t0 on of every
+// query head of the group.
+template <int BQ, int RB>
+struct KeyWalk {
+    int bh, hk, b, kb, parts;
+    int64_t at_part;  // of the parts' sums
+    Sequence seq;
+    int last, t0, per_query_head, from, to;
+    __device__ __forceinline__ explicit KeyWalk(const Backward& p) {
+        bh = blockIdx.x % p.pairs;
+        const int slot = blockIdx.x / p.pairs;
+        hk = bh % p.s.kv_heads, b = bh / p.s.kv_heads;
+        const bool sink = slot < p.sink_slots();
+        parts = sink ? p.sink_parts : p.near_parts;
+        const int local = sink ? slot : slot - p.sink_slots(), part = local % parts;
+        kb = (sink ? 0 : p.sink_blocks) + local / parts;
+        at_part = static_cast<int64_t>(bh) * p.sums() + local + (sink ? 0 : p.sums_of_sinks());
+        seq = sequence_of(p.s, b);
+        last = min(kb * RB + RB, seq.length) - 1;
+        // queries that see a key of the block: from the block's first key on, to
+        // the window's end behind its last one or, of first tokens, to the end
+        const int64_t reach = kb * RB < p.s.rule.sinks ? int64_t{kNoWindow} : int64_t{last} + p.s.rule.window - 1;
+        const int i0 = max(kb * RB - seq.start, seq.first);
+        const int i1 = static_cast<int>(min(reach - seq.start, static_cast<int64_t>(seq.end) - 1));
+        t0 = i0 / BQ;
+        per_query_head = last >= kb * RB && i0 <= i1 ? i1 / BQ - t0 + 1 : 0;
+        const int64_t all = static_cast<int64_t>(per_query_head) * p.s.group;
+        from = static_cast<int>(all * part / parts), to = static_cast<int>(all * (part + 1) / parts);
+    }
+};
+
+// Rows of dk and dv (or of a part's sums) that hold a NaN, where `bad`, each
+// lane's its own key: see "sums again".  A query without a sum counts as unseen,
+// whatever it holds.
+template <typename T, int BQ, int W>
+__device__ __attribute__((noinline)) void keys_again(const Backward* launched, bool bad) {
+    constexpr int RB = 32 * W;
+    const Backward& p = as_launched(launched);
+    const KeyWalk<BQ, RB> walk(p);
+    const int b = walk.b, hk = walk.hk, last = walk.last, from = walk.from, to = walk.to;
+    const Sequence& seq = walk.seq;
+    const int mine = walk.kb * RB + static_cast<int>(threadIdx.x / kWave * 32 + threadIdx.x % 32);
+    const S_<T>* kh = static_cast<const S_<T>*>(p.k.data) + b * p.k.batch + hk * p.k.head;
+    const S_<T>* vh = static_cast<const S_<T>*>(p.v.data) + b * p.v.batch + hk * p.v.head;
+    const S_<T>* qb = static_cast<const S_<T>*>(p.q.data) + b * p.q.batch;
+    const S_<T>* db = static_cast<const S_<T>*>(p.dout.data) + b * p.dout.batch;
+    const int lane_id = threadIdx.x % kWave;
+    // of tile `it`, f(query head, its statistics, its rows)
+    auto tile = [&](int it, const auto& f) __attribute__((always_inline)) {
+        const int h = hk * p.s.group + it / walk.per_query_head, r0 = (walk.t0 + it % walk.per_query_head) * BQ;
+        f(h, (static_cast<int64_t>(b) * p.s.heads + h) * p.s.queries, max(r0, seq.first), min(r0 + BQ, seq.end));
+    };
+    // a key that is not finite itself keeps what it has
+    bool beside = false;
+    if (bad && mine <= last) bad = row_is_finite<T>(kh + mine * p.k.token, p.s.dim) && row_is_finite<T>(vh + mine * p.v.token, p.s.dim);
+    for (int it = from; it < to && __any(bad); ++it) {
+        tile(it, [&](int h, int64_t stat, int i0, int i1) __attribute__((always_inline)) {
+            const int i = i0 + lane_id;
+            bool odd = false, none = false;
+            if (i < i1) {
+                const float bias = p.bias[stat + i];
+                none = bias == -INFINITY;
+                odd = bias != bias || !finite(p.delta[stat + i]) || !row_is_finite<T>(qb + h * p.q.head + i * p.q.token, p.s.dim) ||
+                      !row_is_finite<T>(db + h * p.dout.head + i * p.dout.token, p.s.dim);
+            }
+            const uint64_t without = __ballot(none);
+            for (uint64_t found = __ballot(odd); found != 0; found &= found - 1) {
+                const int at = __ffsll(static_cast<unsigned long long>(found)) - 1;
+                const bool sees = mine <= last && !(without >> at & 1) && p.s.rule.sees(seq.start + i0 + at, mine);
+                beside = beside || !sees;
+                bad = bad && !sees;
+            }
+        });
+    }
+    for_each_question(bad && beside, [&](int lane) __attribute__((always_inline)) {
+        const int key = __builtin_amdgcn_readlane(mine, lane);
+        const S_<T>*k = kh + key * p.k.token, *v = vh + key * p.v.token;
+        Two dk{0.0f, 0.0f}, dv{0.0f, 0.0f};
+        for (int it = from; it < to && key <= last; ++it) {
+            tile(it, [&](int h, int64_t stat, int i0, int i1) __attribute__((always_inline)) {
+                const int i = i0 + lane_id;
+                const S_<T>*q = qb + h * p.q.head + i0 * p.q.token, *g = db + h * p.dout.head + i0 * p.dout.token;
+                float pr = 0.0f, ds = 0.0f;
+                const float bias = i < i1 ? p.bias[stat + i] : -INFINITY;
+                const bool sees = bias != -INFINITY && p.s.rule.sees(seq.start + i, key);
+                const uint64_t seen = __ballot(sees);
+                if (seen == 0) return;
+                if (sees) {
+                    pr = __builtin_amdgcn_exp2f(fmaf(row_product<T>(q + lane_id * p.q.token, k, p.s.dim), p.scale2, bias - kProbabilityBits<T>));
+                    ds = pr * (row_product<T>(g + lane_id * p.dout.token, v, p.s.dim) - p.delta[stat + i]);
+                }
+                add_rows<T>(dk, ds, q, p.q.token, seen, p.s.dim);
+                add_rows<T>(dv, pr, g, p.dout.token, seen, p.s.dim);
+            });
+        }
+        if (walk.parts > 1) {
+            float* at = p.part + (walk.at_part * 2 * RB + key - walk.kb * RB) * p.s.dim;
+            store_two<float>(at, p.s.dim, dk);
+            store_two<float>(at + RB * p.s.dim, p.s.dim, dv);
+        } else {
+            const int64_t row = ((static_cast<int64_t>(b) * p.s.keys + key) * p.s.kv_heads + hk) * p.s.dim;
+            store_two<T>(static_cast<S_<T>*>(p.dk) + row, p.s.dim, Two{dk.x * p.scale, dk.y * p.scale});
+            store_two<T>(static_cast<S_<T>*>(p.dv) + row, p.s.dim, dv);
+        }
+        return mine == key;
+    });
+}
+
 template <typename T, int DT, int BK, int W>
 __global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4) ? 1 : 2) void attention_dq_kernel(Backward p) {
     using S = S_<T>;
@@ -140,7 +279,7 @@ __global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4)
 #pragma unroll
     for (int d = 0; d < DT; ++d) dq[d] = zeros();
     ColumnScale<T> scaled;
-    float bias = 0.0f;
+    float bias = 0.0f, delta = 0.0f;
     if (b0 <= b1) {
         const int p0 = seq.start + b0, p1 = seq.start + b1;
         const KeyTiles tiles(p.s.rule, p0, p1, BK);
@@ -158,7 +297,6 @@ __global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4)
         };
         if (tiles.count > 0) issue(0, k0s, v0s);
         uint4 qf[Keys::kSteps], df[Keys::kSteps];
-        float delta = 0.0f;
         {
             auto rows_of = [&](const TokenRows& t) {
                 const S* at = static_cast<const S*>(t.data) + b * t.batch + h * t.head + static_cast<int64_t>(qb * RB) * t.token;
@@ -253,20 +391,23 @@ __global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4)
         }
         walk(std::true_type{});
     }
-    if (mine >= p.s.queries) return;
     // A row that is outside its sequence or has no sum, beside keys and values
     // that may be infinite: zeros by selection.
     const bool any = alive && bias != -INFINITY;
-    S* out = static_cast<S*>(p.dq) + ((static_cast<int64_t>(b) * p.s.queries + mine) * p.s.heads + h) * p.s.dim;
+    if (mine < p.s.queries) {
+        S* out = static_cast<S*>(p.dq) + ((static_cast<int64_t>(b) * p.s.queries + mine) * p.s.heads + h) * p.s.dim;
 #pragma unroll
-    for (int d = 0; d < DT; ++d)
+        for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int at = 32 * d + row_of(e, half);
-            if (at >= p.s.dim) continue;
-            const auto value = [&](int j) { return any ? dq[d][e + j] * scaled.down() * p.scale : 0.0f; };
-            store4<T>(out + at, value(0), value(1), value(2), value(3));
-        }
+            for (int e = 0; e < 16; e += 4) {
+                const int at = 32 * d + row_of(e, half);
+                if (at >= p.s.dim) continue;
+                const auto value = [&](int j) { return any ? dq[d][e + j] * scaled.down() * p.scale : 0.0f; };
+                store4<T>(out + at, value(0), value(1), value(2), value(3));
+            }
+    }
+    const bool bad = any && holds_nan(dq) && finite(bias) && finite(delta);
+    if (__any(bad)) queries_again<T>(launched_with<Backward>(), b, h, seq.start + b0, seq.start + b1, bad, mine, row, bias, delta);
 }
 
 template <typename T, int DT, int BQ, int W>
@@ -287,28 +428,14 @@ __global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) voi
     __shared__ __attribute__((aligned(1024))) float l0s[2 * kWave];
     __shared__ __attribute__((aligned(1024))) float l1s[2 * kWave];
 
-    const int bh = blockIdx.x % p.pairs, slot = blockIdx.x / p.pairs;
-    const int hk = bh % p.s.kv_heads, b = bh / p.s.kv_heads;
-    const bool sink = slot < p.sink_slots();
-    const int parts = sink ? p.sink_parts : p.near_parts;
-    const int local = sink ? slot : slot - p.sink_slots();
-    const int kb = (sink ? 0 : p.sink_blocks) + local / parts, part = local % parts;
+    const KeyWalk<BQ, RB> walk(p);
+    const int b = walk.b, hk = walk.hk, kb = walk.kb, last = walk.last, t0 = walk.t0, per_query_head = walk.per_query_head;
+    const int from = walk.from, to = walk.to;
+    const Sequence& seq = walk.seq;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave, l32 = lane % 32, half = lane / 32;
-    const Sequence seq = sequence_of(p.s, b);
-
     const int mine = kb * RB + wave * 32 + l32;  // this lane's key
-    const int last = min(kb * RB + RB, seq.length) - 1;
     const int w0 = kb * RB + wave * 32, w1 = min(w0 + 32, seq.length) - 1;
-    // queries that see a key of the block: from the block's first key on, to
-    // the window's end behind its last one or, of first tokens, to the end
-    const int64_t reach = kb * RB < p.s.rule.sinks ? int64_t{kNoWindow} : int64_t{last} + p.s.rule.window - 1;
-    const int i0 = max(kb * RB - seq.start, seq.first);
-    const int i1 = static_cast<int>(min(reach - seq.start, static_cast<int64_t>(seq.end) - 1));
-    const int t0 = i0 / BQ;
-    const int per_query_head = last >= kb * RB && i0 <= i1 ? i1 / BQ - t0 + 1 : 0;
-    const int64_t all = static_cast<int64_t>(per_query_head) * p.s.group;
-    const int from = static_cast<int>(all * part / parts), to = static_cast<int>(all * (part + 1) / parts);
 
     f32x16 dk[DT], dv[DT];
 #pragma unroll
@@ -446,7 +573,7 @@ __global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) voi
             step(it + 1, q1s, d1s, l1s, q0s, d0s, l0s);
         }
     }
-    if (mine >= p.s.keys) return;
+    const bool bad = mine < p.s.keys && (holds_nan(dk) || holds_nan(dv));
     if constexpr (ColumnScale<T>::kOn) {
         constexpr float kDown = 1.0f / (1 << kProbabilityBits<T>);
         const float down = scaled.down() * kDown;
@@ -458,31 +585,26 @@ __global__ __launch_bounds__(W* kWave, W == 1 || sizeof(S_<T>) == 4 ? 1 : 2) voi
                 dv[d][e] *= kDown;
             }
     }
-    if (parts > 1) {
-        const int64_t at_part = static_cast<int64_t>(bh) * p.sums() + local + (sink ? 0 : p.sums_of_sinks());
-        float* sums = p.part + (at_part * 2 * RB + wave * 32 + l32) * p.s.dim;
+    if (mine < p.s.keys) {
+        const int64_t at_row = ((static_cast<int64_t>(b) * p.s.keys + mine) * p.s.kv_heads + hk) * p.s.dim;
+        float* const sums = p.part + (walk.at_part * 2 * RB + wave * 32 + l32) * p.s.dim;
 #pragma unroll
         for (int d = 0; d < DT; ++d)
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
                 const int at = 32 * d + row_of(e, half);
                 if (at >= p.s.dim) continue;
-                store4<float>(sums + at, dk[d][e], dk[d][e + 1], dk[d][e + 2], dk[d][e + 3]);
-                store4<float>(sums + RB * p.s.dim + at, dv[d][e], dv[d][e + 1], dv[d][e + 2], dv[d][e + 3]);
+                if (walk.parts > 1) {
+                    store4<float>(sums + at, dk[d][e], dk[d][e + 1], dk[d][e + 2], dk[d][e + 3]);
+                    store4<float>(sums + RB * p.s.dim + at, dv[d][e], dv[d][e + 1], dv[d][e + 2], dv[d][e + 3]);
+                } else {
+                    store4<T>(static_cast<S*>(p.dk) + at_row + at, dk[d][e] * p.scale, dk[d][e + 1] * p.scale, dk[d][e + 2] * p.scale,
+                              dk[d][e + 3] * p.scale);
+                    store4<T>(static_cast<S*>(p.dv) + at_row + at, dv[d][e], dv[d][e + 1], dv[d][e + 2], dv[d][e + 3]);
+                }
             }
-        return;
     }
-    const int64_t at_row = ((static_cast<int64_t>(b) * p.s.keys + mine) * p.s.kv_heads + hk) * p.s.dim;
-#pragma unroll
-    for (int d = 0; d < DT; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int at = 32 * d + row_of(e, half);
-            if (at >= p.s.dim) continue;
-            store4<T>(static_cast<S*>(p.dk) + at_row + at, dk[d][e] * p.scale, dk[d][e + 1] * p.scale, dk[d][e + 2] * p.scale,
-                      dk[d][e + 3] * p.scale);
-            store4<T>(static_cast<S*>(p.dv) + at_row + at, dv[d][e], dv[d][e + 1], dv[d][e + 2], dv[d][e + 3]);
-        }
+    if (__any(bad)) keys_again<T, BQ, W>(launched_with<Backward>(), bad);
 }
 
 // The parts of a block's sums in order, four elements a thread: blockIdx.x

@@ -331,6 +331,168 @@ __device__ __forceinline__ void store4(S_<T>* at, float a, float b, float c, flo
     else *reinterpret_cast<uint4*>(at) = __builtin_bit_cast(uint4, v);
 }
 
+// ---- sums again ----------------------------------------------------------------------
+//
+// A matrix instruction sums over all rows of a tile, and what a column does not
+// see has a factor of 0 there: beside a value that is not finite that is NaN, in
+// columns that never saw it.  So a wave that finds a NaN in its sums at the end of
+// its walk looks for such values among the rows its block has read.  A column
+// that sees one keeps what it has; one that only shared a tile with it is summed
+// again over what it sees, all lanes on one column.  The test is one sum of the
+// accumulators.  What follows it stands in functions of its own, where it costs
+// the walks no registers; the search reads the rows once more, and the columns
+// beside a value, fewer than a block has, take some 0.2 us a row each: 8192
+// tokens, 32 heads of 128 on 8, forward and backward 3.4 ms, with one infinity in
+// the value of token 4000 16, in the gradient of token 4000's result 105.
+
+// Whether the sums hold a NaN (or infinities of both signs).
+template <int DT>
+__device__ __forceinline__ bool holds_nan(const f32x16 (&sums)[DT]) {
+    float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e % 4] += sums[d][e];
+    const float all = (x[0] + x[1]) + (x[2] + x[3]);
+    return all != all;
+}
+
+__device__ __forceinline__ bool finite(float x) { return x - x == 0.0f; }
+
+// The kernel's argument, for a function that it calls: as it was launched, so
+// that the kernel's own stays in registers.  The function takes its fields by
+// scalar loads, and what all lanes share of its other arguments into scalars.
+template <typename Args>
+__device__ __forceinline__ const Args* launched_with() {
+    return (const Args*)__builtin_amdgcn_kernarg_segment_ptr();
+}
+template <typename Args>
+__device__ __forceinline__ const Args& as_launched(const Args* at) {
+    const uint64_t a = reinterpret_cast<uint64_t>(at);
+    const uint64_t shared = static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a >> 32)))) << 32 |
+                            static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(a)));
+    return *(const Args*)(__attribute__((address_space(4))) const Args*)shared;
+}
+__device__ __forceinline__ int shared_by_lanes(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// Whether all elements of a token row are finite.
+template <typename T>
+__device__ __forceinline__ bool row_is_finite(const S_<T>* row, int dim) {
+    constexpr int N = Packet<T>::N;
+    float none = 0.0f;
+#pragma unroll 1
+    for (int d = 0; d < dim; d += N) {
+        float x[N];
+        unpack<T>(*reinterpret_cast<const uint4*>(row + d), x);
+#pragma unroll
+        for (int j = 0; j < N; ++j) none = fmaf(x[j], 0.0f, none);
+    }
+    return none == none;
+}
+
+// A lane's two elements of a token row that all lanes share (the last two again
+// in lanes past its end).
+struct Two {
+    float x, y;
+};
+template <typename T>
+__device__ __forceinline__ Two two_of(const S_<T>* row, int dim) {
+    const int at = min(2 * static_cast<int>(threadIdx.x % kWave), dim - 2);
+    struct alignas(2 * sizeof(S_<T>)) Pair {
+        S_<T> x, y;
+    };
+    const Pair v = *reinterpret_cast<const Pair*>(row + at);
+    return Two{Elem<T>::load(v.x), Elem<T>::load(v.y)};
+}
+template <typename T>
+__device__ __forceinline__ void store_two(S_<T>* row, int dim, const Two& v) {
+    const int at = 2 * (threadIdx.x % kWave);
+    if (at >= dim) return;
+    row[at] = Elem<T>::store(v.x);
+    row[at + 1] = Elem<T>::store(v.y);
+}
+__device__ __forceinline__ void add_two(Two& sum, float f, const Two& v) {
+    sum.x = fmaf(f, v.x, sum.x);
+    sum.y = fmaf(f, v.y, sum.y);
+}
+
+// Product of a lane's row with another.
+template <typename T>
+__device__ __forceinline__ float row_product(const S_<T>* a, const S_<T>* b, int dim) {
+    float sum = 0.0f;
+#pragma unroll 2
+    for (int d = 0; d < dim; d += Packet<T>::N) {
+        float x[Packet<T>::N], y[Packet<T>::N];
+        unpack<T>(*reinterpret_cast<const uint4*>(a + d), x);
+        unpack<T>(*reinterpret_cast<const uint4*>(b + d), y);
+#pragma unroll
+        for (int j = 0; j < Packet<T>::N; ++j) sum = fmaf(x[j], y[j], sum);
+    }
+    return sum;
+}
+
+__device__ __forceinline__ float from_lane(float v, int lane) {
+    return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
+}
+
+// sum += the lanes' f times their rows (lane l's `step` l elements from `rows`
+// on), of the lanes in `seen`, which is not 0.
+template <typename T>
+__device__ __forceinline__ void add_rows(Two& sum, float f, const S_<T>* rows, int64_t step, uint64_t seen, int dim) {
+    const int first = __ffsll(static_cast<unsigned long long>(seen)) - 1;
+#pragma unroll 16
+    for (int l = 0; l < kWave; ++l) {
+        const bool in = seen >> l & 1;
+        add_two(sum, in ? from_lane(f, l) : 0.0f, two_of<T>(rows + (in ? l : first) * step, dim));
+    }
+}
+
+// The wave's lanes together.
+template <typename Op>
+__device__ __forceinline__ float over_wave(float v, Op op) {
+    for (int m = 1; m < kWave; m *= 2) v = op(v, wave_shfl_xor(v, m));
+    return v;
+}
+
+// f(j0, seen) for the keys that row p sees: 64 of them from j0 on, one a lane,
+// those in `seen`.
+template <typename F>
+__device__ __forceinline__ void for_seen(const Rule& r, int p, const F& f) {
+    const KeyTiles tiles(r, p, p, kWave);
+    for (int i = 0; i < tiles.count; ++i) {
+        const int j0 = tiles.at(i) * kWave;
+        const uint64_t seen = __ballot(r.sees(p, j0 + static_cast<int>(threadIdx.x % kWave)));
+        if (seen != 0) f(j0, seen);
+    }
+}
+
+// Of the lanes that ask (`bad`, on row `row`): those whose row sees none of the
+// values that are not finite among the keys that rows p0 .. p1 read, where there
+// is one that it does not see.  `rows` is the first key's row of the tensor.
+template <typename T>
+__device__ __forceinline__ bool only_beside(const Shape& s, const S_<T>* rows, int64_t step, int p0, int p1, bool bad, int row) {
+    const KeyTiles tiles(s.rule, p0, p1, kWave);
+    const KeysSeen keep(s.rule, tiles, p1);
+    bool beside = false;
+    for (int i = 0; i < tiles.count && __any(bad); ++i) {
+        const int j0 = tiles.at(i) * kWave, mine = j0 + static_cast<int>(threadIdx.x % kWave);
+        uint64_t found = __ballot(keep(mine) && !row_is_finite<T>(rows + mine * step, s.dim));
+        for (; found != 0; found &= found - 1) {
+            const bool sees = s.rule.sees(row, j0 + __ffsll(static_cast<unsigned long long>(found)) - 1);
+            beside = beside || !sees;
+            bad = bad && !sees;
+        }
+    }
+    return bad && beside;
+}
+
+// f(lane) for the first lane that asks, and again until no lane does that f has
+// not answered: f returns whether a lane's question is the same.
+template <typename F>
+__device__ __forceinline__ void for_each_question(bool asks, const F& f) {
+    for (uint64_t left = __ballot(asks); left != 0;) left &= ~__ballot(f(__ffsll(static_cast<unsigned long long>(left)) - 1));
+}
+
 // Waits until this wave's loads have landed and its LDS reads are done, then
 // meets the block's other waves.  (Not __syncthreads(): the compiler would
 // place the wait where it likes among the loads into LDS.)

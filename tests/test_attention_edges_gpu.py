@@ -176,7 +176,7 @@ def test_rows_whose_scores_are_minus_infinity(dev, ops, dtype, tq, heads, kv):
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("heads,kv", [(1, 1), (256, 128)])
-@pytest.mark.parametrize("where", ["out"])
+@pytest.mark.parametrize("where", ["query", "gradient", "out"])
 def test_rows_given_as_without_a_sum(dev, ops, dtype, heads, kv, where):
     """A query whose l is handed in as -inf has no gradient and takes no part
     in the keys', whatever it, its result and its gradient hold."""
@@ -298,3 +298,102 @@ def test_gradients_of_rows_that_see_few_keys(dev, ops, dtype, shape, rule):
     dq, dk, _ = ops.sliding_window_attention_backward(g, q, k, v, out, lse, **rule)
     assert_within(dq.numpy(), want[0], a.tokens(bq), dtype, "dq")
     assert_within(dk.numpy(), want[1], a.shared(bk), dtype, "dk")
+
+
+# ---- what is not finite stays with those that see it ------------------------------------
+
+
+CROSS = [((1, 200, 200, 2, 1, 64), dict(window=40, sinks=3), 150),
+         ((2, 40, 90, 4, 2, 32), dict(), 70),
+         ((1, 300, 300, 3, 3, 128), dict(window=33), 100),
+         ((1, 6, 500, 8, 2, 96), dict(window=100, sinks=2), 496),
+         ((2, 200, 200, 128, 64, 40), dict(window=70, sinks=1), 130)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("what", ["key", "value"])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf], ids=["nan", "inf", "-inf"])
+@pytest.mark.parametrize("shape,rule,at", CROSS, ids=str)
+def test_keys_and_values_reach_their_queries_only(dev, ops, dtype, what, value, shape, rule, at):
+    """Key ``at`` of key head 0 or its value is not finite: queries that do not
+    see it, and keys that none of its queries sees, are as without it."""
+    host = make(dtype, *shape, 90)
+    w = [wide(x, dtype) for x in host]
+    a = Attention(dtype, *w[:3], **rule)
+    want, bounds = a.backward(w[3], dtype)
+    group = shape[3] // shape[4]
+    struck = host[1 if what == "key" else 2]
+    struck[0, at, 0, 5] = one(value, dtype)
+    q, k, v, do = (put(x, dtype) for x in host)
+    out, lse = ops.sliding_window_attention(q, k, v, **rule)
+    grads = ops.sliding_window_attention_backward(do, q, k, v, out, lse, **rule)
+    rows = np.zeros(a.lse.shape, bool)  # [B, H, Tq]: those that see it
+    rows[0, :group] = a.see[0, 0][:, at]
+    assert rows.any() and not rows.all()
+    keys = np.zeros((shape[0], shape[4], shape[2]), bool)  # seen by one of those
+    keys[0, 0] = a.see[0, 0][rows[0, 0]].any(0)
+    r, c = rows.transpose(0, 2, 1)[..., None], keys.transpose(0, 2, 1)[..., None]
+    o = wide(out.numpy(), dtype)
+    if what == "value":
+        assert not np.isfinite(o[0, rows[0, 0], 0, 5]).any()
+        fine = r & (np.arange(shape[5]) != 5)
+        assert np.isfinite(o[np.broadcast_to(fine, o.shape)]).all()
+    elif value != value:
+        assert np.isnan(o[np.broadcast_to(r, o.shape)]).all()
+
+    def clean(x, x64, bound, mask, name):
+        x = wide(x, dtype if x.ndim == 4 else F32)
+        mask = np.broadcast_to(mask, x.shape)
+        kept = np.where(mask, 0.0, x)
+        store = orc.from_float(kept.astype(np.float32), dtype) if x.ndim == 4 else kept.astype(np.float32)
+        assert_within(store, np.where(mask, 0.0, x64), np.where(mask, 0.0, bound), dtype if x.ndim == 4 else F32, name)
+
+    clean(out.numpy(), a.tokens(a.out), a.tokens(a.out_bound), r, "out")
+    clean(lse.numpy(), a.lse, a.lse_bound, rows, "lse")
+    for g, x, bound, m, name in zip(grads, want, bounds, (r, c, c), ("dq", "dk", "dv")):
+        clean(g.numpy(), x, bound, m, name)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("what", ["query", "gradient"])
+@pytest.mark.parametrize("value", [np.nan, np.inf], ids=["nan", "inf"])
+@pytest.mark.parametrize("shape,rule,at", CROSS, ids=str)
+def test_queries_and_gradients_reach_their_keys_only(dev, ops, dtype, what, value, shape, rule, at):
+    """One query of head 0 or its gradient is not finite: keys that it does not
+    see are as without it, and so is every other query."""
+    host = make(dtype, *shape, 95)
+    w = [wide(x, dtype) for x in host]
+    a = Attention(dtype, *w[:3], **rule)
+    want, bounds = a.backward(w[3], dtype)
+    i = shape[1] // 2
+    struck = host[0 if what == "query" else 3]
+    struck[0, i, 0, 5] = one(value, dtype)
+    q, k, v, do = (put(x, dtype) for x in host)
+    out, lse = ops.sliding_window_attention(q, k, v, **rule)
+    grads = ops.sliding_window_attention_backward(do, q, k, v, out, lse, **rule)
+    seen = a.see[0, 0, i]
+    for g, x, bound, name in zip(grads, want, bounds, ("dq", "dk", "dv")):
+        g64, x, bound = wide(g.numpy(), dtype), x.copy(), bound.copy()
+        at_ = (0, i, 0) if name == "dq" else (0, seen, 0)
+        g64[at_] = x[at_] = bound[at_] = 0.0
+        assert_within(orc.from_float(g64.astype(np.float32), dtype), x, bound, dtype, name)
+    dv = wide(grads[2].numpy(), dtype)[0, seen, 0]
+    assert not np.isfinite(dv[:, 5]).any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("tq,heads", [(3, 2), (200, 2), (200, 256)])
+def test_keys_that_no_query_sees(dev, ops, dtype, tq, heads):
+    """A window of none leaves the first tokens alone: NaN in every other key
+    and value reaches nothing, and their own gradients are zeros."""
+    host = make(dtype, 1, tq, 200, heads, heads, 32, 99)
+    w = [wide(x, dtype) for x in host]
+    a = Attention(dtype, *w[:3], window=0, sinks=4)
+    want, bounds = a.backward(w[3], dtype)
+    for x in host[1:3]:
+        x[:, 4:] = one(np.nan, dtype)
+    q, k, v, do = (put(x, dtype) for x in host)
+    out, lse = ops.sliding_window_attention(q, k, v, 0, 4)
+    assert_within(out.numpy(), a.tokens(a.out), a.tokens(a.out_bound), dtype, "out")
+    for g, x, bound, name in zip(ops.sliding_window_attention_backward(do, q, k, v, out, lse, 0, 4), want, bounds, ("dq", "dk", "dv")):
+        assert_within(g.numpy(), x, bound, dtype, name)
