@@ -28,6 +28,13 @@ namespace {
 
 constexpr float kSlack = 8.0f;
 
+// How far the bound m lies under the scores that set it.  float16 steps by 2^-24
+// below 2^-14, and many keys far below the largest can be what a row is made of:
+// with its probabilities rounded at 2^7 times their size, 2^15 at most, 2^21 keys
+// lose less by those steps than half a step of the result.
+template <typename T>
+constexpr float kUnder = std::is_same_v<T, f16_t> ? 7.0f : 0.0f;
+
 struct Forward {
     Shape s;
     TokenRows q, k, v;
@@ -50,14 +57,14 @@ struct Columns {
         t = 0.0f;
     }
     // Scores of NS x 32 keys become probabilities in place.
-    template <int NS>
+    template <typename T, int NS>
     __device__ __forceinline__ void absorb(f32x16 (&s)[NS], float scale) {
         float top = s[0][0];
 #pragma unroll
         for (int u = 0; u < NS; ++u)
 #pragma unroll
             for (int e = u == 0 ? 1 : 0; e < 16; ++e) top = fmaxf(top, s[u][e]);
-        top = both_halves(top, MaxOf{}) * scale;
+        top = both_halves(top, MaxOf{}) * scale - kUnder<T>;
         if (__any(top > m + kSlack || (m == -INFINITY && top > m))) {
             const float now = fmaxf(m, top);
             const float turn = now == m ? 1.0f : __builtin_amdgcn_exp2f(m - now);
@@ -242,7 +249,7 @@ __global__ __launch_bounds__(kWide* kWave, sizeof(S_<T>) == 4 && DT == 4 ? 1 : 2
                         if (!p.s.rule.sees(row, j0 + 32 * u + row_of(e, half))) s[u][e] = -INFINITY;
                     }
             }
-            col.template absorb<NS>(s, p.scale);
+            col.template absorb<T, NS>(s, p.scale);
 #pragma unroll
             for (int u = 0; u < NS; ++u)
 #pragma unroll
@@ -410,7 +417,7 @@ __global__ __launch_bounds__((kSplitWaves<T, DT> * kWave), 1) void attention_spl
                         if (!p.s.rule.sees(row, j0 + row_of(e, half))) s[0][e] = -INFINITY;
                     }
                 }
-                col.template absorb<1>(s, p.scale);
+                col.template absorb<T, 1>(s, p.scale);
                 if (more) wait_but<2 * Keys::kIssue>();  // and its values
                 else wait_but<0>();
 #pragma unroll

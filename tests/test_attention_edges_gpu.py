@@ -397,3 +397,29 @@ def test_keys_that_no_query_sees(dev, ops, dtype, tq, heads):
     assert_within(out.numpy(), a.tokens(a.out), a.tokens(a.out_bound), dtype, "out")
     for g, x, bound, name in zip(ops.sliding_window_attention_backward(do, q, k, v, out, lse, 0, 4), want, bounds, ("dq", "dk", "dv")):
         assert_within(g.numpy(), x, bound, dtype, name)
+
+
+# ---- many small probabilities ---------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("tq,tk,heads", [(1, 4097, 2), (1, 70001, 2), (40, 4097, 2), (130, 2200, 64)])
+@pytest.mark.parametrize("first", [True, False], ids=["first", "last"])
+def test_many_keys_far_below_the_largest(dev, ops, dtype, tq, tk, heads, first):
+    """One key stands 17 above all others, whose probabilities of 2^-24.5 are
+    what the result is made of.  float16 has them as subnormals: a probability
+    is rounded at 2^7 times its size against the row's bound, so it is off by
+    half of the smallest step, 2^-25, over 2^7, besides its half step."""
+    d = 16
+    q, k, v, _ = (wide(x, dtype) for x in make(dtype, 1, tq, tk, heads, heads, d, 110))
+    q[:], k[:] = 0.0, 0.0
+    q[..., 0] = 1.0
+    k[:, 0 if first else tk - tq, :, 0] = 17.0
+    v = np.abs(v)
+    v[:, 0 if first else tk - tq] = 0.0
+    host = [orc.from_float(x.astype(np.float32), dtype) for x in (q, k, v)]
+    a = Attention(dtype, *[wide(x, dtype) for x in host], scale=1.0)
+    out, lse = ops.sliding_window_attention(*[put(x, dtype) for x in host], scale=1.0)
+    bound = a.out_bound + (2.0 ** -32 * (a.see @ np.abs(a.v)) if dtype == F16 else 0.0)
+    assert_within(out.numpy(), a.tokens(a.out), a.tokens(bound), dtype, "out")
+    assert_within(lse.numpy(), a.lse, a.lse_bound, F32, "lse")
