@@ -5,7 +5,7 @@
 // the first R elements of n turn in R / 2 pairs (a, b) -> (a c - b s,
 // b c + a s) with c, s from the position's row of a table.  Pair j is
 // elements (j, j + R / 2), or (2 j, 2 j + 1) when interleaved; elements past
-// R keep n.  Backward, with g the gradient turned back, u = g w and
+// R keep n, whatever lies beside them in a lane.  Backward, with g the gradient turned back, u = g w and
 // m = x r: dx = r (u - m mean(u m)), dw = sum over rows of g m.
 //
 // Bound by memory: a row is read once (backward: x and dy) and written once.
@@ -222,8 +222,11 @@ __global__ __launch_bounds__(kBlock) void head_norm_kernel(HeadNormPlan w) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float na = a[r][k][j] * scale[r] * wa[j], nb = b[r][k][j] * scale[r] * wb[j];
-                ya[j] = na * c[j] - nb * s[j];
-                yb[j] = nb * c[j] + na * s[j];
+                ya[j] = na * c[j], yb[j] = nb * c[j];
+                if (unit.turns) {
+                    ya[j] -= nb * s[j];
+                    yb[j] += na * s[j];
+                }
             }
             const int64_t row = static_cast<int64_t>(token) * side.heads + h0 + r;
             store_unit<T, V, INTER>(static_cast<S_<T>*>(side.out) + row * w.p.dim, unit, ya, yb);
@@ -271,7 +274,11 @@ __global__ __launch_bounds__(kBlock) void head_norm_backward_kernel(HeadNormPlan
             load_turn<V>(w, pos, u, c, s);
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const float ta = ga[j] * c[j] + gb[j] * s[j], tb = gb[j] * c[j] - ga[j] * s[j];
+                float ta = ga[j] * c[j], tb = gb[j] * c[j];
+                if (unit.turns) {
+                    ta += gb[j] * s[j];
+                    tb -= ga[j] * s[j];
+                }
                 ma[k][j] *= r;
                 mb[k][j] *= r;
                 da[k][j] = fmaf(ta, ma[k][j], da[k][j]);

@@ -196,3 +196,33 @@ def test_recorded_and_replayed(dev, ops):
                 assert np.array_equal(a.numpy(), b.numpy())
     finally:
         g.reset()
+
+
+@pytest.mark.parametrize("interleaved", [False, True], ids=["halves", "neighbours"])
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("dim,rotary", [(64, 0), (80, 48), (64, 32), (33, 16), (7, 0), (256, 64)])
+def test_an_element_that_does_not_turn_stays_by_itself(dev, ops, dtype, dim, rotary, interleaved):
+    """Elements past the rotated ones have no partner: where the weight or the
+    gradient of one is infinite, the others' results and weight gradients are as
+    without it."""
+    h = 3
+    q, k, dq, dk = (sample((2, 5, h, dim), dtype, 90 + i) for i in range(4))
+    tab, pos = table_of(20, rotary), np.arange(10).reshape(2, 5)
+    at = rotary
+    others = np.arange(dim) != at
+    w = sample((dim,), dtype, 95, 0.2, 1.0)
+    w[at] = orc_from(np.array([np.inf], np.float32), dtype)[0]
+    y, ky, r, kr = ops.qk_norm_rope(put(q, dtype), put(k, dtype), put(tab), put(pos), put(w, dtype), put(w, dtype), interleaved=interleaved)
+    w64 = np.where(others, wide(w, dtype), 0.0)
+    for got, x in ((y, q), (ky, k)):
+        want, _, mag = head_norm(wide(x, dtype), w64, tab, pos, 1e-6, interleaved)
+        assert_within(got.numpy()[..., others], want[..., others], 20 * U * mag[..., others], dtype)
+        assert np.isinf(wide(got.numpy(), dtype)[..., at]).all()
+    dq[1, 2, 1, at] = orc_from(np.array([np.inf], np.float32), dtype)[0]
+    _, _, r, kr = ops.qk_norm_rope(put(q, dtype), put(k, dtype), put(tab), put(pos), interleaved=interleaved)
+    grads = ops.qk_norm_rope_backward(put(dq, dtype), put(dk, dtype), put(q, dtype), put(k, dtype), put(tab), put(pos), r, kr,
+                                      interleaved=interleaved)
+    dy = wide(dq, dtype)
+    dy[1, 2, 1, at] = 0.0
+    _, dw, _, total = head_norm_backward(dy, wide(q, dtype), r.numpy().astype(np.float64), np.ones(dim), tab, pos, interleaved)
+    assert_within(grads[2].numpy()[others], dw[others], 70 * U * total[others], dtype)
