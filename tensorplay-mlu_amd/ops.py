@@ -450,7 +450,11 @@ def qk_norm_rope_backward(grad_query, grad_key, query, key, table, positions, qu
 
 
 def _attention_scale(query, scale):
-    return float(scale) if scale is not None else max(query.shape[-1], 1) ** -0.5
+    """D ** -0.5 unless given; a query without a last axis is the library's to refuse."""
+    if scale is not None:
+        return float(scale)
+    shape = query.shape if query is not None else ()
+    return max(shape[-1], 1) ** -0.5 if shape else 1.0
 
 
 def sliding_window_attention(query, key, value, window=-1, sinks=0, scale=None, lengths=None,
@@ -462,16 +466,17 @@ def sliding_window_attention(query, key, value, window=-1, sinks=0, scale=None, 
     first query (None: the queries are its last tokens).  lse [B, Hq, Tq] is
     float32, -inf for a query that sees nothing, whose row of out is zeros."""
     return _call_results(L().tp_amd_sliding_window_attention, _ref(query), _ref(key), _ref(value),
-                         int(window), int(sinks), _attention_scale(query, scale), _ref(lengths),
-                         _ref(starts), count=2)
+                         int(window), int(sinks), _attention_scale(query, scale),
+                         _ref(lengths), _ref(starts), count=2)
 
 
 def sliding_window_attention_backward(grad_out, query, key, value, out, lse, window=-1, sinks=0,
                                       scale=None, lengths=None, starts=None):
     """(dquery, dkey, dvalue) from the forward's operands and results."""
     return _call_results(L().tp_amd_sliding_window_attention_backward, _ref(grad_out), _ref(query),
-                         _ref(key), _ref(value), _ref(out), _ref(lse), int(window), int(sinks),
-                         _attention_scale(query, scale), _ref(lengths), _ref(starts), count=3)
+                         _ref(key), _ref(value), _ref(out), _ref(lse), int(window),
+                         int(sinks), _attention_scale(query, scale), _ref(lengths),
+                         _ref(starts), count=3)
 
 
 #: The 72 operator names of the reference's registrations (64 on the hot

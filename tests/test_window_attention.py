@@ -115,3 +115,16 @@ def test_backward_refused(ops, change, error):
         a[i] = t
     with pytest.raises(getattr(mod("tensor"), error)):
         ops.sliding_window_attention_backward(*a, window=4)
+
+
+@pytest.mark.parametrize("query,error", [(None, "DeviceError"), (fake(()), "DeclinedError"), (fake((16,)), "DeclinedError")],
+                         ids=["none", "scalar", "one_axis"])
+def test_refused_without_a_scale(ops, query, error):
+    """The default scale asks a query for its last axis: one that has none is
+    refused as it is with a scale."""
+    t = mod("tensor")
+    with pytest.raises(getattr(t, error)) as given:
+        call(ops, query=query, scale=0.25)
+    with pytest.raises(getattr(t, error)) as default:
+        call(ops, query=query)
+    assert str(default.value) == str(given.value)
