@@ -457,6 +457,11 @@ def _attention_scale(query, scale):
     return max(shape[-1], 1) ** -0.5 if shape else 1.0
 
 
+def _tokens(n):
+    """A number of tokens as the library's 64 bits hold it: past them is as many as there can be."""
+    return max(min(int(n), (1 << 63) - 1), -(1 << 63))
+
+
 def sliding_window_attention(query, key, value, window=-1, sinks=0, scale=None, lengths=None,
                              starts=None):
     """(out, lse): causal attention of query [B, Tq, Hq, D] over key and value
@@ -466,7 +471,7 @@ def sliding_window_attention(query, key, value, window=-1, sinks=0, scale=None, 
     first query (None: the queries are its last tokens).  lse [B, Hq, Tq] is
     float32, -inf for a query that sees nothing, whose row of out is zeros."""
     return _call_results(L().tp_amd_sliding_window_attention, _ref(query), _ref(key), _ref(value),
-                         int(window), int(sinks), _attention_scale(query, scale),
+                         _tokens(window), _tokens(sinks), _attention_scale(query, scale),
                          _ref(lengths), _ref(starts), count=2)
 
 
@@ -474,8 +479,8 @@ def sliding_window_attention_backward(grad_out, query, key, value, out, lse, win
                                       scale=None, lengths=None, starts=None):
     """(dquery, dkey, dvalue) from the forward's operands and results."""
     return _call_results(L().tp_amd_sliding_window_attention_backward, _ref(grad_out), _ref(query),
-                         _ref(key), _ref(value), _ref(out), _ref(lse), int(window),
-                         int(sinks), _attention_scale(query, scale), _ref(lengths),
+                         _ref(key), _ref(value), _ref(out), _ref(lse), _tokens(window),
+                         _tokens(sinks), _attention_scale(query, scale), _ref(lengths),
                          _ref(starts), count=3)
 
 

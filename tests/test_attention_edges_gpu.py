@@ -423,3 +423,20 @@ def test_many_keys_far_below_the_largest(dev, ops, dtype, tq, tk, heads, first):
     bound = a.out_bound + (2.0 ** -32 * (a.see @ np.abs(a.v)) if dtype == F16 else 0.0)
     assert_within(out.numpy(), a.tokens(a.out), a.tokens(bound), dtype, "out")
     assert_within(lse.numpy(), a.lse, a.lse_bound, F32, "lse")
+
+
+# ---- numbers of tokens past 64 bits -----------------------------------------------------
+
+
+def test_windows_past_64_bits(dev, ops):
+    """A window of 2^70 is none, and 2^63 first tokens are all of them.  (The same
+    keys in tiles of another order: P is off by under 2^-16 of itself, its sums
+    over 40 keys by no more, and dS is a difference of two such sums.)"""
+    q, k, v, do = (put(x, F32) for x in make(F32, 1, 9, 40, 2, 1, 16, 120))
+    want = ops.sliding_window_attention(q, k, v)
+    grads = ops.sliding_window_attention_backward(do, q, k, v, *want)
+    for rule in (dict(window=2 ** 70), dict(window=2, sinks=2 ** 63), dict(window=-2 ** 70)):
+        got = ops.sliding_window_attention(q, k, v, **rule)
+        assert_within(got[0].numpy(), want[0].numpy(), 2.0 ** -15 * np.abs(want[0].numpy()).max(), F32, str(rule))
+        for g, w in zip(ops.sliding_window_attention_backward(do, q, k, v, *got, **rule), grads):
+            assert_within(g.numpy(), w.numpy(), 2.0 ** -13 * np.abs(w.numpy()).max(), F32, str(rule))

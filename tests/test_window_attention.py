@@ -128,3 +128,10 @@ def test_refused_without_a_scale(ops, query, error):
     with pytest.raises(getattr(t, error)) as default:
         call(ops, query=query)
     assert str(default.value) == str(given.value)
+
+
+@pytest.mark.parametrize("n,want", [(5, 5), (-1, -1), (2 ** 63 - 1, 2 ** 63 - 1), (2 ** 63, 2 ** 63 - 1), (2 ** 70, 2 ** 63 - 1),
+                                    (-2 ** 70, -2 ** 63)])
+def test_numbers_of_tokens_past_64_bits(ops, n, want):
+    """They do not come around: 2^70 is no window of 0."""
+    assert ops._tokens(n) == want
