@@ -267,8 +267,8 @@ int tp_amd_qk_norm_rope_backward(const tp_amd_tensor* grad_query, const tp_amd_t
  * (j > p - window or j < sinks); window < 0 is none.  A query outside
  * 0 <= p < lengths[b] is not used; it, and one that sees no key (or whose every
  * score is -inf), gives a row of zeros and an lse of -inf.  A key or value that is
- * not finite reaches the queries that see it and no others; where blocks of
- * neighbouring queries hold one the call is slower.
+ * not finite reaches the queries that see it and no others; keeping it from the
+ * neighbours of those takes such a call many times as long.
  * out [B, Tq, Hq, D] = softmax(scale q.k) v and float32 lse [B, Hq, Tq], the
  * natural logarithm of each row's sum of exponentials; scale > 0.  Scores,
  * statistics and sums are float32, probabilities are rounded to the

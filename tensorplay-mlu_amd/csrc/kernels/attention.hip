@@ -162,11 +162,12 @@ __device__ __forceinline__ bool unexplained(bool nan, float t) { return nan && t
 // Bound by issue: an exponential, two products, a sum, a maximum and half a
 // rounding an element beside the matrix instructions, and with all of them
 // running by the card's power, which holds it near 1.9 GHz.  bf16, 32 heads of
-// 128 on 8 key heads, 8192 tokens: window 1024 165 us, 780 Tflop/s of visible
-// pairs (tiles that the window's edges cut are half empty); all earlier keys
-// 1000 to 1080 Tflop/s, matrix cores busy 55 % of the cycles, where the
-// library's product of 16384 x 16384 makes 1337.  fp16, 4 x 777 queries, 16 heads
-// of 96 on 4 key heads, window 1500 of up to 4001 keys: 53 us, 545.
+// 128 on 8 key heads, 8192 tokens, launched back to back: all earlier keys 523 us,
+// 1050 Tflop/s of visible pairs, matrix cores busy 54 % of the cycles, where the
+// library's product of 16384 x 16384 makes 1340 to 1370; window 1024 162 to 170 us,
+// 770 to 800 Tflop/s, 42 % busy (a block reads 1.18 times the keys its rows see, a
+// wave multiplies 1.12 times).  fp16, 4 x 777 queries, 16 heads of 96 on 4 key
+// heads, window 1500 of up to 4001 keys: 53 us, 545.
 template <typename T, int DT>
 __global__ __launch_bounds__(kWide* kWave, sizeof(S_<T>) == 4 && DT == 4 ? 1 : 2) void attention_kernel(Forward p) {
     using S = S_<T>;

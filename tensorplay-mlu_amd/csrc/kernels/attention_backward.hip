@@ -24,12 +24,14 @@
 // Bound by the instructions that share a wave's issue: matrix products, and
 // beside them an exponential, two products and two roundings an element and
 // the reads from LDS (no bank conflicts).  bf16, 2 x 4096 tokens, 32 heads of
-// 128 on 8 key heads, window 1024: dq 214 us, 845 Tflop/s, its matrix cores busy
-// 49 % of the cycles; dk and dv 350 us, 690 Tflop/s, 35 %: two accumulators of
-// 32 x 128 and the fragments of keys and values leave a wave no registers to
-// read a tile ahead of its products; the join 4.5 us.  float32 is bound by its
-// matrix instructions, a sixteenth of bf16's rate: 1001 tokens, 12 heads of 64,
-// window 256, 77 us in all.
+// 128 on 8 key heads, window 1024, medians (and best): dq 222 us (213), 815
+// Tflop/s, its matrix cores busy 49 % of the cycles; dk and dv 368 us (354), 655
+// Tflop/s, 36 %: two accumulators of 32 x 128 and the fragments of keys and values
+// leave a wave no registers to read a tile ahead of its products, and 17 of them
+// pass through scratch memory in every tile; the join 5 us.  float32, a sixteenth
+// of bf16's rate: 1001 tokens, 12 heads of 64, window 256, 79 us in all, of which
+// dq takes 40 with 384 waves on 1024 SIMDs, each on a walk of up to 11 tiles that
+// only the other kernel cuts.
 
 #include <algorithm>
 

@@ -18,10 +18,12 @@
 // A group takes ROWS heads of one token in a row: their loads go out together
 // and the table's row, as many bytes as a 16-bit head, is read once for all.
 //
-// bf16, 40 heads of 128: 8192 tokens forward 31.5 us, 5.5 TB/s; 4 x 2048 backward
-// 45 us, 5.6 TB/s, and 4 us for the weights' sums over blocks (2 GiB read and
-// written by a plain elementwise pass: 6.35 TB/s).  8 tokens 3.7 us, a launch's
-// own time.
+// bf16, 40 heads of 128: 8192 tokens forward 32 us, 5.4 TB/s; 4 x 2048 backward
+// 46 us, 5.5 TB/s, and 4 us for the weights' sums over blocks (2 GiB read and
+// written by a plain elementwise pass: 6.35 TB/s).  8 tokens 3.5 us, a launch's
+// own time.  float32, 3001 tokens, 24 heads of 80 of which 40 turn as neighbours:
+// 12 us forward, 3.9 TB/s, 15 and 4 us backward (6 of a group's 16 lanes hold
+// nothing there).
 
 #include <algorithm>
 #include <type_traits>
