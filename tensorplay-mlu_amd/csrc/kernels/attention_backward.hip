@@ -378,10 +378,11 @@ __global__ __launch_bounds__(W* kWave, W == 1 || (sizeof(S_<T>) == 4 && DT == 4)
         };
         // Rows of few keys have the largest gradients, and the rounding of
         // their out in D is as large there as that of dS: the D of rows that see
-        // at most 128 keys is summed up from P and dP, in a walk of its own: a
+        // at most 128 keys, and of others in their block, which come behind them,
+        // is summed up from P and dP, in a walk of its own: a
         // tenth of forward and backward (8192 tokens, 32 heads of 128 under a
         // window of 128 273 us, 242 without) where all rows are such.
-        if (sizeof(S) == 2 && p.s.rule.most_seen(p1) <= 128) {
+        if (sizeof(S) == 2 && p.s.rule.count_seen(p0) <= 128) {
             walk(std::false_type{});
             delta = both_halves(exact, SumOf{});
             meet();

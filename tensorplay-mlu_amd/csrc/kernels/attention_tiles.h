@@ -41,8 +41,8 @@ struct Rule {
     int window;  // kNoWindow: every earlier key
     int sinks;
     __device__ __forceinline__ bool sees(int p, int j) const { return j <= p && (j > p - window || j < sinks); }
-    // Keys that a row up to p1 sees at most.
-    __device__ __forceinline__ int most_seen(int p1) const { return p1 - window < sinks ? p1 + 1 : window + sinks; }
+    // Keys that row p sees, no fewer than any row before it.
+    __device__ __forceinline__ int count_seen(int p) const { return p - window < sinks ? p + 1 : window + sinks; }
     // Every row of p0 .. p1 sees all of the keys k0 .. k1.
     __device__ __forceinline__ bool all_see(int p0, int p1, int k0, int k1) const {
         return k1 <= p0 && (k0 > p1 - window || k1 < sinks);
