@@ -121,12 +121,10 @@ __device__ __forceinline__ void finish4(const Forward& p, int64_t b, int i, int 
 // Rows of `out` that hold a NaN and are `bad`, each lane's its own (query i of
 // head h at position `row`): see "sums again".
 template <typename T>
-__device__ __attribute__((noinline)) void rows_again(const Forward* launched, int b_, int hk_, int p0, int p1, bool bad, int i, int h, int row) {
-    const int b = shared_by_lanes(b_), hk = shared_by_lanes(hk_);
-    const Forward& p = as_launched(launched);
+__device__ __forceinline__ void rows_again(const Forward& p, int b, int hk, int p0, int p1, bool bad, int i, int h, int row) {
     const S_<T>* kh = static_cast<const S_<T>*>(p.k.data) + b * p.k.batch + hk * p.k.head;
     const S_<T>* vh = static_cast<const S_<T>*>(p.v.data) + b * p.v.batch + hk * p.v.head;
-    for_each_question(only_beside<T>(p.s, vh, p.v.token, shared_by_lanes(p0), shared_by_lanes(p1), bad, row), [&](int lane) __attribute__((always_inline)) {
+    for_each_question(only_beside<T>(p.s, vh, p.v.token, p0, p1, bad, row), [&](int lane) __attribute__((always_inline)) {
         const int iu = __builtin_amdgcn_readlane(i, lane), hu = __builtin_amdgcn_readlane(h, lane);
         const S_<T>* q = static_cast<const S_<T>*>(p.q.data) + b * p.q.batch + iu * p.q.token + hu * p.q.head;
         Two o{0.0f, 0.0f};
@@ -148,6 +146,12 @@ __device__ __attribute__((noinline)) void rows_again(const Forward* launched, in
         store_two<T>(out, p.s.dim, Two{o.x * inv, o.y * inv});
         return i == iu && h == hu;
     });
+}
+
+// Of a block of 128 queries, those of a wave.
+template <typename T>
+__device__ __attribute__((noinline)) void queries_again(const Forward* launched, int b, int hk, int p0, int p1, bool bad, int i, int h, int row) {
+    rows_again<T>(as_launched(launched), shared_by_lanes(b), shared_by_lanes(hk), shared_by_lanes(p0), shared_by_lanes(p1), bad, i, h, row);
 }
 
 // Whether a row's NaN (if `nan`) is none that its sum has too.
@@ -269,7 +273,7 @@ __global__ __launch_bounds__(kWide* kWave, sizeof(S_<T>) == 4 && DT == 4 ? 1 : 2
     const float t = both_halves(col.t, SumOf{});
     if (mine < p.s.queries) finish_row<T, DT>(p, b, h, mine, half, alive, col.m, t, col);
     const bool bad = unexplained(alive && holds_nan(col.o), t);
-    if (__any(bad)) rows_again<T>(launched_with<Forward>(), b, hk, seq.start + b0, seq.start + b1, bad, mine, h, row);
+    if (__any(bad)) queries_again<T>(launched_with<Forward>(), b, hk, seq.start + b0, seq.start + b1, bad, mine, h, row);
 }
 
 // ---- few queries over many keys -------------------------------------------------
@@ -321,6 +325,41 @@ __device__ __forceinline__ void add_state(float m, float t, const float4& x, flo
 template <typename T, int DT>
 constexpr int kSplitWaves = Tile<T, DT, 32, 1>::kRow == 512 ? 2 : 4;
 
+// What a block of these owns: a split of row tile rt of a key head.
+struct SplitItem {
+    uint32_t tile, split, rt, b, hk;
+    Sequence seq;
+    int packed_end, b0, b1;  // its packed rows' end, its first and last alive query
+    __device__ __forceinline__ explicit SplitItem(const Split& q) {
+        // items: batch, key head, row tile, split
+        const uint32_t id = xcd_run(blockIdx.x, gridDim.x);
+        tile = fastdiv(id, q.by_splits), split = id - tile * q.splits;
+        const uint32_t bh = fastdiv(tile, q.by_row_tiles);
+        rt = tile - bh * q.row_tiles;
+        b = fastdiv(bh, q.by_kv_heads), hk = bh - b * q.f.s.kv_heads;
+    }
+    __device__ __forceinline__ void read_sequence(const Split& q) {
+        seq = sequence_of(q.f.s, b);
+        packed_end = min(static_cast<int>(rt) * 32 + 32, q.rows);
+        b0 = max(static_cast<int>(fastdiv(rt * 32, q.by_group)), seq.first);
+        b1 = min(static_cast<int>(fastdiv(packed_end - 1, q.by_group)), seq.end - 1);
+    }
+};
+
+// The rows that a block's threads finished with a NaN: bit k of a thread's `odd`
+// for the one of its k-th round, of THREADS quads, QUADS of them a row.
+template <typename T, int QUADS, int THREADS>
+__device__ __attribute__((noinline)) void tile_again(const Split* launched, unsigned odd) {
+    const Split& q = as_launched(launched);
+    SplitItem item(q);
+    item.read_sequence(q);
+    for (int k = 0; __any(odd >> k); ++k) {
+        const int packed = item.rt * 32 + (k * THREADS + static_cast<int>(threadIdx.x)) / QUADS, i = fastdiv(packed, q.by_group);
+        rows_again<T>(q.f, item.b, item.hk, item.seq.start + item.b0, item.seq.start + item.b1, odd >> k & 1, i,
+                      item.hk * q.f.s.group + packed - i * q.f.s.group, item.seq.start + i);
+    }
+}
+
 // A block owns 32 packed rows of a key head -- all query heads of the group
 // and all queries together, so the cache is read once -- and one split of the
 // keys they see.  Bound by the cache's bytes: every wave walks a run of 32-key
@@ -344,11 +383,8 @@ __global__ __launch_bounds__((kSplitWaves<T, DT> * kWave), 1) void attention_spl
     __shared__ int last;
     const Forward& p = q.f;
 
-    // items: batch, key head, row tile, split
-    const uint32_t id = xcd_run(blockIdx.x, gridDim.x);
-    const uint32_t tile = fastdiv(id, q.by_splits), split = id - tile * q.splits;
-    const uint32_t bh = fastdiv(tile, q.by_row_tiles), rt = tile - bh * q.row_tiles;
-    const uint32_t b = fastdiv(bh, q.by_kv_heads), hk = bh - b * p.s.kv_heads;
+    SplitItem item(q);
+    const uint32_t tile = item.tile, split = item.split, rt = item.rt, b = item.b, hk = item.hk;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x % kWave, l32 = lane % 32, half = lane / 32;
 
@@ -364,12 +400,11 @@ __global__ __launch_bounds__((kSplitWaves<T, DT> * kWave), 1) void attention_spl
             qf[s] = packed < q.rows && e < p.s.dim ? *reinterpret_cast<const uint4*>(from_row + e) : make_uint4(0, 0, 0, 0);
         }
     }
-    const Sequence seq = sequence_of(p.s, b);
+    item.read_sequence(q);
+    const Sequence& seq = item.seq;
     const bool alive = packed < q.rows && mine >= seq.first && mine < seq.end;
     const int row = seq.start + mine;
-    const int packed_end = min(static_cast<int>(rt) * 32 + 32, q.rows);
-    const int b0 = max(static_cast<int>(fastdiv(rt * 32, q.by_group)), seq.first);
-    const int b1 = min(static_cast<int>(fastdiv(packed_end - 1, q.by_group)), seq.end - 1);
+    const int packed_end = item.packed_end, b0 = item.b0, b1 = item.b1;
 
     Columns<DT> col;
     col.clear();
@@ -471,11 +506,7 @@ __global__ __launch_bounds__((kSplitWaves<T, DT> * kWave), 1) void attention_spl
         if (unexplained(x != x, total)) odd |= 1u << at / (W * kWave);
     };
     auto again = [&]() __attribute__((always_inline)) {
-        for (int k = 0; __any(odd >> k); ++k) {
-            const int packed_r = rt * 32 + (k * W * kWave + static_cast<int>(threadIdx.x)) / (DT * 8), i = fastdiv(packed_r, q.by_group);
-            rows_again<T>(&launched_with<Split>()->f, b, hk, seq.start + b0, seq.start + b1, odd >> k & 1, i,
-                          hk * p.s.group + packed_r - i * p.s.group, seq.start + i);
-        }
+        if (__any(odd != 0)) tile_again<T, DT * 8, W * kWave>(launched_with<Split>(), odd);
     };
     float* const stat = q.stat + (static_cast<int64_t>(tile) * q.splits + split) * q.tile_rows * 2;
     for (int at = threadIdx.x; at < rows_here * DT * 8; at += W * kWave) {

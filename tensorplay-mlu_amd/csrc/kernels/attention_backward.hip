@@ -195,29 +195,37 @@ __device__ __attribute__((noinline)) void keys_again(const Backward* launched, b
         const int h = hk * p.s.group + it / walk.per_query_head, r0 = (walk.t0 + it % walk.per_query_head) * BQ;
         f(h, (static_cast<int64_t>(b) * p.s.heads + h) * p.s.queries, max(r0, seq.first), min(r0 + BQ, seq.end));
     };
-    // a key that is not finite itself keeps what it has
-    bool beside = false;
-    if (bad && mine <= last) bad = row_is_finite<T>(kh + mine * p.k.token, p.s.dim) && row_is_finite<T>(vh + mine * p.v.token, p.s.dim);
-    for (int it = from; it < to && __any(bad); ++it) {
+    // Elements of dk and dv that rows the key sees, and others, make no number
+    // (a row's P makes all of them, its D those of dk).
+    const Elements all = all_elements(p.s.dim);
+    Elements own_k{0, 0}, own_v{0, 0}, beside_k{0, 0}, beside_v{0, 0};
+    for (int it = from; it < to && __any(bad && !(all.all_in(own_k) && all.all_in(own_v))); ++it) {
         tile(it, [&](int h, int64_t stat, int i0, int i1) __attribute__((always_inline)) {
+            const S_<T>*q = qb + h * p.q.head, *g = db + h * p.dout.head;
             const int i = i0 + lane_id;
-            bool odd = false, none = false;
+            bool odd = false, odd_p = false, odd_d = false, none = false;
             if (i < i1) {
                 const float bias = p.bias[stat + i];
                 none = bias == -INFINITY;
-                odd = bias != bias || !finite(p.delta[stat + i]) || !row_is_finite<T>(qb + h * p.q.head + i * p.q.token, p.s.dim) ||
-                      !row_is_finite<T>(db + h * p.dout.head + i * p.dout.token, p.s.dim);
+                odd_p = bias != bias;
+                odd_d = !finite(p.delta[stat + i]);
+                odd = odd_p || odd_d || !row_is_finite<T>(q + i * p.q.token, p.s.dim) || !row_is_finite<T>(g + i * p.dout.token, p.s.dim);
             }
-            const uint64_t without = __ballot(none);
+            const uint64_t without = __ballot(none), by_p = __ballot(odd_p), by_d = __ballot(odd_d);
             for (uint64_t found = __ballot(odd); found != 0; found &= found - 1) {
                 const int at = __ffsll(static_cast<unsigned long long>(found)) - 1;
                 const bool sees = mine <= last && !(without >> at & 1) && p.s.rule.sees(seq.start + i0 + at, mine);
-                beside = beside || !sees;
-                bad = bad && !sees;
+                const Elements in_q = odd_elements<T>(q + (i0 + at) * p.q.token, p.s.dim);
+                const Elements in_g = odd_elements<T>(g + (i0 + at) * p.dout.token, p.s.dim);
+                beside_k.add(in_q, !sees);
+                beside_v.add(in_g, !sees);
+                own_k.add((by_p | by_d) >> at & 1 ? all : in_q, sees);
+                own_v.add(by_p >> at & 1 ? all : in_g, sees);
             }
         });
     }
-    for_each_question(bad && beside, [&](int lane) __attribute__((always_inline)) {
+    bad = bad && !(beside_k.all_in(own_k) && beside_v.all_in(own_v));
+    for_each_question(bad, [&](int lane) __attribute__((always_inline)) {
         const int key = __builtin_amdgcn_readlane(mine, lane);
         const S_<T>*k = kh + key * p.k.token, *v = vh + key * p.v.token;
         Two dk{0.0f, 0.0f}, dv{0.0f, 0.0f};

@@ -337,13 +337,14 @@ __device__ __forceinline__ void store4(S_<T>* at, float a, float b, float c, flo
 // see has a factor of 0 there: beside a value that is not finite that is NaN, in
 // columns that never saw it.  So a wave that finds a NaN in its sums at the end of
 // its walk looks for such values among the rows its block has read.  A column
-// that sees one keeps what it has; one that only shared a tile with it is summed
-// again over what it sees, all lanes on one column.  The test is one sum of the
+// whose elements that hold one are those of rows it sees keeps what it has; one
+// that has an element's from a row that only shared a tile with it is summed again
+// over what it sees, all lanes on one column.  The test is one sum of the
 // accumulators.  What follows it stands in functions of its own, where it costs
 // the walks no registers; the search reads the rows once more, and the columns
 // beside a value, fewer than a block has, take some 0.2 us a row each: 8192
 // tokens, 32 heads of 128 on 8, forward and backward 3.4 ms, with one infinity in
-// the value of token 4000 16, in the gradient of token 4000's result 105.
+// the value of token 4000 22, in the gradient of its result 91.
 
 // Whether the sums hold a NaN (or infinities of both signs).
 template <int DT>
@@ -435,6 +436,29 @@ __device__ __forceinline__ float from_lane(float v, int lane) {
     return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
 }
 
+// Elements of a row, as bits: those at 2 l and at 2 l + 1.
+struct Elements {
+    uint64_t x, y;
+    __device__ __forceinline__ void add(const Elements& e, bool if_) {
+        x |= if_ ? e.x : 0;
+        y |= if_ ? e.y : 0;
+    }
+    __device__ __forceinline__ bool all_in(const Elements& e) const { return ((x & ~e.x) | (y & ~e.y)) == 0; }
+};
+
+__device__ __forceinline__ Elements all_elements(int dim) {
+    const uint64_t half = dim == 2 * kWave ? ~uint64_t{0} : (uint64_t{1} << dim / 2) - 1;
+    return Elements{half, half};
+}
+
+// Those of a row that all lanes share which are not finite.
+template <typename T>
+__device__ __forceinline__ Elements odd_elements(const S_<T>* row, int dim) {
+    const Two v = two_of<T>(row, dim);
+    const bool in = 2 * static_cast<int>(threadIdx.x % kWave) < dim;
+    return Elements{__ballot(in && !finite(v.x)), __ballot(in && !finite(v.y))};
+}
+
 // sum += the lanes' f times their rows (lane l's `step` l elements from `rows`
 // on), of the lanes in `seen`, which is not 0.
 template <typename T>
@@ -442,8 +466,11 @@ __device__ __forceinline__ void add_rows(Two& sum, float f, const S_<T>* rows, i
     const int first = __ffsll(static_cast<unsigned long long>(seen)) - 1;
 #pragma unroll 16
     for (int l = 0; l < kWave; ++l) {
-        const bool in = seen >> l & 1;
-        add_two(sum, in ? from_lane(f, l) : 0.0f, two_of<T>(rows + (in ? l : first) * step, dim));
+        // (bits, not a branch: the loads go out together)
+        const uint32_t in = -static_cast<uint32_t>(seen >> l & 1);
+        const Two v = two_of<T>(rows + (in ? l : first) * step, dim);
+        auto part = [&](float x) { return __uint_as_float(__float_as_uint(x) & in); };
+        add_two(sum, part(from_lane(f, l)), Two{part(v.x), part(v.y)});
     }
 }
 
@@ -466,24 +493,27 @@ __device__ __forceinline__ void for_seen(const Rule& r, int p, const F& f) {
     }
 }
 
-// Of the lanes that ask (`bad`, on row `row`): those whose row sees none of the
-// values that are not finite among the keys that rows p0 .. p1 read, where there
-// is one that it does not see.  `rows` is the first key's row of the tensor.
+// Of the lanes that ask (`bad`, on row `row`): those with an element that is not
+// finite in a key which rows p0 .. p1 read and theirs does not see, and in none
+// that theirs sees.  `rows` is the first key's row of the tensor.
 template <typename T>
 __device__ __forceinline__ bool only_beside(const Shape& s, const S_<T>* rows, int64_t step, int p0, int p1, bool bad, int row) {
     const KeyTiles tiles(s.rule, p0, p1, kWave);
     const KeysSeen keep(s.rule, tiles, p1);
-    bool beside = false;
-    for (int i = 0; i < tiles.count && __any(bad); ++i) {
+    const Elements all = all_elements(s.dim);
+    Elements own{0, 0}, beside{0, 0};
+    for (int i = 0; i < tiles.count && __any(bad && !all.all_in(own)); ++i) {
         const int j0 = tiles.at(i) * kWave, mine = j0 + static_cast<int>(threadIdx.x % kWave);
         uint64_t found = __ballot(keep(mine) && !row_is_finite<T>(rows + mine * step, s.dim));
         for (; found != 0; found &= found - 1) {
-            const bool sees = s.rule.sees(row, j0 + __ffsll(static_cast<unsigned long long>(found)) - 1);
-            beside = beside || !sees;
-            bad = bad && !sees;
+            const int j = j0 + __ffsll(static_cast<unsigned long long>(found)) - 1;
+            const Elements odd = odd_elements<T>(rows + j * step, s.dim);
+            const bool sees = s.rule.sees(row, j);
+            own.add(odd, sees);
+            beside.add(odd, !sees);
         }
     }
-    return bad && beside;
+    return bad && !beside.all_in(own);
 }
 
 // f(lane) for the first lane that asks, and again until no lane does that f has

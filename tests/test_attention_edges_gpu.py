@@ -442,3 +442,46 @@ def test_windows_past_64_bits(dev, ops):
         assert_within(got[0].numpy(), want[0].numpy(), 2.0 ** -15 * np.abs(want[0].numpy()).max(), F32, str(rule))
         for g, w in zip(ops.sliding_window_attention_backward(do, q, k, v, *got, **rule), grads):
             assert_within(g.numpy(), w.numpy(), 2.0 ** -13 * np.abs(w.numpy()).max(), F32, str(rule))
+
+
+# ---- several values that are not finite --------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shape", [(1, 200, 200, 2, 1, 64), (1, 6, 500, 4, 2, 96), (2, 200, 200, 128, 64, 40)], ids=str)
+def test_each_element_has_its_own(dev, ops, dtype, shape):
+    """Two values are infinite, in elements 5 and 9: a query that sees the first
+    alone is infinite in 5 and as ever in 9.  The same of two gradients and dv."""
+    b, tq, tk, h, hk, d = shape
+    host = make(dtype, *shape, 130)
+    w = [wide(x, dtype) for x in host]
+    a = Attention(dtype, *w[:3])
+    want, bounds = a.backward(w[3], dtype)
+    group, last = h // hk, tk - 3
+    at = ((tk - tq, 5), (last, 9))  # every query sees the first, two see the second
+    v = host[2].copy()
+    for key, e in at:
+        v[0, key, 0, e] = one(np.inf, dtype)
+    q, k, dv_ = put(host[0], dtype), put(host[1], dtype), put(host[2], dtype)
+    out, _ = ops.sliding_window_attention(q, k, put(v, dtype))
+    o, o64, bound = wide(out.numpy(), dtype), a.tokens(a.out).copy(), a.tokens(a.out_bound).copy()
+    for key, e in at:
+        rows = tk - tq + np.arange(tq) >= key
+        assert np.isposinf(o[0, rows, :group, e]).all()
+        for x in (o, o64, bound):
+            x[0, rows, :group, e] = 0.0
+    assert_within(orc.from_float(o.astype(np.float32), dtype), o64, bound, dtype, "out")
+    # query 1 sees keys up to tk - tq + 1, the last one all keys
+    do = host[3].copy()
+    at = ((1, 5), (tq - 1, 9))
+    for i, e in at:
+        do[0, i, 0, e] = one(np.inf, dtype)
+    out, lse = ops.sliding_window_attention(q, k, dv_)
+    dv = wide(ops.sliding_window_attention_backward(put(do, dtype), q, k, dv_, out, lse)[2].numpy(), dtype)
+    v64, bound = want[2].copy(), bounds[2].copy()
+    for i, e in at:
+        keys = np.arange(tk) <= tk - tq + i
+        assert np.isposinf(dv[0, keys, 0, e]).all()
+        for x in (dv, v64, bound):
+            x[0, keys, 0, e] = 0.0
+    assert_within(orc.from_float(dv.astype(np.float32), dtype), v64, bound, dtype, "dv")
