@@ -243,8 +243,10 @@ int tp_amd_qk_norm_rope(const tp_amd_tensor* query, const tp_amd_tensor* key, co
 /* qk_norm_rope_backward: the gradients of query, key and both weights from
  * those of the results, with the forward's operands and statistics.
  * output_mask (4 ints; NULL = all) selects them; a weight's gradient may be
- * had for the weight NULL (1) too.  No token gives zero weight gradients.
- * Sums in a fixed order. */
+ * had for the weight NULL (1) too.  No token gives zero weight gradients; one
+ * whose position lies outside the table gives NaN in its own rows and, a term of
+ * every sum over tokens, in the weights' (a padded token takes any position
+ * inside).  Sums in a fixed order. */
 int tp_amd_qk_norm_rope_backward(const tp_amd_tensor* grad_query, const tp_amd_tensor* grad_key,
                                  const tp_amd_tensor* query, const tp_amd_tensor* key, const tp_amd_tensor* table,
                                  const tp_amd_tensor* positions, const tp_amd_tensor* query_rstd,

@@ -226,3 +226,20 @@ def test_an_element_that_does_not_turn_stays_by_itself(dev, ops, dtype, dim, rot
     dy[1, 2, 1, at] = 0.0
     _, dw, _, total = head_norm_backward(dy, wide(q, dtype), r.numpy().astype(np.float64), np.ones(dim), tab, pos, interleaved)
     assert_within(grads[2].numpy()[others], dw[others], 70 * U * total[others], dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_gradients_of_positions_outside_the_table(dev, ops, dtype):
+    """NaN in such a token's rows and in the weights' gradients, whatever the
+    gradient; the other tokens' rows as ever."""
+    q, k, dq, dk = (sample((6, 2, 48), dtype, 100 + i) for i in range(4))
+    pos, tab = np.array([0, 3, -1, 9, 10, 4]), table_of(10, 32)
+    outside = (pos < 0) | (pos >= 10)
+    dq[outside] = 0
+    _, _, r, kr = ops.qk_norm_rope(put(q, dtype), put(k, dtype), put(tab), put(pos))
+    grads = ops.qk_norm_rope_backward(put(dq, dtype), put(dk, dtype), put(q, dtype), put(k, dtype), put(tab), put(pos), r, kr)
+    for got, weight, x, dy, stat in ((grads[0], grads[2], q, dq, r), (grads[1], grads[3], k, dk, kr)):
+        dx, _, mag, _ = head_norm_backward(wide(dy, dtype), wide(x, dtype), stat.numpy().astype(np.float64), np.ones(48), tab, pos, False)
+        assert np.isnan(dx[outside]).all()
+        assert_within(got.numpy(), dx, np.nan_to_num(32 * U * mag), dtype)
+        assert np.isnan(wide(weight.numpy(), dtype)).all()
