@@ -291,6 +291,92 @@ int tp_amd_sliding_window_attention_backward(const tp_amd_tensor* grad_out, cons
                                              const tp_amd_tensor* starts, tp_amd_tensor* dquery, tp_amd_tensor* dkey,
                                              tp_amd_tensor* dvalue);
 
+/* ---- between a model's products (no reference counterpart) --------------- */
+
+/* seeded_dropout: native_dropout without the mask.  Element e of input in
+ * row-major order is kept when the generator of tp_amd_launch_dropout, under
+ * the key ``seed`` and this ``offset``, draws a uniform >= p for it: at offset
+ * 0 the bits of native_dropout under that seed.  out = kept ? input / (1 - p)
+ * : 0.  Nothing is stored: the backward draws again.  ``seed_tensor`` (one
+ * int64 on the device, NULL: none) takes the place of ``seed`` when the kernel
+ * runs, so a recorded step whose seed is rewritten between replays draws anew
+ * (the backward has to see the value that its forward saw); offsets tell
+ * calls under one seed apart.  Declined for other dtypes, or a seed of another
+ * kind; an error for p outside [0, 1]. */
+int tp_amd_seeded_dropout(const tp_amd_tensor* input, double p, uint64_t seed, const tp_amd_tensor* seed_tensor,
+                          uint64_t offset, tp_amd_tensor* result);
+/* seeded_dropout_backward: kept ? grad_output / (1 - p) : 0. */
+int tp_amd_seeded_dropout_backward(const tp_amd_tensor* grad_output, double p, uint64_t seed,
+                                   const tp_amd_tensor* seed_tensor, uint64_t offset, tp_amd_tensor* result);
+
+/* residual_norm: the join of a block to its residual stream with the norms on
+ * both sides of it, in one pass.  residual and branch [tokens..., D] of one
+ * float dtype and shape, any strides of merging token axes.  Per row x, y:
+ *   n = y branch_rstd branch_weight, branch_rstd = (mean(y^2) + branch_eps)^-1/2
+ *       (branch_eps < 0: n = y),
+ *   sum = residual_scale x + branch_scale gate drop(n), and
+ *   normed = sum rstd weight, rstd = (mean(sum^2) + eps)^-1/2 (eps < 0: none).
+ * Weights [D] (NULL for 1) and gate (NULL for 1) have the operands' dtype.  The
+ * gate's last axis is D or 1; its token axes, from the right as in
+ * broadcasting, are the residual's first ones and 1 after those: [D],
+ * [B, 1, D], [B, T, D], [B, T, 1], [1].  drop is seeded_dropout with p, seed,
+ * seed_tensor and offset, elements counted over the branch.  branch NULL: only
+ * the norm, of the residual.  Results sum, normed (dense, the operands' dtype),
+ * float32 branch_rstd and rstd [tokens...]; those not taken come back with data
+ * NULL and dtype TP_AMD_UNDEFINED.  float32 arithmetic, rounded once: the norm is
+ * of the sum before its rounding.  Declined for rows wider than 16384, other
+ * dtypes, operands on different devices, or a gate that repeats over an axis
+ * before one it has. */
+int tp_amd_residual_norm(const tp_amd_tensor* residual, const tp_amd_tensor* branch, const tp_amd_tensor* gate,
+                         const tp_amd_tensor* branch_weight, const tp_amd_tensor* weight, double residual_scale,
+                         double branch_scale, double branch_eps, double eps, double p, uint64_t seed,
+                         const tp_amd_tensor* seed_tensor, uint64_t offset, tp_amd_tensor* sum, tp_amd_tensor* normed,
+                         tp_amd_tensor* branch_rstd, tp_amd_tensor* rstd);
+/* residual_norm_backward: the gradients of residual, branch, gate and weights
+ * from those of sum and normed (either may be NULL for none; without a branch
+ * the sum is the residual) with the forward's operands and statistics; a NULL
+ * branch_rstd says that the branch was not normed.  output_mask (5 ints; NULL =
+ * all) selects them; there is none of an operand that is NULL.  A dropped
+ * element has no gradient.  No token gives zero gradients of weights and of a
+ * gate that repeats over tokens.  Sums in a fixed order. */
+int tp_amd_residual_norm_backward(const tp_amd_tensor* grad_sum, const tp_amd_tensor* grad_normed,
+                                  const tp_amd_tensor* residual, const tp_amd_tensor* branch,
+                                  const tp_amd_tensor* branch_rstd, const tp_amd_tensor* rstd, const tp_amd_tensor* gate,
+                                  const tp_amd_tensor* branch_weight, const tp_amd_tensor* weight, double residual_scale,
+                                  double branch_scale, double p, uint64_t seed, const tp_amd_tensor* seed_tensor,
+                                  uint64_t offset, const int* output_mask, tp_amd_tensor* dresidual, tp_amd_tensor* dbranch,
+                                  tp_amd_tensor* dgate, tp_amd_tensor* dbranch_weight, tp_amd_tensor* dweight);
+
+/* token_log_probs: what a model says about given tokens, from one pass over
+ * logits [rows..., V] (any strides of merging row axes) and without a result of
+ * their size.  With P = softmax(scale x) of a row x, scale > 0:
+ *   logprob [rows...] = ln P[targets] (targets [rows...] int32 / int64; NULL:
+ *       not asked for); NaN for a target outside [0, V), which reads nothing,
+ *   entropy [rows...] = - sum P ln P (want_entropy 0: not asked for),
+ *   stats [rows..., 2] = the largest logit, ln of the sum of e^(scale (x -
+ *       largest)): scale stats[0] + stats[1] is the log-sum-exp,
+ *   top_logprobs, top_indices [rows..., top] = the ``top`` likeliest tokens in
+ *       falling order, of equal ones the lower index first; NaN counts above
+ *       every number.
+ * All float32, top_indices int64; what was not asked for comes back with data NULL
+ * and dtype TP_AMD_UNDEFINED.  A row whose target is ignore_index (padding) is
+ * not read: 0 in all its results, -1 in top_indices.  A token whose logit is
+ * -inf has probability 0; a row with a NaN, +inf, or only -inf has NaN for every
+ * number but its largest logit.  Declined for more than 64 alternatives, other
+ * dtypes, or operands on different devices. */
+int tp_amd_token_log_probs(const tp_amd_tensor* logits, const tp_amd_tensor* targets, double scale, int64_t top,
+                           int want_entropy, int64_t ignore_index, tp_amd_tensor* logprob, tp_amd_tensor* entropy,
+                           tp_amd_tensor* stats, tp_amd_tensor* top_logprobs, tp_amd_tensor* top_indices);
+/* token_log_probs_backward: dlogits (the logits' dtype, dense) from the float32
+ * gradients of logprob and entropy (either may be NULL for none) with the
+ * forward's operands, stats and, for grad_entropy, entropy.  The alternatives
+ * have no gradient.  Skipped rows get zeros, a row whose target lies outside
+ * [0, V) NaN. */
+int tp_amd_token_log_probs_backward(const tp_amd_tensor* grad_logprob, const tp_amd_tensor* grad_entropy,
+                                    const tp_amd_tensor* logits, const tp_amd_tensor* targets, const tp_amd_tensor* stats,
+                                    const tp_amd_tensor* entropy, double scale, int64_t ignore_index,
+                                    tp_amd_tensor* result);
+
 /* ---- host-only helpers (Cnnl.cpp:107-205); no device work --------------- */
 
 /* binary_result_dtype (Cnnl.cpp:178-192) for two tensors' dtypes and

@@ -226,6 +226,13 @@ PROTOTYPES = {
                                            T, T, T, T]),
     "tp_amd_sliding_window_attention": (i32, [T, T, T, i64, i64, f64, T, T, T, T]),
     "tp_amd_sliding_window_attention_backward": (i32, [T, T, T, T, T, T, i64, i64, f64, T, T, T, T, T]),
+    "tp_amd_seeded_dropout": (i32, [T, f64, u64, T, u64, T]),
+    "tp_amd_seeded_dropout_backward": (i32, [T, f64, u64, T, u64, T]),
+    "tp_amd_residual_norm": (i32, [T, T, T, T, T, f64, f64, f64, f64, f64, u64, T, u64, T, T, T, T]),
+    "tp_amd_residual_norm_backward": (i32, [T, T, T, T, T, T, T, T, T, f64, f64, f64, u64, T, u64, C.POINTER(C.c_int),
+                                            T, T, T, T, T]),
+    "tp_amd_token_log_probs": (i32, [T, T, f64, i64, i32, i64, T, T, T, T, T]),
+    "tp_amd_token_log_probs_backward": (i32, [T, T, T, T, T, T, f64, i64, T]),
     "tp_amd_binary_result_dtype": (i32, [i32, i32, i32, i32]),
     "tp_amd_broadcast_shape": (i32, [I64P, i32, I64P, i32, I64P, C.POINTER(C.c_int)]),
     "tp_amd_is_dense": (i32, [T]),

@@ -319,3 +319,12 @@ constexpr uint32_t kOutOfRange = 0xfffffff0u;  // an offset past any resource us
 __device__ __forceinline__ void drain() { __builtin_amdgcn_s_waitcnt(0); }
 
 }  // namespace tp_amd
+
+// FN<T>(...) for a native float dtype.
+#define TP_AMD_DISPATCH_TYPED(dtype, FN, ...)                       \
+    switch (dtype) {                                                \
+        case TP_AMD_FLOAT32: FN<float>(__VA_ARGS__); break;         \
+        case TP_AMD_FLOAT16: FN<f16_t>(__VA_ARGS__); break;         \
+        case TP_AMD_BFLOAT16: FN<bf16_t>(__VA_ARGS__); break;       \
+        default: TP_AMD_CHECK(false, "unsupported dtype ", dtype_name(dtype)); \
+    }

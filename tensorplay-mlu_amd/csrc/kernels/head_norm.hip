@@ -441,24 +441,16 @@ void backward_typed(const HeadNormArgs& p, int device) {
 
 }  // namespace
 
-#define TP_AMD_DISPATCH_FLOAT(dtype, FN, ...)                       \
-    switch (dtype) {                                                \
-        case TP_AMD_FLOAT32: FN<float>(__VA_ARGS__); break;         \
-        case TP_AMD_FLOAT16: FN<f16_t>(__VA_ARGS__); break;         \
-        case TP_AMD_BFLOAT16: FN<bf16_t>(__VA_ARGS__); break;       \
-        default: TP_AMD_CHECK(false, "unsupported dtype ", dtype_name(dtype)); \
-    }
-
 void launch_head_norm(int dtype, const HeadNormArgs& p, int device) {
     check_extent(p);
     const OnDevice scope(device);
-    TP_AMD_DISPATCH_FLOAT(dtype, forward_typed, p, scope.index());
+    TP_AMD_DISPATCH_TYPED(dtype, forward_typed, p, scope.index());
 }
 
 void launch_head_norm_backward(int dtype, const HeadNormArgs& p, int device) {
     check_extent(p);
     const OnDevice scope(device);
-    TP_AMD_DISPATCH_FLOAT(dtype, backward_typed, p, scope.index());
+    TP_AMD_DISPATCH_TYPED(dtype, backward_typed, p, scope.index());
 }
 
 }  // namespace tp_amd

@@ -19,6 +19,7 @@
 #include <type_traits>
 
 #include "device_common.h"
+#include "philox.h"
 #include "../allocator.h"
 #include "../runtime.h"
 #include "tp_amd_kernels.h"
@@ -783,39 +784,7 @@ void layer_norm_backward_typed(int device, int64_t rows, int64_t D, const void* 
     }
 }
 
-// ---- dropout: Philox4x32-10 -------------------------------------------------
-//
-// The counter-based generator of Salmon, Moraes, Dror and Shaw, "Parallel
-// random numbers: as easy as 1, 2, 3" (SC 2011): ten rounds of two 32 x 32
-// -> 64-bit multiplies on a 4-word counter under a 2-word key bumped by the
-// Weyl constants after each round.  Element e of a tensor takes word e % 4
-// of the block for counter (e / 4, 0, offset_lo, offset_hi) under the key
-// (seed_lo, seed_hi); its uniform is (word >> 8) * 2^-24 in [0, 1), and it is
-// kept when the uniform is >= p, decided exactly as word >> 8 >= ceil(p 2^24).
-
-struct Philox {
-    uint32_t c[4];
-};
-
-__device__ __forceinline__ Philox philox4x32_10(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3,
-                                                uint32_t k0, uint32_t k1) {
-    constexpr uint32_t M0 = 0xD2511F53u, M1 = 0xCD9E8D57u, W0 = 0x9E3779B9u, W1 = 0xBB67AE85u;
-#pragma unroll
-    for (int r = 0; r < 10; ++r) {
-        const uint64_t p0 = static_cast<uint64_t>(M0) * c0;
-        const uint64_t p1 = static_cast<uint64_t>(M1) * c2;
-        const uint32_t hi0 = static_cast<uint32_t>(p0 >> 32), lo0 = static_cast<uint32_t>(p0);
-        const uint32_t hi1 = static_cast<uint32_t>(p1 >> 32), lo1 = static_cast<uint32_t>(p1);
-        const uint32_t n0 = hi1 ^ c1 ^ k0, n1 = lo1, n2 = hi0 ^ c3 ^ k1, n3 = lo0;
-        c0 = n0;
-        c1 = n1;
-        c2 = n2;
-        c3 = n3;
-        k0 += W0;
-        k1 += W1;
-    }
-    return Philox{{c0, c1, c2, c3}};
-}
+// ---- dropout: Philox4x32-10 (philox.h) ---------------------------------------
 
 // The keep bits of Philox blocks b0 .. b0 + NB - 1, four elements each.
 template <int NB>
@@ -1745,9 +1714,7 @@ int tp_amd_launch_dropout(int device, int dtype, int64_t n, const void* x, doubl
         const OnDevice scope(device);
         const int index = scope.index();
         const float scale = static_cast<float>(1.0 / (1.0 - p));
-        // p 2^24 is exact in double; a 24-bit uniform u 2^-24 is >= p exactly
-        // when u >= ceil(p 2^24) (at most 2^24, which keeps nothing).
-        const uint32_t threshold = static_cast<uint32_t>(std::ceil(std::ldexp(p, 24)));
+        const uint32_t threshold = keep_threshold(p);
         TP_AMD_DISPATCH_NN(dtype, T, {
             constexpr int N = Packet<T>::N;
             const bool vec = aligned16(x) && aligned16(out) && reinterpret_cast<uintptr_t>(mask) % N == 0;

@@ -7,52 +7,13 @@
 // each other are errors, operands are read where they lie and copied only when
 // the kernels cannot address them.
 
-#include <initializer_list>
-
 #include "../kernels/attention.h"
-#include "tensor.h"
+#include "entries.h"
 #include "tp_amd_ops.h"
 
 using namespace tp_amd;
 
 namespace {
-
-template <typename Body>
-int guarded_results(std::initializer_list<tp_amd_tensor*> slots, Body&& body) noexcept {
-    return guarded([&] {
-        for (tp_amd_tensor* s : slots) TP_AMD_CHECK(s != nullptr, "null result pointer");
-        body();
-    });
-}
-
-void set_undefined(tp_amd_tensor* r) {
-    *r = tp_amd_tensor{};
-    r->dtype = TP_AMD_UNDEFINED;
-    r->device = -1;
-}
-
-bool index_tensor(const TensorRef& t, int device) {
-    return on_device(t) && t.device == device && (t.dtype == TP_AMD_INT64 || t.dtype == TP_AMD_INT32);
-}
-
-// On ``like``'s device with its dtype.
-bool same_kind(const TensorRef& t, const TensorRef& like) { return on_device(t) && t.device == like.device && t.dtype == like.dtype; }
-
-// The first n axes of ``t`` as one index stepping by ``step``: false when
-// they do not merge.
-bool axes_merge(const TensorRef& t, int n, int64_t& step) {
-    bool seen = false;
-    int64_t next = 0;
-    step = 0;
-    for (int d = n - 1; d >= 0; --d) {
-        if (t.sizes[d] == 1) continue;
-        if (seen && t.strides[d] != next) return false;
-        if (!seen) step = t.strides[d];
-        seen = true;
-        next = t.strides[d] * t.sizes[d];
-    }
-    return true;
-}
 
 // ---- norm and rotation of heads -------------------------------------------------
 

@@ -484,6 +484,83 @@ def sliding_window_attention_backward(grad_out, query, key, value, out, lse, win
                          _ref(starts), count=3)
 
 
+# ---- between a model's products (no registration of the reference's) ------------
+
+
+def _seed(seed):
+    """(seed, its tensor): a number, or one int64 in device memory."""
+    if isinstance(seed, DeviceTensor):
+        return 0, C.byref(seed.ref)
+    return int(seed) & 0xFFFFFFFFFFFFFFFF, None
+
+
+def seeded_dropout(input, p, seed, offset=0):  # noqa: A002 - as native_dropout names it
+    """native_dropout in training without its mask: at ``offset`` 0 the same
+    bits under the same ``seed``.  ``seed`` may be a DeviceTensor of one int64,
+    read when the kernel runs: a recorded step draws anew once it is rewritten.
+    ``offset`` tells calls under one seed apart."""
+    return _call_result(L().tp_amd_seeded_dropout, _ref(input), float(p), *_seed(seed), int(offset) & 0xFFFFFFFFFFFFFFFF)
+
+
+def seeded_dropout_backward(grad_output, p, seed, offset=0):
+    """The gradient of input from the forward's p, seed and offset."""
+    return _call_result(L().tp_amd_seeded_dropout_backward, _ref(grad_output), float(p), *_seed(seed),
+                        int(offset) & 0xFFFFFFFFFFFFFFFF)
+
+
+def residual_norm(residual, branch=None, gate=None, branch_weight=None, weight=None, residual_scale=1.0, branch_scale=1.0,
+                  branch_eps=None, eps=1e-6, p=0.0, seed=0, offset=0):
+    """(sum, normed, branch_rstd, rstd) of rows [tokens..., D]:
+    sum = residual_scale residual + branch_scale gate drop(norm(branch)) and
+    normed = norm(sum), norm by the root mean square and times a weight [D].
+    ``branch_eps`` None: the branch is not normed; ``eps`` None: the sum is not;
+    ``branch`` None: the norm of the residual alone.  ``gate``: [D], [B, 1, D],
+    [B, T, D], or with a last axis of 1.  p, seed, offset: seeded_dropout of the
+    branch.  Results not taken are None."""
+    return _call_results(L().tp_amd_residual_norm, _ref(residual), _ref(branch), _ref(gate), _ref(branch_weight), _ref(weight),
+                         float(residual_scale), float(branch_scale), _eps(branch_eps), _eps(eps), float(p), *_seed(seed),
+                         int(offset) & 0xFFFFFFFFFFFFFFFF, count=4)
+
+
+def _eps(eps):
+    """A norm's eps; below zero, no norm."""
+    if eps is None:
+        return -1.0
+    if eps < 0:
+        raise ValueError("a norm's eps is not negative")
+    return float(eps)
+
+
+def residual_norm_backward(grad_sum, grad_normed, residual, branch=None, branch_rstd=None, rstd=None, gate=None,
+                           branch_weight=None, weight=None, residual_scale=1.0, branch_scale=1.0, p=0.0, seed=0, offset=0,
+                           output_mask=(True, True, True, True, True)):
+    """(dresidual, dbranch, dgate, dbranch_weight, dweight) from the gradients
+    of sum and normed (None for none) with the forward's operands and
+    statistics; None where output_mask is False or there is no such operand."""
+    mask = (C.c_int * 5)(*[int(bool(m)) for m in output_mask])
+    return _call_results(L().tp_amd_residual_norm_backward, _ref(grad_sum), _ref(grad_normed), _ref(residual), _ref(branch),
+                         _ref(branch_rstd), _ref(rstd), _ref(gate), _ref(branch_weight), _ref(weight), float(residual_scale),
+                         float(branch_scale), float(p), *_seed(seed), int(offset) & 0xFFFFFFFFFFFFFFFF, mask, count=5)
+
+
+def token_log_probs(logits, targets=None, scale=1.0, top=0, entropy=True, ignore_index=-100):
+    """(logprob, entropy, stats, top_logprobs, top_indices) of rows of logits
+    [rows..., V] under softmax(scale logits): of the given ``targets`` [rows...],
+    and the ``top`` likeliest tokens (at most 64; of equal ones the lower index
+    first).  stats [rows..., 2]: the largest logit and the logarithm of the sum
+    over it, for the backward.  A row whose target is ``ignore_index`` is not
+    read and has 0 for results, -1 for indices.  None where not asked for."""
+    return _call_results(L().tp_amd_token_log_probs, _ref(logits), _ref(targets), float(scale), int(top), int(bool(entropy)),
+                         int(ignore_index), count=5)
+
+
+def token_log_probs_backward(grad_logprob, grad_entropy, logits, targets, stats, entropy=None, scale=1.0, ignore_index=-100):
+    """dlogits from the float32 gradients of logprob and entropy (None for
+    none) with the forward's operands and results."""
+    return _call_result(L().tp_amd_token_log_probs_backward, _ref(grad_logprob), _ref(grad_entropy), _ref(logits), _ref(targets),
+                        _ref(stats), _ref(entropy), float(scale), int(ignore_index))
+
+
 #: The 72 operator names of the reference's registrations (64 on the hot
 #: path, 8 neural-network layers) and the function here that serves each.
 REGISTRATIONS = {
