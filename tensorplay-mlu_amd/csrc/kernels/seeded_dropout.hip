@@ -32,15 +32,18 @@ __global__ __launch_bounds__(kBlock) void seeded_dropout_kernel(const S_<T>* x, 
     const DropKey key(args);
     const int64_t step = static_cast<int64_t>(gridDim.x) * kBlock * N;
     for (int64_t e = (static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x) * N; e < n; e += step) {
-        const uint32_t keep = keep_blocks<N / 4>(key, static_cast<uint64_t>(e) >> 2);
+        // a wave's packets start at a multiple of their length: one high word for all of them
+        const uint64_t block = static_cast<uint64_t>(e) >> 2;
+        const uint32_t keep = keep_blocks<N / 4>(key, static_cast<uint32_t>(block),
+                                                 __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(block >> 32)));
         if (e + N <= n) {
             float f[N];
             unpack<T>(load_raw_any_nt(x + e), f);
 #pragma unroll
-            for (int j = 0; j < N; ++j) f[j] = keep >> j & 1 ? opaque(f[j] * args.scale) : 0.0f;
+            for (int j = 0; j < N; ++j) f[j] = kept(opaque(f[j] * args.scale), keep, j);
             store_raw_any_nt(out + e, pack<T>(f));
         } else {
-            for (int j = 0; e + j < n; ++j) out[e + j] = Elem<T>::store(keep >> j & 1 ? opaque(Elem<T>::load(x[e + j]) * args.scale) : 0.0f);
+            for (int j = 0; e + j < n; ++j) out[e + j] = Elem<T>::store(kept(opaque(Elem<T>::load(x[e + j]) * args.scale), keep, j));
         }
     }
 }
