@@ -51,7 +51,10 @@ __global__ __launch_bounds__(kMaxWaves* kWave) void residual_norm_kernel(Plan w)
     if constexpr (DROP) {
         const DropKey key(w.p.drop);
 #pragma unroll
-        for (int k = 0; k < UPL; ++k) keep[k] = drawn<V>(w, key, r, Place<V>(lane + k * w.lanes, dim).at);
+        for (int k = 0; k < UPL; ++k) {
+            keep[k] = drawn<V>(w, key, r, Place<V>(lane + k * w.lanes, dim).at);
+            now(keep[k]);
+        }
     }
     float z[UPL][V];
     if (!branch) {

@@ -70,7 +70,7 @@ struct Terms {
 
 template <typename T, int V, bool NORM, bool DROP, Gate GATE>
 __device__ __forceinline__ void terms_of(const Plan& w, const Loaded<T, V, GATE>& in, const Raw<T, V>& rw1, const Raw<T, V>& rw2,
-                                         const RowScalars& row, float bs, uint32_t keep, int part, Terms<kPart<V>>& out,
+                                         const RowScalars& row, float bs, uint32_t keep, int bit, int part, Terms<kPart<V>>& out,
                                          float (&dh)[kPart<V>], float (&v)[kPart<V>], float (&t)[kPart<V>]) {
     constexpr int P = kPart<V>;
     float w1[P], w2[P], g[P], x[P];
@@ -84,7 +84,7 @@ __device__ __forceinline__ void terms_of(const Plan& w, const Loaded<T, V, GATE>
 #pragma unroll
     for (int j = 0; j < P; ++j) {
         if constexpr (NORM) out.m1[j] *= row.r1;
-        t[j] = branch_of<NORM, DROP>(out.m1[j], NORM ? w1[j] : 1.0f, bs, keep, part * P + j);
+        t[j] = branch_of<NORM, DROP>(out.m1[j], NORM ? w1[j] : 1.0f, bs, keep, bit + j);
         if constexpr (GATE == kGateRow) t[j] *= g[j];
         out.m2[j] = fmaf(w.p.a, x[j], GATE == kGateOne ? g[j] * t[j] : t[j]) * row.r2;
         v[j] = dh[j] * w2[j];
@@ -160,7 +160,7 @@ __global__ __launch_bounds__(WAVES ? kMaxWaves* kWave : 256, 4) void residual_no
             RowScalars row{1.0f, 0.0f};
             if (there) row = scalars(r);
             Terms<P> terms[HELD ? V / P : 1];
-            uint32_t keep[UPL];
+            uint32_t keep = 0;  // V bits a unit
             float sums[K] = {0.0f, 0.0f, 0.0f};
             if (there) {
 #pragma unroll
@@ -168,12 +168,15 @@ __global__ __launch_bounds__(WAVES ? kMaxWaves* kWave : 256, 4) void residual_no
                     const Place<V> at((HELD ? here : stays(lane)) + k * w.lanes, dim);
                     in.template load<HELD>(w, r, at.at);
                     if (!HELD) weights(at.at);
-                    keep[k] = DROP ? drawn<V>(w, key, r, at.at) : 0;
+                    if constexpr (DROP) {
+                        keep |= (drawn<V>(w, key, r, at.at) & ((1u << V) - 1)) << (k * V);
+                        now(keep);
+                    }
 #pragma unroll
                     for (int i = 0; i < V / P; ++i) {
                         Terms<P>& o = terms[HELD ? i : 0];
                         float dh[P], v[P], t[P];
-                        terms_of<T, V, NORM, DROP, GATE>(w, in, rw1, rw2, row, bs, keep[k], i, o, dh, v, t);
+                        terms_of<T, V, NORM, DROP, GATE>(w, in, rw1, rw2, row, bs, keep, k * V + i * P, i, o, dh, v, t);
 #pragma unroll
                         for (int j = 0; j < P; ++j) {
                             s2[k][i * P + j] = fmaf(dh[j], o.m2[j], s2[k][i * P + j]);
@@ -191,10 +194,11 @@ __global__ __launch_bounds__(WAVES ? kMaxWaves* kWave : 256, 4) void residual_no
                             sums[0] = fmaf(v[j], o.m2[j], sums[0]);
                             if constexpr (NORM || GATE == kGateOne) {
                                 // (a dropped element has no part in a sum, whatever its gradient)
-                                sums[1] = fmaf(t[j], DROP ? kept(o.d[j], keep[k], i * P + j) : o.d[j], sums[1]);
+                                sums[1] = fmaf(t[j], DROP ? kept(o.d[j], keep, k * V + i * P + j) : o.d[j], sums[1]);
                                 sums[2] = fmaf(t[j], o.m2[j], sums[2]);
                             }
                         }
+                        now(sums[0]), now(sums[1]), now(sums[2]);
                         __builtin_amdgcn_sched_barrier(0);  // one part after the other: fewer registers
                     }
                 }
@@ -224,7 +228,7 @@ __global__ __launch_bounds__(WAVES ? kMaxWaves* kWave : 256, 4) void residual_no
                     Terms<P>& o = terms[HELD ? i : 0];
                     if constexpr (!HELD) {
                         float dh[P], v[P], t[P];
-                        terms_of<T, V, NORM, DROP, GATE>(w, in, rw1, rw2, row, bs, keep[k], i, o, dh, v, t);
+                        terms_of<T, V, NORM, DROP, GATE>(w, in, rw1, rw2, row, bs, keep, k * V + i * P, i, o, dh, v, t);
                     }
                     float w1[P], g[P];
                     if constexpr (NORM) expand_part<T, V>(rw1, i, w1);
@@ -235,7 +239,7 @@ __global__ __launch_bounds__(WAVES ? kMaxWaves* kWave : 256, 4) void residual_no
                         const float G = fmaf(-cr, o.m2[j], o.d[j]);
                         dx[e] = w.p.a * G;
                         float E = bs * G;
-                        if constexpr (DROP) E = kept(E, keep[k], e);
+                        if constexpr (DROP) E = kept(E, keep, k * V + e);
                         dy[e] = E;
                         if constexpr (GATE != kNoGate) dy[e] *= g[j];
                         if constexpr (NORM || GATE != kNoGate) {

@@ -4,8 +4,8 @@
 //
 // A team of threads owns a row, UPL units of V elements a thread: lanes of one
 // wave for rows of up to 64 units (no barrier), whole waves for wider ones,
-// several teams a block where they fit.  V is a 16-byte packet, half of one for
-// rows of more than 1024 packets, or one element for rows shorter than that.  The unit that ends a row starts
+// several teams a block where they fit.  V is a 16-byte packet, or one element
+// for rows shorter than that.  The unit that ends a row starts
 // early enough to be whole: the elements that it shares with the unit before
 // it are computed twice, to the same bits, and left out of sums.
 #pragma once
@@ -43,60 +43,21 @@ struct Plan {
     float *part1, *part2, *part_gate;  // [blocks][dim]; the gate's [blocks][dim or 1]
 };
 
-// A unit as it lies: 16 or 8 bytes, or one element.
+// A unit as it lies: a packet, or one element.
 template <typename T, int V>
-using Raw = std::conditional_t<V == 1, S_<T>, std::conditional_t<V * sizeof(S_<T>) == 16, uint4, uint2>>;
-
-typedef unsigned int U32x2Any __attribute__((ext_vector_type(2), aligned(2)));
+using Raw = std::conditional_t<V == 1, S_<T>, uint4>;
 
 // At any element address; ONCE: nothing of it is read again.
 template <typename T, int V, bool ONCE>
 __device__ __forceinline__ Raw<T, V> load_unit(const S_<T>* p) {
-    if constexpr (V == 1) {
-        return *p;
-    } else if constexpr (sizeof(Raw<T, V>) == 16) {
-        return ONCE ? load_raw_any_nt(p) : load_raw_any(p);
-    } else {
-        const auto* q = reinterpret_cast<const U32x2Any*>(p);
-        const U32x2Any v = ONCE ? __builtin_nontemporal_load(q) : *q;
-        return make_uint2(v[0], v[1]);
-    }
-}
-
-// Two words' worth of elements as float32 and back.
-template <typename T, int N>
-__device__ __forceinline__ void expand_words(uint32_t a, uint32_t b, float (&f)[N]) {
-    if constexpr (sizeof(S_<T>) == 4) {
-        f[0] = __uint_as_float(a), f[1] = __uint_as_float(b);
-    } else if constexpr (std::is_same_v<T, bf16_t>) {
-        f[0] = __uint_as_float(a << 16), f[1] = __uint_as_float(a & 0xffff0000u);
-        f[2] = __uint_as_float(b << 16), f[3] = __uint_as_float(b & 0xffff0000u);
-    } else {
-        f[0] = f16_to_float(static_cast<uint16_t>(a & 0xffffu)), f[1] = f16_to_float(static_cast<uint16_t>(a >> 16));
-        f[2] = f16_to_float(static_cast<uint16_t>(b & 0xffffu)), f[3] = f16_to_float(static_cast<uint16_t>(b >> 16));
-    }
+    if constexpr (V == 1) return *p;
+    else return ONCE ? load_raw_any_nt(p) : load_raw_any(p);
 }
 
 template <typename T, int V>
 __device__ __forceinline__ void expand(const Raw<T, V>& raw, float (&f)[V]) {
     if constexpr (V == 1) f[0] = Elem<T>::load(raw);
-    else if constexpr (sizeof(Raw<T, V>) == 16) unpack<T>(raw, f);
-    else expand_words<T>(raw.x, raw.y, f);
-}
-
-template <typename T, int V>
-__device__ __forceinline__ Raw<T, V> packed(const float (&f)[V]) {
-    if constexpr (V == 1) {
-        return Elem<T>::store(f[0]);
-    } else if constexpr (sizeof(Raw<T, V>) == 16) {
-        return pack<T>(f);
-    } else {
-        float wide[Packet<T>::N] = {};
-#pragma unroll
-        for (int j = 0; j < V; ++j) wide[j] = f[j];
-        const uint4 raw = pack<T>(wide);
-        return make_uint2(raw.x, raw.y);
-    }
+    else unpack<T>(raw, f);
 }
 
 template <typename T, int V>
@@ -104,7 +65,8 @@ __device__ __forceinline__ Raw<T, V> ones() {
     float f[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) f[j] = 1.0f;
-    return packed<T, V>(f);
+    if constexpr (V == 1) return Elem<T>::store(f[0]);
+    else return pack<T>(f);
 }
 
 // Keeps what is made of a unit, or of a lane, inside the loop that uses it: made
@@ -113,15 +75,17 @@ __device__ __forceinline__ Raw<T, V> ones() {
 template <typename R>
 __device__ __forceinline__ void stay(R& raw) {
     if constexpr (sizeof(R) == 16) asm volatile("" : "+v"(raw.x), "+v"(raw.y), "+v"(raw.z), "+v"(raw.w));
-    else if constexpr (sizeof(R) == 8) asm volatile("" : "+v"(raw.x), "+v"(raw.y));
 }
 __device__ __forceinline__ int stays(int lane) {
     asm volatile("" : "+v"(lane));
     return lane;
 }
-// A sum that is needed a row later, added here and not where its operands
-// would have to wait for it.
-__device__ __forceinline__ void now(float& v) { asm volatile("" : "+v"(v)); }
+// A value that is needed later (a sum a row later, keep bits a phase later),
+// made here and not where its operands would have to wait for it.
+template <typename F>
+__device__ __forceinline__ void now(F& v) {
+    asm volatile("" : "+v"(v));
+}
 
 // Elements of a unit that are worked on at a time, so that what they need fits
 // the registers beside what stays: four, half a 16-bit packet.
@@ -131,21 +95,24 @@ constexpr int kPart = V < 4 ? V : 4;
 // Part i of a unit as float32.
 template <typename T, int V>
 __device__ __forceinline__ void expand_part(const Raw<T, V>& raw, int i, float (&f)[kPart<V>]) {
-    if constexpr (kPart<V> == V) expand<T, V>(raw, f);
-    else expand_words<T>(i ? raw.z : raw.x, i ? raw.w : raw.y, f);
+    if constexpr (kPart<V> == V) {
+        expand<T, V>(raw, f);
+    } else {
+        const uint32_t a = i ? raw.z : raw.x, b = i ? raw.w : raw.y;
+        if constexpr (std::is_same_v<T, bf16_t>) {
+            f[0] = __uint_as_float(a << 16), f[1] = __uint_as_float(a & 0xffff0000u);
+            f[2] = __uint_as_float(b << 16), f[3] = __uint_as_float(b & 0xffff0000u);
+        } else {
+            f[0] = f16_to_float(static_cast<uint16_t>(a & 0xffffu)), f[1] = f16_to_float(static_cast<uint16_t>(a >> 16));
+            f[2] = f16_to_float(static_cast<uint16_t>(b & 0xffffu)), f[3] = f16_to_float(static_cast<uint16_t>(b >> 16));
+        }
+    }
 }
 
 template <typename T, int V>
 __device__ __forceinline__ void store_unit(S_<T>* p, const float (&f)[V]) {
-    if constexpr (V == 1) {
-        *p = Elem<T>::store(f[0]);
-    } else if constexpr (sizeof(Raw<T, V>) == 16) {
-        store_raw_any_nt(p, packed<T, V>(f));
-    } else {
-        const uint2 raw = packed<T, V>(f);
-        const U32x2Any v = {raw.x, raw.y};
-        __builtin_nontemporal_store(v, reinterpret_cast<U32x2Any*>(p));
-    }
+    if constexpr (V == 1) *p = Elem<T>::store(f[0]);
+    else store_raw_any_nt(p, pack<T>(f));
 }
 
 // A unit's first element and how many of its first ones are not its own.
@@ -182,8 +149,7 @@ __device__ __forceinline__ Raw<T, V> load_gate(const Plan& w, int64_t r, int at)
     } else {
         const uint32_t one = sizeof(S_<T>) == 4 ? __builtin_bit_cast(uint32_t, static_cast<float>(Elem<T>::load(*row)))
                                                 : static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(row)) * 0x10001u;
-        if constexpr (sizeof(Raw<T, V>) == 16) return make_uint4(one, one, one, one);
-        else return make_uint2(one, one);
+        return make_uint4(one, one, one, one);
     }
 }
 
@@ -233,8 +199,7 @@ struct Shape {
     int threads() const { return lanes * teams; }
 };
 
-// Teams of `most` threads a block at most, or one team.  Rows of more packets
-// than a block has threads go in 8-byte units, 16 elements a thread.
+// Teams of `most` threads a block at most, or one team.
 template <typename T>
 Shape shape_of(int dim, int most) {
     constexpr int N = Packet<T>::N;
@@ -246,7 +211,7 @@ Shape shape_of(int dim, int most) {
         s.teams = 256 / s.lanes;
         return s;
     }
-    if (units > kMaxWaves * kWave) s.unit = N / 2, s.upl = 16 / s.unit;
+    if (units > kMaxWaves * kWave) s.upl = 16 / N;
     s.lanes = ((dim + s.unit * s.upl - 1) / (s.unit * s.upl) + kWave - 1) / kWave * kWave;
     s.teams = std::max(1, most / s.lanes);
     return s;
@@ -284,7 +249,7 @@ inline void check_extent(const ResidualNormArgs& p) {
     (!(s).waves      ? ((s).unit == 1 ? TP_AMD_RESIDUAL_FORM(KERNEL, T, 1, 1, false, p)                          \
                                       : TP_AMD_RESIDUAL_FORM(KERNEL, T, Packet<T>::N, 1, false, p))              \
      : (s).upl == 1  ? TP_AMD_RESIDUAL_FORM(KERNEL, T, Packet<T>::N, 1, true, p)                                 \
-                     : TP_AMD_RESIDUAL_FORM(KERNEL, T, Packet<T>::N / 2, 32 / Packet<T>::N, true, p))
+                     : TP_AMD_RESIDUAL_FORM(KERNEL, T, Packet<T>::N, 16 / Packet<T>::N, true, p))
 
 }  // namespace residual
 }  // namespace tp_amd

@@ -8,15 +8,15 @@
 // maximum moves.  Backward, p_j = e^(c (x_j - m)) / S:
 //   dx_j = c (da ([j = t] - p_j) - db p_j (ln p_j + H)).
 //
-// The likeliest tokens come from the same pass.  A block looks at its first
-// chunk's largest element of each thread: the `top`-th largest of those in a
-// wave is a bound that at least `top` elements reach.  Elements that reach the
-// bound go to a list in LDS, in chunks of rising index, so a later element
-// that only equals the bound is never wanted.  Where too many reach it (equal
-// logits) the list is cut down to its best between packets.
+// The likeliest tokens come from the same pass.  A wave holds its 64 best so far
+// sorted, one a lane, and the least of the wanted ones as its bound.  Of a chunk
+// of logits only those above the bound go on, through a list in LDS that is
+// sorted and merged into the best whenever it holds 64.  Where many lanes have one
+// above (a first chunk, a rising row), the `top`-th largest of the lanes' maxima
+// is a bound that `top` elements reach, and comes first.
 //
-// Bound by memory; a row is split over blocks where rows are few, and a second
-// kernel joins the splits.
+// Bound by memory; waves share nothing until their ends meet.  A row is split
+// over blocks where rows are few, and a second kernel joins the splits.
 
 #include <algorithm>
 
@@ -34,7 +34,8 @@ namespace {
 
 constexpr int kBlock = 256;
 constexpr int kWaves = kBlock / kWave;
-constexpr int kUnits = 4;  // packets a thread and chunk
+constexpr int kUnits = 4;  // packets a lane takes at a time: the running maximum moves once for them
+constexpr int kMostSplits = 16;
 constexpr float kLowest = -3.402823466e38f;
 // What an exponent is held above: 2^-4096 is 0 and times a finite number stays 0.
 constexpr float kFloor = -4096.0f;
@@ -70,6 +71,45 @@ __device__ __forceinline__ uint64_t key_of(float v, uint32_t index) {
 }
 __device__ __forceinline__ uint32_t index_of(uint64_t key) { return 0xffffffffu - static_cast<uint32_t>(key); }
 
+// The value of lane ^ STEP (a power of two), or of lane 63 - lane (STEP 63), by
+// moves between registers: a few cycles, where an exchange through LDS takes a
+// hundred and these networks are chains of them.
+template <int STEP>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+    auto dpp = [](uint32_t x, auto control) {
+        return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), decltype(control)::value, 0xf, 0xf, true));
+    };
+    using std::integral_constant;
+    if constexpr (STEP == 1) {
+        return dpp(v, integral_constant<int, 0xb1>{});  // within four lanes: 1 0 3 2
+    } else if constexpr (STEP == 2) {
+        return dpp(v, integral_constant<int, 0x4e>{});  // 2 3 0 1
+    } else if constexpr (STEP == 4) {
+        return dpp(dpp(v, integral_constant<int, 0x1b>{}), integral_constant<int, 0x141>{});  // 3 2 1 0, then eight lanes mirrored
+    } else if constexpr (STEP == 8) {
+        return dpp(v, integral_constant<int, 0x128>{});  // sixteen lanes rotated by 8
+    } else if constexpr (STEP == 16) {
+        // rows 1 and 3 of the one, 0 and 2 of the other change places
+        const auto both = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return threadIdx.x & 16 ? both[0] : both[1];
+    } else if constexpr (STEP == 32) {
+        const auto both = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        return threadIdx.x & 32 ? both[0] : both[1];
+    } else {
+        static_assert(STEP == 63);
+        return lane_xor<32>(lane_xor<16>(dpp(v, integral_constant<int, 0x140>{})));  // sixteen lanes mirrored
+    }
+}
+template <int STEP>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t v) {
+    const uint32_t lo = lane_xor<STEP>(static_cast<uint32_t>(v)), hi = lane_xor<STEP>(static_cast<uint32_t>(v >> 32));
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+template <int STEP>
+__device__ __forceinline__ float lane_xor(float v) {
+    return __uint_as_float(lane_xor<STEP>(__float_as_uint(v)));
+}
+
 // Running statistics: the largest logit, S and E (in powers of two) against it.
 struct Stats {
     float m, s, e;
@@ -84,26 +124,34 @@ __device__ __forceinline__ void join(Stats& a, const Stats& b, float c) {
     a.m = m;
 }
 
+// A wave's lanes as one, in every lane.
+template <int STEP = 1>
+__device__ __forceinline__ void join_lanes(Stats& st, float c) {
+    const Stats other{lane_xor<STEP>(st.m), lane_xor<STEP>(st.s), lane_xor<STEP>(st.e)};
+    join(st, other, c);
+    if constexpr (STEP < kWave / 2) join_lanes<2 * STEP>(st, c);
+}
+
 __device__ __forceinline__ int64_t target_at(const TokenProbsArgs& p, int64_t r) {
     return p.wide_target ? static_cast<const int64_t*>(p.target)[r] : static_cast<const int32_t*>(p.target)[r];
 }
 
+// The logit of a row's target, loaded long before it is needed; NaN for a
+// target outside the row.
+template <typename T>
+__device__ __forceinline__ float target_logit(const Plan& w, int64_t r, int64_t target) {
+    if (target < 0 || target >= w.p.vocab) return __uint_as_float(0x7fc00000u);
+    return Elem<T>::load(static_cast<const S_<T>*>(w.p.logits.data)[r * w.p.logits.step + target]);
+}
+
 // Results of a row from its statistics.  A row without a finite or larger
 // logit has the sum 0 and NaN for results.
-template <typename T>
-__device__ __forceinline__ void write_row(const Plan& w, int64_t r, const Stats& t) {
+__device__ __forceinline__ void write_row(const Plan& w, int64_t r, const Stats& t, float given) {
     const float ls = logf(t.s);
     w.p.stats[2 * r] = t.s == 0.0f ? -__builtin_inff() : t.m;  // every logit -inf
     w.p.stats[2 * r + 1] = ls;
     if (w.p.entropy != nullptr) w.p.entropy[r] = ls - t.e / t.s * kLn2;
-    if (w.p.target != nullptr) {
-        const int64_t at = target_at(w.p, r);
-        float lp = __uint_as_float(0x7fc00000u);
-        if (at >= 0 && at < w.p.vocab) {
-            lp = fmaf(Elem<T>::load(static_cast<const S_<T>*>(w.p.logits.data)[r * w.p.logits.step + at]) - t.m, w.p.scale, -ls);
-        }
-        w.p.logprob[r] = lp;
-    }
+    if (w.p.target != nullptr) w.p.logprob[r] = fmaf(given - t.m, w.p.scale, -ls);
 }
 
 __device__ __forceinline__ void write_top(const Plan& w, int64_t r, int i, uint64_t key, const Stats& t) {
@@ -123,116 +171,177 @@ __device__ __forceinline__ void write_skipped(const Plan& w, int64_t r, int thre
     if (w.p.entropy != nullptr) w.p.entropy[r] = 0.0f;
 }
 
-// A wave's 64 keys in falling order.
-__device__ __forceinline__ uint32_t wave_sorted(uint32_t v) {
+// ---- the likeliest tokens ---------------------------------------------------------
+
+template <typename K>
+__device__ __forceinline__ K larger_of(K a, K b) { return a > b ? a : b; }
+template <typename K>
+__device__ __forceinline__ K smaller_of(K a, K b) { return a < b ? a : b; }
+
+// A bitonic network on a wave's 64 keys, one a lane.  Steps STEP, STEP / 2, ..
+// 1: runs of 2 STEP lanes sorted, falling or, where lane & SIZE, rising (SIZE
+// 64: all falling).
+template <int STEP, int SIZE, typename K>
+__device__ __forceinline__ K bitonic_steps(K v) {
     const int lane = threadIdx.x % kWave;
+    const K other = lane_xor<STEP>(v);
+    const K kept = ((lane & STEP) == 0) == ((lane & SIZE) == 0) ? larger_of(v, other) : smaller_of(v, other);
+    if constexpr (STEP > 1) return bitonic_steps<STEP / 2, SIZE>(kept);
+    else return kept;
+}
+
+// In falling order by lane; LANES: the keys past them are 0.
+template <int LANES = kWave, int SIZE = 2, typename K>
+__device__ __forceinline__ K wave_sorted(K v) {
+    v = bitonic_steps<SIZE / 2, SIZE == LANES ? kWave : SIZE>(v);
+    if constexpr (SIZE < LANES) return wave_sorted<LANES, 2 * SIZE>(v);
+    else return v;
+}
+
+// The 64 largest of two falling lists, falling: the larger of each pair from
+// opposite ends is a bitonic list of them.
+__device__ __forceinline__ uint64_t wave_merged(uint64_t a, uint64_t b) {
+    return bitonic_steps<kWave / 2, kWave>(larger_of(a, lane_xor<kWave - 1>(b)));
+}
+
+// What lanes of one wave wrote to LDS is there for its others.
+__device__ __forceinline__ void wave_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+__device__ __forceinline__ uint64_t lane_key(uint64_t v, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<uint32_t>(v), lane);
+    const uint32_t hi = __builtin_amdgcn_readlane(static_cast<uint32_t>(v >> 32), lane);
+    return static_cast<uint64_t>(hi) << 32 | lo;
+}
+
+// A wave's best keys (0: none yet).
+struct Best {
+    uint64_t key = 0;    // the lane's of the 64 best, falling by lane
+    uint64_t bound = 0;  // keys up to it are not wanted: `top` larger ones are known
+    float reach = __uint_as_float(0x7fc00000u);  // what is less is below the bound's value (NaN: nothing is)
+    uint32_t count = 0;  // keys in the list
+    uint64_t* list;      // 128 keys of LDS
+
+    // The list's first 64 into the best.
+    __device__ __forceinline__ void flush(int top) {
+        const uint32_t lane = threadIdx.x % kWave, kept = count;
+        wave_lds();
+        const uint64_t mine = lane < count ? list[lane] : 0;
+        const uint64_t rest = kWave + lane < count ? list[kWave + lane] : 0;
+        wave_lds();
+        if (kWave + lane < count) list[lane] = rest;
+        count = count > kWave ? count - kWave : 0;
+        const bool few = kept <= 16;
+        key = wave_merged(key, few ? wave_sorted<16>(mine) : wave_sorted<>(mine));
+        raise(lane_key(key, top - 1));
+    }
+
+    __device__ __forceinline__ void raise(uint64_t least) {
+        if (least <= bound) return;
+        bound = least;
+        reach = from_ordered(static_cast<uint32_t>(least >> 32));
+    }
+
+    // One candidate a lane.
+    __device__ __forceinline__ void add(uint64_t candidate, bool wanted, int top) {
+        const uint64_t lanes = __ballot(wanted);
+        if (lanes == 0) return;
+        const uint32_t before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0u));
+        if (wanted) list[count + before] = candidate;
+        count += static_cast<uint32_t>(__popcll(lanes));
+        if (count >= kWave) flush(top);
+    }
+
+    // The elements of a lane's packet, of which those before `end` are there.
+    template <int N>
+    __device__ __forceinline__ void add_packet(const float (&f)[N], int64_t at, int64_t end, int top) {
+        uint32_t left = 0;
 #pragma unroll
-    for (int size = 2; size <= kWave; size *= 2) {
+        for (int j = N - 1; j >= 0; --j) left = left + left + (!(f[j] < reach) ? 1u : 0u);
+        if (at + N > end) left = at < end ? left & ((1u << static_cast<uint32_t>(end - at)) - 1) : 0u;
+        // one element a lane and round: hardly ever more than one or two
+        while (__ballot(left != 0) != 0) {
+            const uint32_t j = __builtin_ctz(left | 1u << 31);
+            float v = f[0];
 #pragma unroll
-        for (int step = size / 2; step > 0; step /= 2) {
-            const uint32_t other = wave_shfl_xor(v, step);
-            const bool low = (lane & step) == 0, falling = (lane & size) == 0;
-            v = (low == falling) ? (v > other ? v : other) : (v < other ? v : other);
+            for (int i = 1; i < N; ++i) v = j == static_cast<uint32_t>(i) ? f[i] : v;
+            const uint64_t candidate = key_of(v, static_cast<uint32_t>(at) + j);
+            add(candidate, left != 0 && candidate > bound, top);
+            left &= left - 1;
         }
     }
-    return v;
-}
-
-__device__ __forceinline__ uint64_t wave_largest(uint64_t v) {
-#pragma unroll
-    for (int m = kWave / 2; m > 0; m /= 2) {
-        const uint64_t other = wave_shfl_xor(v, m);
-        v = v > other ? v : other;
-    }
-    return v;
-}
-
-// The block's list of candidates: `list` holds `n` keys, `bound` the least
-// ordered value worth a look, strictly above it where `strict`.
-template <int CAP>
-struct Candidates {
-    uint64_t list[CAP];
-    uint64_t best[kTokenProbsMaxTop];
-    uint64_t wave_best[kWaves];
-    uint32_t wave_top[kWaves][2];
-    uint32_t n;
 };
 
-// Cuts the list to its `top` best, in falling order.  All threads; the list
-// and n are visible on entry and on return.
-template <int CAP>
-__device__ void cut(Candidates<CAP>& c, int top) {
-    constexpr int PER = (CAP + kBlock - 1) / kBlock;
-    const uint32_t n = c.n;
-    uint64_t mine[PER];
-#pragma unroll
-    for (int i = 0; i < PER; ++i) mine[i] = threadIdx.x + i * kBlock < n ? c.list[threadIdx.x + i * kBlock] : 0;
-    const int want = n < static_cast<uint32_t>(top) ? static_cast<int>(n) : top;
-    for (int k = 0; k < want; ++k) {
-        uint64_t v = 0;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) v = mine[i] > v ? mine[i] : v;
-        v = wave_largest(v);
-        if (threadIdx.x % kWave == 0) c.wave_best[threadIdx.x / kWave] = v;
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) v = c.wave_best[i] > v ? c.wave_best[i] : v;
-        // keys differ (by their index), so one element leaves
-#pragma unroll
-        for (int i = 0; i < PER; ++i) mine[i] = mine[i] == v ? 0 : mine[i];
-        if (threadIdx.x == 0) c.best[k] = v;
-        __syncthreads();
-    }
-    if (threadIdx.x < static_cast<unsigned>(want)) c.list[threadIdx.x] = c.best[threadIdx.x];
-    if (threadIdx.x == 0) c.n = want;
-    __syncthreads();
-}
-
-template <typename T, bool ENTROPY, bool TOP>
+// WAVES waves a row's split: four of a block's, or one.
+template <typename T, int U, int WAVES, bool ENTROPY, bool TOP>
 __global__ __launch_bounds__(kBlock) void token_log_probs_kernel(Plan w) {
-    constexpr int N = Packet<T>::N;
-    constexpr int CAP = kBlock * N + kTokenProbsMaxTop;
+    constexpr int N = Packet<T>::N, kTeam = WAVES * kWave;
+    constexpr int64_t kChunk = kTeam * N * U;
     __shared__ Stats wave_stats[kWaves];
-    __shared__ std::conditional_t<TOP, Candidates<CAP>, int> shared;
-    const int64_t r = blockIdx.x / static_cast<unsigned>(w.splits);
-    const int split = static_cast<int>(blockIdx.x % static_cast<unsigned>(w.splits));
-    if (w.p.target != nullptr && target_at(w.p, r) == w.p.ignore) {
-        if (split == 0) write_skipped(w, r, threadIdx.x, kBlock);
-        return;
+    __shared__ uint64_t lists[TOP ? kWaves : 1][TOP ? 2 * kWave : 1];
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int64_t r = WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * kWaves + wave : blockIdx.x / static_cast<unsigned>(w.splits);
+    const int split = WAVES == 1 ? 0 : static_cast<int>(blockIdx.x % static_cast<unsigned>(w.splits));
+    if (WAVES == 1 && r >= w.p.rows) return;
+    const int mine = WAVES == 1 ? lane : static_cast<int>(threadIdx.x);  // of the team
+    float given = 0.0f;
+    if (w.p.target != nullptr) {
+        const int64_t target = target_at(w.p, r);
+        if (target == w.p.ignore) {
+            if (split == 0) write_skipped(w, r, mine, kTeam);
+            return;
+        }
+        if (w.splits == 1) given = target_logit<T>(w, r, target);
     }
     const int64_t first = split * w.span, end = first + w.span < w.p.vocab ? first + w.span : w.p.vocab;
     const S_<T>* x = static_cast<const S_<T>*>(w.p.logits.data) + r * w.p.logits.step;
+    const int top = w.p.top;
     Stats st{kLowest, 0.0f, 0.0f};
-    uint32_t bound = 0, have = 0;
-    bool strict = false, begun = false;
-    if constexpr (TOP) {
-        if (threadIdx.x == 0) shared.n = 0;
-        __syncthreads();
-    }
-    for (int64_t base = first; base < end; base += kBlock * N * kUnits) {
-        float f[kUnits][N];
-        const int64_t at0 = base + threadIdx.x * N;
-        uint4 raw[kUnits];
+    Best best;
+    if constexpr (TOP) best.list = lists[wave];
+    // unit u of a chunk lies at base + (u kTeam + mine) N: every wave has its share of a last short one
+    uint4 next[U];
+    auto fetch = [&](int64_t base) {
+        if (base + kChunk <= end) {
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-            const int64_t at = at0 + u * kBlock * N;
-            if (at + N <= end) raw[u] = load_raw_any_nt(x + at);
+            for (int u = 0; u < U; ++u) next[u] = load_raw_any_nt(x + base + (u * kTeam + mine) * N);
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int64_t at = base + (u * kTeam + mine) * N;
+                if (at + N <= end) next[u] = load_raw_any_nt(x + at);
+            }
         }
+    };
+    if (first < end) fetch(first);
+    for (int64_t base = first; base < end; base += kChunk) {
+        float f[U][N], um[U];
+        const bool whole = base + kChunk <= end;
+        // units of which this wave has any element
+        const int64_t left = end - base - (WAVES == 1 ? 0 : wave * (kWave * N));
+        const int units = whole ? U : left <= 0 ? 0 : static_cast<int>(min<int64_t>(U, (left + kTeam * N - 1) / (kTeam * N)));
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
-            const int64_t at = at0 + u * kBlock * N;
-            if (at + N <= end) {
-                unpack<T>(raw[u], f[u]);
+        for (int u = 0; u < U; ++u) {
+            if (u >= units) break;
+            const int64_t at = base + (u * kTeam + mine) * N;
+            if (whole || at + N <= end) {
+                unpack<T>(next[u], f[u]);
             } else {
 #pragma unroll
                 for (int j = 0; j < N; ++j) f[u][j] = at + j < end ? Elem<T>::load(x[at + j]) : -__builtin_inff();
             }
         }
-        float cm = f[0][0];
+        if (base + kChunk < end) fetch(base + kChunk);
+        float cm = -__builtin_inff();
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
+        for (int u = 0; u < U; ++u) {
+            if (u >= units) break;
+            um[u] = f[u][0];
 #pragma unroll
-            for (int j = 0; j < N; ++j) cm = larger(cm, f[u][j]);
+            for (int j = 1; j < N; ++j) um[u] = larger(um[u], f[u][j]);
+            cm = larger(cm, um[u]);
         }
         const float m = larger(st.m, cm);
         {
@@ -242,144 +351,122 @@ __global__ __launch_bounds__(kBlock) void token_log_probs_kernel(Plan w) {
             st.m = m;
         }
 #pragma unroll
-        for (int u = 0; u < kUnits; ++u) {
+        for (int u = 0; u < U; ++u) {
+            if (u >= units) break;
 #pragma unroll
             for (int j = 0; j < N; ++j) {
-                const float d = larger((f[u][j] - m) * w.c, kFloor), e = __builtin_amdgcn_exp2f(d);
-                st.s += e;
-                if constexpr (ENTROPY) st.e = fmaf(e, d, st.e);
+                if constexpr (ENTROPY) {
+                    const float d = larger((f[u][j] - m) * w.c, kFloor), e = __builtin_amdgcn_exp2f(d);
+                    st.s += e;
+                    st.e = fmaf(e, d, st.e);
+                } else {
+                    st.s += __builtin_amdgcn_exp2f((f[u][j] - m) * w.c);
+                }
             }
         }
         if constexpr (TOP) {
-            const int top = w.p.top;
-            if (!begun) {
-                const uint32_t sorted = wave_sorted(ordered(cm + 0.0f));
-                const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-                if (lane == top - 1) shared.wave_top[wave][0] = sorted;
-                if (lane == (top + kWaves - 1) / kWaves - 1) shared.wave_top[wave][1] = sorted;
-                __syncthreads();
-                // `top` threads of one wave reach its first number, a quarter as many of every wave the least second one
-                uint32_t most = 0, least = 0xffffffffu;
-#pragma unroll
-                for (int i = 0; i < kWaves; ++i) {
-                    most = shared.wave_top[i][0] > most ? shared.wave_top[i][0] : most;
-                    least = shared.wave_top[i][1] < least ? shared.wave_top[i][1] : least;
-                }
-                bound = most > least ? most : least;
-                begun = true;
+            const uint64_t above = __ballot(!(cm < best.reach));
+            if (__popcll(above) >= top) {
+                const uint32_t reached = __builtin_amdgcn_readlane(wave_sorted(ordered(cm + 0.0f)), top - 1);
+                best.raise((static_cast<uint64_t>(reached) << 32) - 1);
             }
-            auto wanted = [&](float v) {
-                const uint32_t o = ordered(v + 0.0f);
-                return strict ? o > bound : o >= bound;
-            };
-            uint32_t mine = 0;
-            if (wanted(cm)) {
+            if (above != 0) {
 #pragma unroll
-                for (int u = 0; u < kUnits; ++u) {
-#pragma unroll
-                    for (int j = 0; j < N; ++j) mine += at0 + u * kBlock * N + j < end && wanted(f[u][j]) ? 1 : 0;
+                for (int u = 0; u < U; ++u) {
+                    if (u >= units) break;
+                    if (__ballot(!(um[u] < best.reach)) != 0) best.add_packet(f[u], base + (u * kTeam + mine) * N, end, top);
                 }
+                // a closer bound for the chunks to come
+                if (best.count >= static_cast<uint32_t>(top) && base + kChunk < end) best.flush(top);
             }
-            uint32_t place = mine ? atomicAdd(&shared.n, mine) : 0;
-            __syncthreads();
-            const uint32_t total = shared.n;
-            __syncthreads();
-            if (total <= CAP) {
-                if (mine) {
-#pragma unroll
-                    for (int u = 0; u < kUnits; ++u) {
-#pragma unroll
-                        for (int j = 0; j < N; ++j) {
-                            const int64_t at = at0 + u * kBlock * N + j;
-                            if (at < end && wanted(f[u][j])) shared.list[place++] = key_of(f[u][j], static_cast<uint32_t>(at));
-                        }
-                    }
-                }
-            } else {
-                // packet by packet, the list cut to its best before each
-                if (threadIdx.x == 0) shared.n = have;
-                __syncthreads();
-                for (int u = 0; u < kUnits; ++u) {
-                    if (shared.n > static_cast<uint32_t>(top)) {
-                        cut(shared, top);
-                        bound = static_cast<uint32_t>(shared.list[top - 1] >> 32);
-                        strict = true;
-                    }
-                    __syncthreads();
-#pragma unroll
-                    for (int j = 0; j < N; ++j) {
-                        float v = f[0][j];
-#pragma unroll
-                        for (int i = 1; i < kUnits; ++i) v = i == u ? f[i][j] : v;
-                        const int64_t at = at0 + u * kBlock * N + j;
-                        if (at < end && wanted(v)) shared.list[atomicAdd(&shared.n, 1u)] = key_of(v, static_cast<uint32_t>(at));
-                    }
-                    __syncthreads();
-                }
-            }
-            have = total <= CAP ? total : shared.n;
-            // at least `top` elements so far reach the bound, all of lower index than what follows
-            strict = true;
         }
     }
-    // the threads' statistics as one
-#pragma unroll
-    for (int i = 1; i < kWave; i *= 2) {
-        const Stats other{wave_shfl_xor(st.m, i), wave_shfl_xor(st.s, i), wave_shfl_xor(st.e, i)};
-        join(st, other, w.c);
+    join_lanes(st, w.c);
+    if constexpr (TOP) {
+        if (best.count > 0) best.flush(top);
     }
-    if (threadIdx.x % kWave == 0) wave_stats[threadIdx.x / kWave] = st;
-    __syncthreads();
-    st = wave_stats[0];
+    if constexpr (WAVES > 1) {
+        static_assert(WAVES == kWaves && kWaves == 4);
+        if (lane == 0) wave_stats[wave] = st;
+        if constexpr (TOP) {
+            wave_lds();
+            best.list[lane] = best.key;
+        }
+        __syncthreads();
+        st = wave_stats[0];
 #pragma unroll
-    for (int i = 1; i < kWaves; ++i) join(st, wave_stats[i], w.c);
-    if constexpr (TOP) cut(shared, w.p.top);
+        for (int i = 1; i < kWaves; ++i) join(st, wave_stats[i], w.c);
+        if constexpr (TOP) {
+            if (wave % 2 == 0) {
+                best.key = wave_merged(best.key, lists[wave + 1][lane]);
+                if (wave == 2) best.list[lane] = best.key;
+            }
+            __syncthreads();
+            if (wave == 0) best.key = wave_merged(best.key, lists[2][lane]);
+        }
+        if (wave != 0) return;
+    }
     if (w.splits == 1) {
-        if (threadIdx.x == 0) write_row<T>(w, r, st);
-        if constexpr (TOP) {
-            if (threadIdx.x < static_cast<unsigned>(w.p.top)) write_top(w, r, threadIdx.x, shared.list[threadIdx.x], st);
-        }
+        if (lane == 0) write_row(w, r, st, given);
+        if (TOP && lane < top) write_top(w, r, lane, best.key, st);
         return;
     }
     const int64_t at = r * w.splits + split;
-    if (threadIdx.x == 0) {
+    if (lane == 0) {
         w.part[3 * at] = st.m;
         w.part[3 * at + 1] = st.s;
         w.part[3 * at + 2] = st.e;
     }
-    if constexpr (TOP) {
-        const unsigned n = shared.n;
-        if (threadIdx.x < static_cast<unsigned>(w.p.top)) w.part_top[at * w.p.top + threadIdx.x] = threadIdx.x < n ? shared.list[threadIdx.x] : 0;
-    }
+    if (TOP && lane < top) w.part_top[at * top + lane] = best.key;
 }
 
-// A wave joins a row's splits, one a lane; the best of the lanes' lists, each
-// in falling order, leave one after another.
+// A block joins a row's splits: their statistics one a lane, their lists one
+// after another by every wave, and the waves' as above.
 template <typename T>
-__global__ __launch_bounds__(kWave) void token_log_probs_join_kernel(Plan w) {
+__global__ __launch_bounds__(kBlock) void token_log_probs_join_kernel(Plan w) {
+    __shared__ uint64_t lists[kWaves][kWave];
     const int64_t r = blockIdx.x;
-    const int lane = threadIdx.x;
-    if (w.p.target != nullptr && target_at(w.p, r) == w.p.ignore) return;
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, top = w.p.top;
+    float given = 0.0f;
+    if (w.p.target != nullptr) {
+        const int64_t target = target_at(w.p, r);
+        if (target == w.p.ignore) return;
+        given = target_logit<T>(w, r, target);
+    }
     Stats st{kLowest, 0.0f, 0.0f};
     const int64_t at = r * w.splits + lane;
     if (lane < w.splits) st = Stats{w.part[3 * at], w.part[3 * at + 1], w.part[3 * at + 2]};
+    uint64_t key = 0;
+    if (top > 0) {
+        uint64_t mine[kMostSplits / kWaves];
 #pragma unroll
-    for (int i = 1; i < kWave; i *= 2) {
-        const Stats other{wave_shfl_xor(st.m, i), wave_shfl_xor(st.s, i), wave_shfl_xor(st.e, i)};
-        join(st, other, w.c);
+        for (int i = 0; i < kMostSplits / kWaves; ++i) {
+            const int split = wave + i * kWaves;
+            mine[i] = split < w.splits && lane < top ? w.part_top[(r * w.splits + split) * top + lane] : 0;
+        }
+        key = mine[0];
+#pragma unroll
+        for (int i = 1; i < kMostSplits / kWaves; ++i) {
+            if (wave + i * kWaves < w.splits) key = wave_merged(key, mine[i]);
+        }
+        lists[wave][lane] = key;
     }
-    if (lane == 0) write_row<T>(w, r, st);
-    const int top = w.p.top;
-    int next = 0;
-    for (int k = 0; k < top; ++k) {
-        const uint64_t mine = lane < w.splits && next < top ? w.part_top[at * top + next] : 0;
-        const uint64_t v = wave_largest(mine);
-        if (mine == v) ++next;
-        if (lane == k) write_top(w, r, k, v, st);
+    __syncthreads();
+    if (top > 0) {
+        if (wave % 2 == 0) {
+            key = wave_merged(key, lists[wave + 1][lane]);
+            if (wave == 2) lists[2][lane] = key;
+        }
+        __syncthreads();
+        if (wave == 0) key = wave_merged(key, lists[2][lane]);
     }
+    if (wave != 0) return;
+    join_lanes(st, w.c);
+    if (lane == 0) write_row(w, r, st, given);
+    if (lane < top) write_top(w, r, lane, key, st);
 }
 
-// dx of kUnits packets a thread; a row's blocks follow one another.
+// dx of a span a block; a row's blocks follow one another.
 template <typename T, bool ENTROPY>
 __global__ __launch_bounds__(kBlock) void token_log_probs_backward_kernel(Plan w) {
     constexpr int N = Packet<T>::N;
@@ -425,13 +512,13 @@ __global__ __launch_bounds__(kBlock) void token_log_probs_backward_kernel(Plan w
     }
 }
 
-Plan plan_of(const TokenProbsArgs& p, int packet, int splits) {
+// Rows in at most `splits` spans of whole steps of `step` elements.
+Plan plan_of(const TokenProbsArgs& p, int64_t step, int64_t splits) {
     Plan w{};
     w.p = p;
     w.c = p.scale * kLog2e;
-    const int64_t most = std::max<int64_t>(1, (p.vocab + kBlock * packet - 1) / (kBlock * packet));
-    const int64_t each = (most + std::min<int64_t>(splits, most) - 1) / std::min<int64_t>(splits, most);
-    w.span = each * kBlock * packet;
+    const int64_t steps = (p.vocab + step - 1) / step, most = std::min(std::max<int64_t>(splits, 1), steps);
+    w.span = (steps + most - 1) / most * step;
     w.splits = static_cast<int>((p.vocab + w.span - 1) / w.span);
     return w;
 }
@@ -442,29 +529,36 @@ void check_extent(const TokenProbsArgs& p) {
     TP_AMD_CHECK(p.rows < (int64_t{1} << 30), "token_log_probs: ", p.rows, " rows");
 }
 
-template <typename T>
-void forward_typed(const TokenProbsArgs& p, int device) {
-    // About four blocks a CU; a wave joins a row's splits.
-    const int64_t want = 4 * cu_count(device);
-    Plan w = plan_of(p, Packet<T>::N, static_cast<int>(std::min<int64_t>(kWave, std::max<int64_t>(1, want / p.rows))));
+template <typename T, int U, int WAVES>
+void forward_units(const TokenProbsArgs& p, int64_t splits, int device) {
+    Plan w = plan_of(p, static_cast<int64_t>(WAVES) * kWave * Packet<T>::N * U, std::min<int64_t>(splits, kMostSplits));
     const int64_t parts = w.splits > 1 ? p.rows * w.splits : 0;
     const Workspace lists(static_cast<size_t>(parts) * p.top * sizeof(uint64_t), device);
     const Workspace part(static_cast<size_t>(parts) * 3 * sizeof(float), device);
     w.part_top = static_cast<uint64_t*>(lists.get());
     w.part = static_cast<float*>(part.get());
-    const unsigned blocks = grid_of(p.rows * w.splits, kBlock, "token_log_probs");
-    auto* kernel = p.top > 0 ? (p.entropy != nullptr ? token_log_probs_kernel<T, true, true> : token_log_probs_kernel<T, false, true>)
-                             : (p.entropy != nullptr ? token_log_probs_kernel<T, true, false> : token_log_probs_kernel<T, false, false>);
+    const unsigned blocks = grid_of(WAVES == 1 ? (p.rows + kWaves - 1) / kWaves : p.rows * w.splits, kBlock, "token_log_probs");
+    auto* kernel = p.top > 0 ? (p.entropy != nullptr ? token_log_probs_kernel<T, U, WAVES, true, true> : token_log_probs_kernel<T, U, WAVES, false, true>)
+                             : (p.entropy != nullptr ? token_log_probs_kernel<T, U, WAVES, true, false> : token_log_probs_kernel<T, U, WAVES, false, false>);
     kernel<<<blocks, kBlock, 0, stream(device)>>>(w);
     TP_AMD_HIP_CHECK(hipGetLastError());
     if (w.splits == 1) return;
-    token_log_probs_join_kernel<T><<<static_cast<unsigned>(p.rows), kWave, 0, stream(device)>>>(w);
+    token_log_probs_join_kernel<T><<<static_cast<unsigned>(p.rows), kBlock, 0, stream(device)>>>(w);
     TP_AMD_HIP_CHECK(hipGetLastError());
 }
 
 template <typename T>
+void forward_typed(const TokenProbsArgs& p, int device) {
+    constexpr int64_t kPass = static_cast<int64_t>(kBlock) * Packet<T>::N;  // of a block, a packet a lane
+    const int64_t cus = cu_count(device);
+    if (p.vocab <= 8 * kPass && p.rows >= 16 * cus) forward_units<T, kUnits, 1>(p, 1, device);
+    else if (p.vocab > kMostSplits * kPass || p.rows >= 2 * cus) forward_units<T, kUnits, kWaves>(p, std::max<int64_t>(4 * cus / p.rows, 1), device);
+    else forward_units<T, 1, kWaves>(p, 2 * cus / p.rows, device);
+}
+
+template <typename T>
 void backward_typed(const TokenProbsArgs& p, int device) {
-    const Plan w = plan_of(p, Packet<T>::N * kUnits, 1 << 20);
+    const Plan w = plan_of(p, kBlock * Packet<T>::N * 4, p.vocab);
     const unsigned blocks = grid_of(p.rows * w.splits, kBlock, "token_log_probs_backward");
     auto* kernel = p.db != nullptr ? token_log_probs_backward_kernel<T, true> : token_log_probs_backward_kernel<T, false>;
     kernel<<<blocks, kBlock, 0, stream(device)>>>(w);
