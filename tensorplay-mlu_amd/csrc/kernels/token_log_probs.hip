@@ -16,7 +16,7 @@
 // is a bound that `top` elements reach, and comes first.
 //
 // Bound by memory; waves share nothing until their ends meet.  A row is split
-// over blocks where rows are few, and a second kernel joins the splits.
+// over blocks where rows are few, and its last block to arrive joins the splits.
 
 #include <algorithm>
 
@@ -48,9 +48,20 @@ struct Plan {
     int splits;
     int64_t span;  // elements of a split: whole chunks' packets
     float c;       // scale log2 e
-    float* part;   // [rows][splits][3]
-    uint64_t* part_top;  // [rows][splits][top]
+    uint64_t* part;  // [rows][splits][2 + top]: m and S, E, the best keys
 };
+
+// One arrival counter a row that is split, on a 128-byte line of its own (atomics
+// on one line serialize); zero between launches.  A device's launches are all on
+// one stream.
+constexpr int kCounterStride = 32, kMaxSplitRows = 1024;
+__device__ unsigned int split_counters[kMaxSplitRows * kCounterStride];
+
+// Words written through to, and read from, the level all XCDs share.  Relaxed
+// agent-scope stores are acknowledged there before s_waitcnt vmcnt(0) returns,
+// so they precede the arrival that is counted after it.
+__device__ __forceinline__ void store_shared(uint64_t* at, uint64_t v) { __hip_atomic_store(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ uint64_t load_shared(const uint64_t* at) { return __hip_atomic_load(at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 // The larger; NaN where either is.
 __device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
@@ -150,7 +161,7 @@ __device__ __forceinline__ void write_row(const Plan& w, int64_t r, const Stats&
     const float ls = logf(t.s);
     w.p.stats[2 * r] = t.s == 0.0f ? -__builtin_inff() : t.m;  // every logit -inf
     w.p.stats[2 * r + 1] = ls;
-    if (w.p.entropy != nullptr) w.p.entropy[r] = ls - t.e / t.s * kLn2;
+    if (w.p.entropy != nullptr) w.p.entropy[r] = larger(ls - t.e / t.s * kLn2, 0.0f);  // (rounding may pass 0)
     if (w.p.target != nullptr) w.p.logprob[r] = fmaf(given - t.m, w.p.scale, -ls);
 }
 
@@ -202,6 +213,20 @@ __device__ __forceinline__ K wave_sorted(K v) {
 // opposite ends is a bitonic list of them.
 __device__ __forceinline__ uint64_t wave_merged(uint64_t a, uint64_t b) {
     return bitonic_steps<kWave / 2, kWave>(larger_of(a, lane_xor<kWave - 1>(b)));
+}
+
+// The block's best in wave 0, from the waves'; all threads.
+template <int STRIDE>
+__device__ __forceinline__ uint64_t block_merged(uint64_t key, uint64_t (&lists)[kWaves][STRIDE], int lane, int wave) {
+    static_assert(kWaves == 4);
+    lists[wave][lane] = key;
+    __syncthreads();
+    if (wave % 2 == 0) {
+        key = wave_merged(key, lists[wave + 1][lane]);
+        if (wave == 2) lists[2][lane] = key;
+    }
+    __syncthreads();
+    return wave == 0 ? wave_merged(key, lists[2][lane]) : key;
 }
 
 // What lanes of one wave wrote to LDS is there for its others.
@@ -280,7 +305,8 @@ __global__ __launch_bounds__(kBlock) void token_log_probs_kernel(Plan w) {
     constexpr int N = Packet<T>::N, kTeam = WAVES * kWave;
     constexpr int64_t kChunk = kTeam * N * U;
     __shared__ Stats wave_stats[kWaves];
-    __shared__ uint64_t lists[TOP ? kWaves : 1][TOP ? 2 * kWave : 1];
+    __shared__ uint64_t lists[kWaves][TOP ? 2 * kWave : 1];
+    __shared__ bool last;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int64_t r = WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * kWaves + wave : blockIdx.x / static_cast<unsigned>(w.splits);
     const int split = WAVES == 1 ? 0 : static_cast<int>(blockIdx.x % static_cast<unsigned>(w.splits));
@@ -293,7 +319,7 @@ __global__ __launch_bounds__(kBlock) void token_log_probs_kernel(Plan w) {
             if (split == 0) write_skipped(w, r, mine, kTeam);
             return;
         }
-        if (w.splits == 1) given = target_logit<T>(w, r, target);
+        given = target_logit<T>(w, r, target);
     }
     const int64_t first = split * w.span, end = first + w.span < w.p.vocab ? first + w.span : w.p.vocab;
     const S_<T>* x = static_cast<const S_<T>*>(w.p.logits.data) + r * w.p.logits.step;
@@ -386,84 +412,60 @@ __global__ __launch_bounds__(kBlock) void token_log_probs_kernel(Plan w) {
         if (best.count > 0) best.flush(top);
     }
     if constexpr (WAVES > 1) {
-        static_assert(WAVES == kWaves && kWaves == 4);
+        static_assert(WAVES == kWaves);
         if (lane == 0) wave_stats[wave] = st;
-        if constexpr (TOP) {
-            wave_lds();
-            best.list[lane] = best.key;
-        }
-        __syncthreads();
+        if constexpr (TOP) best.key = block_merged(best.key, lists, lane, wave);
+        else __syncthreads();
         st = wave_stats[0];
 #pragma unroll
         for (int i = 1; i < kWaves; ++i) join(st, wave_stats[i], w.c);
-        if constexpr (TOP) {
-            if (wave % 2 == 0) {
-                best.key = wave_merged(best.key, lists[wave + 1][lane]);
-                if (wave == 2) best.list[lane] = best.key;
+        if (w.splits > 1) {
+            const int words = 2 + top;
+            uint64_t* const parts = w.part + r * w.splits * words;
+            if (wave == 0) {
+                uint64_t* part = parts + split * words;
+                if (lane == 0) {
+                    store_shared(part, static_cast<uint64_t>(__float_as_uint(st.s)) << 32 | __float_as_uint(st.m));
+                    store_shared(part + 1, __float_as_uint(st.e));
+                }
+                if (TOP && lane < top) store_shared(part + 2 + lane, best.key);
+                __builtin_amdgcn_s_waitcnt(0);
             }
             __syncthreads();
-            if (wave == 0) best.key = wave_merged(best.key, lists[2][lane]);
+            if (threadIdx.x == 0) {
+                unsigned int* counter = &split_counters[r * kCounterStride];
+                last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == w.splits - 1u;
+                if (last) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            if (!last) return;
+            // the splits' statistics one a lane, their lists one after another by every wave
+            st = Stats{kLowest, 0.0f, 0.0f};
+            if (lane < w.splits) {
+                const uint64_t ms = load_shared(parts + lane * words), e = load_shared(parts + lane * words + 1);
+                st = Stats{__uint_as_float(static_cast<uint32_t>(ms)), __uint_as_float(static_cast<uint32_t>(ms >> 32)),
+                           __uint_as_float(static_cast<uint32_t>(e))};
+            }
+            if constexpr (TOP) {
+                uint64_t keys[kMostSplits / kWaves];
+#pragma unroll
+                for (int i = 0; i < kMostSplits / kWaves; ++i) {
+                    const int from = wave + i * kWaves;
+                    keys[i] = from < w.splits && lane < top ? load_shared(parts + from * words + 2 + lane) : 0;
+                }
+                best.key = keys[0];
+#pragma unroll
+                for (int i = 1; i < kMostSplits / kWaves; ++i) {
+                    if (wave + i * kWaves < w.splits) best.key = wave_merged(best.key, keys[i]);
+                }
+                best.key = block_merged(best.key, lists, lane, wave);
+            }
+            join_lanes(st, w.c);
         }
         if (wave != 0) return;
     }
-    if (w.splits == 1) {
-        if (lane == 0) write_row(w, r, st, given);
-        if (TOP && lane < top) write_top(w, r, lane, best.key, st);
-        return;
-    }
-    const int64_t at = r * w.splits + split;
-    if (lane == 0) {
-        w.part[3 * at] = st.m;
-        w.part[3 * at + 1] = st.s;
-        w.part[3 * at + 2] = st.e;
-    }
-    if (TOP && lane < top) w.part_top[at * top + lane] = best.key;
-}
-
-// A block joins a row's splits: their statistics one a lane, their lists one
-// after another by every wave, and the waves' as above.
-template <typename T>
-__global__ __launch_bounds__(kBlock) void token_log_probs_join_kernel(Plan w) {
-    __shared__ uint64_t lists[kWaves][kWave];
-    const int64_t r = blockIdx.x;
-    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave, top = w.p.top;
-    float given = 0.0f;
-    if (w.p.target != nullptr) {
-        const int64_t target = target_at(w.p, r);
-        if (target == w.p.ignore) return;
-        given = target_logit<T>(w, r, target);
-    }
-    Stats st{kLowest, 0.0f, 0.0f};
-    const int64_t at = r * w.splits + lane;
-    if (lane < w.splits) st = Stats{w.part[3 * at], w.part[3 * at + 1], w.part[3 * at + 2]};
-    uint64_t key = 0;
-    if (top > 0) {
-        uint64_t mine[kMostSplits / kWaves];
-#pragma unroll
-        for (int i = 0; i < kMostSplits / kWaves; ++i) {
-            const int split = wave + i * kWaves;
-            mine[i] = split < w.splits && lane < top ? w.part_top[(r * w.splits + split) * top + lane] : 0;
-        }
-        key = mine[0];
-#pragma unroll
-        for (int i = 1; i < kMostSplits / kWaves; ++i) {
-            if (wave + i * kWaves < w.splits) key = wave_merged(key, mine[i]);
-        }
-        lists[wave][lane] = key;
-    }
-    __syncthreads();
-    if (top > 0) {
-        if (wave % 2 == 0) {
-            key = wave_merged(key, lists[wave + 1][lane]);
-            if (wave == 2) lists[2][lane] = key;
-        }
-        __syncthreads();
-        if (wave == 0) key = wave_merged(key, lists[2][lane]);
-    }
-    if (wave != 0) return;
-    join_lanes(st, w.c);
     if (lane == 0) write_row(w, r, st, given);
-    if (lane < top) write_top(w, r, lane, key, st);
+    if (TOP && lane < top) write_top(w, r, lane, best.key, st);
 }
 
 // dx of a span a block; a row's blocks follow one another.
@@ -531,19 +533,13 @@ void check_extent(const TokenProbsArgs& p) {
 
 template <typename T, int U, int WAVES>
 void forward_units(const TokenProbsArgs& p, int64_t splits, int device) {
-    Plan w = plan_of(p, static_cast<int64_t>(WAVES) * kWave * Packet<T>::N * U, std::min<int64_t>(splits, kMostSplits));
-    const int64_t parts = w.splits > 1 ? p.rows * w.splits : 0;
-    const Workspace lists(static_cast<size_t>(parts) * p.top * sizeof(uint64_t), device);
-    const Workspace part(static_cast<size_t>(parts) * 3 * sizeof(float), device);
-    w.part_top = static_cast<uint64_t*>(lists.get());
-    w.part = static_cast<float*>(part.get());
+    Plan w = plan_of(p, static_cast<int64_t>(WAVES) * kWave * Packet<T>::N * U, p.rows > kMaxSplitRows ? 1 : std::min<int64_t>(splits, kMostSplits));
+    const Workspace part(w.splits > 1 ? static_cast<size_t>(p.rows * w.splits) * (2 + p.top) * sizeof(uint64_t) : 0, device);
+    w.part = static_cast<uint64_t*>(part.get());
     const unsigned blocks = grid_of(WAVES == 1 ? (p.rows + kWaves - 1) / kWaves : p.rows * w.splits, kBlock, "token_log_probs");
     auto* kernel = p.top > 0 ? (p.entropy != nullptr ? token_log_probs_kernel<T, U, WAVES, true, true> : token_log_probs_kernel<T, U, WAVES, false, true>)
                              : (p.entropy != nullptr ? token_log_probs_kernel<T, U, WAVES, true, false> : token_log_probs_kernel<T, U, WAVES, false, false>);
     kernel<<<blocks, kBlock, 0, stream(device)>>>(w);
-    TP_AMD_HIP_CHECK(hipGetLastError());
-    if (w.splits == 1) return;
-    token_log_probs_join_kernel<T><<<static_cast<unsigned>(p.rows), kBlock, 0, stream(device)>>>(w);
     TP_AMD_HIP_CHECK(hipGetLastError());
 }
 

@@ -539,3 +539,28 @@ def test_recorded_and_replayed(dev, ops):
         assert not np.array_equal(seen[0] == 0, seen[1] == 0)
     finally:
         g.reset()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+def test_entropy_of_a_sure_row(dev, ops, dtype):
+    """Never below 0, whatever rounding makes of a row with one likely token."""
+    x = sample((64, 3001), dtype, 50)
+    x[np.arange(64), np.arange(64) * 7] = bits(np.linspace(10, 60, 64), dtype)
+    h = ops.token_log_probs(put(x, dtype))[1].numpy()
+    want = Probs(wide(x, dtype))
+    assert (h >= 0).all()
+    assert_within(h, want.h, want.h_bound, F32)
+
+
+@pytest.mark.parametrize("shape", [(2, 0, 3), (0, 2), (2, 3, 0)], ids=str)
+def test_token_axes_without_a_token(dev, ops, shape):
+    """An axis of no tokens anywhere among the others."""
+    x = put(np.zeros((*shape, 16), np.float32))
+    z, h, _, r = ops.residual_norm(x, x)
+    assert z.shape == h.shape == (*shape, 16) and r.shape == shape
+    got = ops.token_log_probs(x, put(np.zeros(shape, np.int64)))
+    assert got[0].shape == shape and got[2].shape == (*shape, 2)
+    q = put(np.zeros((*shape, 4, 16), np.float32))
+    table = put(np.ones((5, 16), np.float32))
+    out = ops.qk_norm_rope(q, q, table, put(np.zeros(shape[-1:], np.int64)))
+    assert out[0].shape == (*shape, 4, 16) and out[2].shape == (*shape, 4)
