@@ -8,13 +8,21 @@
 // c, and q w1 m1 = g u G: the row's sums need no G, sum(g u G) = sum(g u d) -
 // c r2 sum(g u m2), and all go through one exchange (one barrier a row).
 //
-// Bound by memory: x, y, dz and dh are read once, dx and dy written once.
 // Teams walk rows and keep their columns' running sums: of dh m2, and of E m1
 // with E = b G / (1 - p) where kept, which is both dw1 = sum g E m1 and dg =
 // sum w1 E m1 where the rows of a walk share their gate (the rows of one gate are
-// walked together for that); a block adds its teams' in LDS
-// and writes one float32 row of partials, which a second kernel adds up in
-// block order: the same bits every time.
+// walked together for that).  A block adds its teams' in LDS and writes one
+// float32 row of partials, which a second kernel adds up in block order: the
+// same bits every time.
+//
+// Bound by memory: x, y, dz and dh are read once, dx and dy written once; a row
+// of more than 1024 packets is read a second time, from L2, as its sums and it
+// do not fit the registers.  What was worked on at a time decides: a part of
+// four elements after the other, and the sums made where their terms are
+// (left alone, the compiler moves the additions past the exchange, keeps every
+// term for them and spills).  bf16 8192 x 4096 (403 MB; an elementwise pass of
+// it 65 us): 71 us with one norm, 80 with both and a gate, 88 with dropout too,
+// and 5 us for the fold; 1700 x 16384 102 (54), float32 3003 x 1000 19 (12).
 
 #include "attention.h"
 #include "residual_norm_rows.h"
@@ -349,7 +357,7 @@ __global__ void residual_norm_rows_kernel(S_<T>* zeros, S_<T>* one, int dim) {
 
 template <typename T>
 void backward_typed(const ResidualNormArgs& given, int device) {
-    const Shape s = shape_of<T>(given.dim, 512);
+    const Shape s = shape_of<T>(given.dim, 512, kMaxWaves * kWave);
     // The kernel reads every operand without asking whether it is there: branches
     // around its loads cost registers and the order of the loads.
     ResidualNormArgs p = given;

@@ -173,18 +173,25 @@ __device__ __forceinline__ void team_sums(float (&v)[K], int lanes, float (&red)
         }
     } else {
         const int wave = threadIdx.x / kWave, waves = lanes / kWave, first = wave / waves * waves;
+        const auto plus = [](float a, float b) { return a + b; };
 #pragma unroll
-        for (int k = 0; k < K; ++k) v[k] = wave_allreduce(v[k], [](float a, float b) { return a + b; });
+        for (int k = 0; k < K; ++k) v[k] = wave_allreduce(v[k], plus);
+        if (waves == 1) return;  // (teams of one wave share a block: the same for all)
         if (threadIdx.x % kWave == 0) {
 #pragma unroll
             for (int k = 0; k < K; ++k) red[turn][k][wave] = v[k];
         }
         __syncthreads();
+        // every row of 16 lanes reads the team's sums and adds them up: one trip to LDS
+        const int one = threadIdx.x % kMaxWaves;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
-            float t = 0.0f;
-            for (int i = 0; i < waves; ++i) t += red[turn][k][first + i];
-            v[k] = t;
+            float t = red[turn][k][first + (one < waves ? one : 0)];
+            t = one < waves ? t : 0.0f;
+            t += row_ror<8>(t);
+            t += row_ror<4>(t);
+            t += row_ror<2>(t);
+            v[k] = t + row_ror<1>(t);
         }
         turn ^= 1;
     }
@@ -199,9 +206,10 @@ struct Shape {
     int threads() const { return lanes * teams; }
 };
 
-// Teams of `most` threads a block at most, or one team.
+// Teams of `most` threads a block at most, or one team; rows of more than
+// `single` packets go 16 elements a thread.
 template <typename T>
-Shape shape_of(int dim, int most) {
+Shape shape_of(int dim, int most, int single) {
     constexpr int N = Packet<T>::N;
     Shape s{1, dim < N ? 1 : N, false, 1, 1};
     const int units = (dim + s.unit - 1) / s.unit;
@@ -211,7 +219,7 @@ Shape shape_of(int dim, int most) {
         s.teams = 256 / s.lanes;
         return s;
     }
-    if (units > kMaxWaves * kWave) s.upl = 16 / N;
+    if (units > single) s.upl = 16 / N;
     s.lanes = ((dim + s.unit * s.upl - 1) / (s.unit * s.upl) + kWave - 1) / kWave * kWave;
     s.teams = std::max(1, most / s.lanes);
     return s;

@@ -1,6 +1,11 @@
 // Dropout whose mask is never stored: out = keep ? x / (1 - p) : 0, the keep
 // bits drawn again from the element's place and the seed wherever they are
 // needed, so the backward is the same kernel on the gradient.
+//
+// Bound by memory, the generator (20 products of 32 bits a block of four
+// elements) close behind: bf16 8192 x 4096, 134 MB, 24 us, 5.6 TB/s (an
+// elementwise pass 6.2), 26 before its rounds took three-way xors and a
+// scalar high word.
 
 #include <algorithm>
 
