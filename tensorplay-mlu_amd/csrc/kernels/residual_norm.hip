@@ -132,16 +132,41 @@ __global__ __launch_bounds__(kMaxWaves* kWave) void residual_norm_kernel(Plan w)
     }
 }
 
+// 16-bit rows of a full device whose units lie between a half and three quarters
+// of a power of two of lanes: a quarter of the lanes, three units each.  Lanes
+// that hold nothing draw and wait like the others, and a row's sums take fewer
+// moves.  bf16 with dropout 7812 x 768 16.8 -> 11.8 us, 9983 x 601 21.0 -> 17.8,
+// 5454 x 1100 18.2 -> 16.5; without 11.6 -> 10.1, 13.6 -> 13.4 and 11.9 -> 12.7, so
+// rows without dropout that fill less than three quarters of the units stay as they
+// are.  Not kept: float32 (5.9 M elements: 22.4 -> 21.3 us in rows of 384, 19.8 ->
+// 21.4 of 768), four lanes for rows of 72 (21.4 -> 24.1), and two or four units for
+// powers of two (5859 x 1024 13.7 -> 13.2, 2929 x 2048 14 -> 20).
+inline bool three_units(int units, bool drops, int& lanes) {
+    int few = 16;
+    while (few < kWave && 3 * few < units) few *= 2;
+    if (units <= 2 * few || units > 3 * few || (!drops && 4 * units < 9 * few)) return false;
+    lanes = few;
+    return true;
+}
+
 template <typename T>
 void forward_typed(const ResidualNormArgs& p, int device) {
     // Of rows that fill the device wide ones go to fewer threads, which wait for
     // each other less: bf16 8192 x 4096 with dropout 57 -> 53 us, 3400 x 8192 49 ->
     // 44; eight rows of 4096 3.2 us by 512 threads, 3.6 by 256.
     const bool many = p.rows >= 2 * cu_count(device);
-    const Shape s = shape_of<T>(p.dim, 256, many ? 256 : kMaxWaves * kWave);
+    Shape s = shape_of<T>(p.dim, 256, many ? 256 : kMaxWaves * kWave);
+    bool three = false;
+    if constexpr (sizeof(S_<T>) == 2) {
+        three = many && s.unit > 1 && three_units((p.dim + s.unit - 1) / s.unit, p.drops, s.lanes);
+        if (three) s.upl = 3, s.waves = false, s.teams = 256 / s.lanes;
+    }
     const Plan w = plan_of(p, s);
     const unsigned blocks = grid_of((p.rows + s.teams - 1) / s.teams, s.threads(), "residual_norm");
     auto* kernel = TP_AMD_RESIDUAL_KERNEL(residual_norm_kernel, T, s, p);
+    if constexpr (sizeof(S_<T>) == 2) {
+        if (three) kernel = TP_AMD_RESIDUAL_FORM(residual_norm_kernel, T, Packet<T>::N, 3, false, p);
+    }
     kernel<<<blocks, s.threads(), 0, stream(device)>>>(w);
     TP_AMD_HIP_CHECK(hipGetLastError());
 }

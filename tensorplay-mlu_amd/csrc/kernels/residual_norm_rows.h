@@ -3,7 +3,8 @@
 // threads, and the loads, sums and draws of a row.
 //
 // A team of threads owns a row, UPL units of V elements a thread: lanes of one
-// wave for rows of up to 64 units (no barrier), whole waves for wider ones,
+// wave for rows of up to 64 units (no barrier; of up to 192 in the forward's
+// form of three units a lane), whole waves for wider ones,
 // several teams a block where they fit.  V is a 16-byte packet, or one element
 // for rows shorter than that.  The unit that ends a row starts
 // early enough to be whole: the elements that it shares with the unit before

@@ -179,6 +179,13 @@ def test_join_many_rows(dev, ops, dtype, form, shape):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("form", ["plain", "both_norms", "no_norm", "channel", "full"])
+@pytest.mark.parametrize("dim", [129, 191, 193, 257, 267, 383, 384, 385, 513, 601, 767, 768, 769, 1025, 1100, 1535, 1536, 1537])
+def test_join_many_rows_between_powers_of_two(dev, ops, dtype, form, dim):
+    check_join(ops, dtype, (13, 47, dim), form)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("shape", [(64,), (5, 64), (2, 2, 2, 2, 2, 2, 2, 24)], ids=str)
 def test_join_axes(dev, ops, dtype, shape):
     for form in ("plain", "no_norm", "scalar"):
