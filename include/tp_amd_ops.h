@@ -337,7 +337,8 @@ int tp_amd_residual_norm(const tp_amd_tensor* residual, const tp_amd_tensor* bra
  * the sum is the residual) with the forward's operands and statistics; a NULL
  * branch_rstd says that the branch was not normed.  output_mask (5 ints; NULL =
  * all) selects them; there is none of an operand that is NULL.  A dropped
- * element has no gradient.  No token gives zero gradients of weights and of a
+ * element has no gradient.  Without grad_normed residual and weight are
+ * not read.  No token gives zero gradients of weights and of a
  * gate that repeats over tokens.  Sums in a fixed order. */
 int tp_amd_residual_norm_backward(const tp_amd_tensor* grad_sum, const tp_amd_tensor* grad_normed,
                                   const tp_amd_tensor* residual, const tp_amd_tensor* branch,
@@ -362,7 +363,7 @@ int tp_amd_residual_norm_backward(const tp_amd_tensor* grad_sum, const tp_amd_te
  * and dtype TP_AMD_UNDEFINED.  A row whose target is ignore_index (padding) is
  * not read: 0 in all its results, -1 in top_indices.  A token whose logit is
  * -inf has probability 0; a row with a NaN, +inf, or only -inf has NaN for every
- * number but its largest logit.  Declined for more than 64 alternatives, other
+ * number but its largest logit and, of only -inf, its log-sum-exp, -inf.  Declined for more than 64 alternatives, other
  * dtypes, or operands on different devices. */
 int tp_amd_token_log_probs(const tp_amd_tensor* logits, const tp_amd_tensor* targets, double scale, int64_t top,
                            int want_entropy, int64_t ignore_index, tp_amd_tensor* logprob, tp_amd_tensor* entropy,

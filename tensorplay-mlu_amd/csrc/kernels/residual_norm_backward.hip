@@ -95,6 +95,7 @@ __device__ __forceinline__ void terms_of(const Plan& w, const Loaded<T, V, GATE>
         t[j] = branch_of<NORM, DROP>(out.m1[j], NORM ? w1[j] : 1.0f, bs, keep, bit + j);
         if constexpr (GATE == kGateRow) t[j] *= g[j];
         out.m2[j] = fmaf(w.p.a, x[j], GATE == kGateOne ? g[j] * t[j] : t[j]) * row.r2;
+        if (!w.p.norm2) out.m2[j] = 0.0f;  // (z may be infinite)
         v[j] = dh[j] * w2[j];
         out.d[j] = fmaf(row.r2, v[j], out.d[j]);
     }
@@ -361,14 +362,15 @@ void backward_typed(const ResidualNormArgs& given, int device) {
     // The kernel reads every operand without asking whether it is there: branches
     // around its loads cost registers and the order of the loads.
     ResidualNormArgs p = given;
+    if (!p.norm2) p.x.data = nullptr, p.w2 = nullptr;  // (only the norm's gradient needs them)
     Workspace rows;
     const bool reread = s.upl > 1;
-    if (p.y.data == nullptr || p.dz.data == nullptr || p.dh.data == nullptr || (reread && ((p.norm1 && p.w1 == nullptr) || p.w2 == nullptr))) {
+    if (p.x.data == nullptr || p.y.data == nullptr || p.dz.data == nullptr || p.dh.data == nullptr || (reread && ((p.norm1 && p.w1 == nullptr) || p.w2 == nullptr))) {
         rows = Workspace(2 * sizeof(S_<T>) * p.dim, device);
         S_<T>*zeros = static_cast<S_<T>*>(rows.get()), *one = zeros + p.dim;
         residual_norm_rows_kernel<T><<<(p.dim + 255) / 256, 256, 0, stream(device)>>>(zeros, one, p.dim);
         TP_AMD_HIP_CHECK(hipGetLastError());
-        for (Rows* t : {&p.y, &p.dz, &p.dh}) {
+        for (Rows* t : {&p.x, &p.y, &p.dz, &p.dh}) {
             if (t->data == nullptr) *t = Rows{zeros, 0};
         }
         if (reread && p.w1 == nullptr) p.w1 = one;

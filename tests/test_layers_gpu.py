@@ -338,6 +338,40 @@ def test_join_drops_infinite_gradients(dev, ops, dtype, dim):
     assert_within(dy.numpy(), want["dy"], bound["dy"], dtype)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("gate", [None, "channel", "token"])
+@pytest.mark.parametrize("branch_norm", [False, True], ids=["", "branch_norm"])
+@pytest.mark.parametrize("dim", [36, 1028, 9000])
+def test_join_without_a_gradient_of_its_norm(dev, ops, dtype, dim, branch_norm, gate):
+    """No gradient comes through the sum then: what is not finite in the residual,
+    in the norm's weight, or elsewhere in a row of the branch, reaches none."""
+    shape = (5, dim)
+    x, y, dz = (sample(shape, dtype, 70 + i) for i in range(3))
+    x[1, 3], x[2, dim - 1] = bits([np.inf], dtype)[0], bits([np.nan], dtype)[0]
+    y[3, 5], y[4, 0] = bits([np.inf], dtype)[0], bits([np.nan], dtype)[0]
+    w2 = sample((dim,), dtype, 74, 0.2, 1.0)
+    w2[7] = bits([np.inf], dtype)[0]
+    g = None if gate is None else sample(gate_shape(gate, shape), dtype, 75, 0.4, 0.9)
+    d = [None if v is None else put(v, dtype) for v in (x, y, g, w2, dz)]
+    eps1 = 1e-6 if branch_norm else None
+    for weight in (None, d[3]):
+        _, _, r1, r2 = ops.residual_norm(d[0], d[1], d[2], None, weight, 0.5, 0.75, eps1, None if weight is None else 1e-6)
+        back = ops.residual_norm_backward(d[4], None, d[0], d[1], r1, r2, d[2], None, weight, 0.5, 0.75)
+        # two products, and the rounding to the type
+        assert_within(back[0].numpy(), 0.5 * wide(dz, dtype), 2.0 ** -22 * np.abs(wide(dz, dtype)), dtype, "dx")
+        dy = 0.75 * wide(dz, dtype) * (1.0 if g is None else wide(g, dtype))
+        if not branch_norm:
+            assert_within(back[1].numpy(), dy, 2.0 ** -22 * np.abs(dy), dtype, "dy")
+        gate3 = None if g is None else wide(g, dtype)[:3] if gate == "token" else wide(g, dtype)
+        j = Join(np.zeros((3, dim)), wide(y, dtype)[:3], gate3, a=0.5, b=0.75, eps1=eps1, eps2=None)
+        want, bound = j.backward(wide(dz, dtype)[:3], None, r1.numpy()[:3].astype(np.float64) if branch_norm else None)
+        assert_within(back[1].numpy()[:3], want["dy"], bound["dy"], dtype, "dy")
+        if gate == "token":
+            assert_within(back[2].numpy()[:3], want["dgate"], bound["dgate"], dtype, "dgate")
+        if weight is not None:
+            assert (wide(back[4].numpy(), dtype) == 0).all()
+
+
 # ---- log probabilities --------------------------------------------------------------------
 
 

@@ -1,13 +1,15 @@
 """Dropout of more elements than 2^34: their generator's blocks have numbers
 past 32 bits.  The join's operands are one row expanded, so that only its
-result takes memory."""
+result takes memory.  The join's backward and the log probabilities past 2^31
+elements."""
 
 import numpy as np
 import pytest
 
 from oracle import binding as orc
 
-from _attention import BF16, mod, put, sample, wide
+from _attention import BF16, F32, assert_within, put, sample, wide
+from _layers import Join, Probs
 
 pytestmark = pytest.mark.gpu
 
@@ -53,3 +55,40 @@ def test_dropout(dev, ops, memory):
     for r in (0, (1 << 20) - 1, 1 << 20, ROWS - 1):
         want = np.where(kept_row(r, DIM), wide(x[0], BF16).astype(np.float32) * np.float32(1 / (1 - P)), np.float32(0))
         assert np.array_equal(out[r].numpy(), orc.from_float(want, BF16)), r
+
+
+def test_join_backward(dev, ops, memory):
+    """More than 2^31 elements a tensor; rows differ by what dropout left of them."""
+    width, rows = 4096, (1 << 19) + 9
+    x = ops.seeded_dropout(put(sample((1, width), BF16, 4), BF16).expand(rows, width), P, SEED)
+    y, dz = (put(sample((1, width), BF16, i), BF16).expand(rows, width) for i in (5, 6))
+    z, h, r1, r2 = ops.residual_norm(x, y, branch_eps=1e-6, p=P, seed=SEED, offset=1)
+    dx, dy, _, _, _ = ops.residual_norm_backward(dz, h, x, y, r1, r2, p=P, seed=SEED, offset=1)
+    for r in (0, (1 << 19) - 1, 1 << 19, rows - 1):
+        row = [wide(t[r: r + 1].numpy(), BF16) for t in (x, y, dz, h)]
+        j = Join(row[0], row[1], eps1=1e-6, keep=kept_row(r, width, 1)[None], p=P)
+        assert_within(z[r: r + 1].numpy(), j.z, j.z_bound, BF16, "sum")
+        assert_within(h[r: r + 1].numpy(), j.h, j.h_bound, BF16, "normed")
+        want, bound = j.backward(row[2], row[3], *(t[r: r + 1].numpy().astype(np.float64) for t in (r1, r2)))
+        assert_within(dx[r: r + 1].numpy(), want["dx"], bound["dx"], BF16, "dx")
+        assert_within(dy[r: r + 1].numpy(), want["dy"], bound["dy"], BF16, "dy")
+
+
+def test_log_probs(dev, ops, memory):
+    """More than 2^31 logits."""
+    vocab, rows = 32000, 70001
+    x = ops.seeded_dropout(put(sample((1, vocab), BF16, 7), BF16).expand(rows, vocab), P, SEED)
+    t = np.random.default_rng(8).integers(0, vocab, rows)
+    da, db = (np.random.default_rng(i).standard_normal(rows).astype(np.float32) for i in (9, 10))
+    lp, h, stats, top, index = ops.token_log_probs(x, put(t), top=3, entropy=True)
+    dx = ops.token_log_probs_backward(put(da), put(db), x, put(t), stats, h)
+    for r in (0, (1 << 31) // vocab, (1 << 31) // vocab + 1, rows - 1):
+        want = Probs(wide(x[r: r + 1].numpy(), BF16), t[r: r + 1])
+        given, bound = want.given()
+        assert_within(lp[r: r + 1].numpy(), given, bound, F32, "logprob")
+        assert_within(h[r: r + 1].numpy(), want.h, want.h_bound, F32, "entropy")
+        order, values, bound = want.top(3)
+        assert np.array_equal(index[r: r + 1].numpy(), order)
+        assert_within(top[r: r + 1].numpy(), values, bound, F32, "alternatives")
+        grad, bound = want.backward(da[r: r + 1], db[r: r + 1])
+        assert_within(dx[r: r + 1].numpy(), grad, bound, BF16, "gradient")
