@@ -10,18 +10,19 @@
 //
 // The likeliest tokens come from the same pass.  A wave holds its 64 best so far
 // sorted, one a lane, and the least of the wanted ones as its bound.  Of a chunk
-// of logits only those above the bound go on, through a list in LDS that is
-// sorted and merged into the best whenever it holds 64.  Where many lanes have one
-// above (a first chunk, a rising row), the `top`-th largest of the lanes' maxima
-// is a bound that `top` elements reach, and comes first.
+// of logits only those above the bound go on: one by one where few are wanted,
+// else through a list in LDS that is sorted and merged into the best whenever it
+// holds 64.  Where many lanes have one above (a first chunk, a rising row), the
+// `top`-th largest of the lanes' maxima is a bound that `top` elements reach, and
+// comes first.
 //
 // Bound by memory, with the exponentials' issue close behind for 16-bit logits;
 // waves share nothing until their ends meet, and have their next chunk's loads
 // out.  A row is split over blocks where rows are few, and its last block to
 // arrive joins the splits; many short rows go to a wave each.  bf16 4096 x 32000
 // (262 MB; 42.5 us as an elementwise pass) 48 us, backward (524 MB; 85) 87; 1024 x
-// 128000 with five alternatives 71 (54 without), 8 x 32000 with twenty 10.3,
-// 8000 x 1001 with one 15 (63 by four waves a row).
+// 128000 with five alternatives 65 (54 without), 8 x 32000 with twenty 10.4,
+// 8000 x 1001 with one 13 (63 by four waves a row).
 
 #include <algorithm>
 
@@ -246,7 +247,22 @@ __device__ __forceinline__ uint64_t lane_key(uint64_t v, int lane) {
     return static_cast<uint64_t>(hi) << 32 | lo;
 }
 
-// A wave's best keys (0: none yet).
+// The value of the lane before (lane 0: 0).
+__device__ __forceinline__ uint64_t lane_before(uint64_t v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, static_cast<int>(v), 0x138, 0xf, 0xf, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, static_cast<int>(v >> 32), 0x138, 0xf, 0xf, true);
+    return static_cast<uint64_t>(static_cast<uint32_t>(hi)) << 32 | static_cast<uint32_t>(lo);
+}
+
+// Up to so many wanted, candidates go straight into the best, one after another;
+// of more, through the list: bf16 4096 x 32000 by four waves a row (us, one against
+// the other) one 69 and 85, five 84 and 96, 16 106 and 115, 20 115 and 115, 32 135
+// and 118.  Fewer instructions, but a longer chain of them: few short rows, whose
+// waves wait and do not issue, keep to the list (32 x 32000 with five 14.3 and 14.0).
+constexpr int kInsertTop = 16;
+
+// A wave's best keys (0: none yet).  DIRECT: up to kInsertTop wanted need no list.
+template <bool DIRECT>
 struct Best {
     uint64_t key = 0;    // the lane's of the 64 best, falling by lane
     uint64_t bound = 0;  // keys up to it are not wanted: `top` larger ones are known
@@ -274,10 +290,24 @@ struct Best {
         reach = from_ordered(static_cast<uint32_t>(least >> 32));
     }
 
+    // One key of the wave's into the best.
+    __device__ __forceinline__ void insert(uint64_t one) {
+        const bool greater = key > one;
+        const uint32_t place = static_cast<uint32_t>(__popcll(__ballot(greater)));
+        const uint64_t before = lane_before(key);
+        const uint64_t moved = threadIdx.x % kWave == place ? one : before;
+        key = greater ? key : moved;
+    }
+
     // One candidate a lane.
     __device__ __forceinline__ void add(uint64_t candidate, bool wanted, int top) {
-        const uint64_t lanes = __ballot(wanted);
+        uint64_t lanes = __ballot(wanted);
         if (lanes == 0) return;
+        if (DIRECT && top <= kInsertTop && __popcll(lanes) <= 16) {
+            for (; lanes != 0; lanes &= lanes - 1) insert(lane_key(candidate, __builtin_ctzll(lanes)));
+            raise(lane_key(key, top - 1));
+            return;
+        }
         const uint32_t before = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(lanes >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(lanes), 0u));
         if (wanted) list[count + before] = candidate;
         count += static_cast<uint32_t>(__popcll(lanes));
@@ -330,7 +360,7 @@ __global__ __launch_bounds__(kBlock) void token_log_probs_kernel(Plan w) {
     const S_<T>* x = static_cast<const S_<T>*>(w.p.logits.data) + r * w.p.logits.step;
     const int top = w.p.top;
     Stats st{kLowest, 0.0f, 0.0f};
-    Best best;
+    Best<(U > 1)> best;
     if constexpr (TOP) best.list = lists[wave];
     // unit u of a chunk lies at base + (u kTeam + mine) N: every wave has its share of a last short one
     uint4 next[U];
@@ -397,7 +427,7 @@ __global__ __launch_bounds__(kBlock) void token_log_probs_kernel(Plan w) {
         }
         if constexpr (TOP) {
             const uint64_t above = __ballot(!(cm < best.reach));
-            if (__popcll(above) >= top) {
+            if (__popcll(above) >= (U > 1 && top <= kInsertTop ? top + 6 : top)) {
                 const uint32_t reached = __builtin_amdgcn_readlane(wave_sorted(ordered(cm + 0.0f)), top - 1);
                 best.raise((static_cast<uint64_t>(reached) << 32) - 1);
             }
@@ -552,12 +582,17 @@ template <typename T>
 void forward_typed(const TokenProbsArgs& p, int device) {
     constexpr int64_t kPass = static_cast<int64_t>(kBlock) * Packet<T>::N;  // of a block, a packet a lane
     const int64_t cus = cu_count(device);
-    // A wave a row where rows of few chunks fill the device by themselves; else
-    // a block a split, four packets a lane.  Rows too few to fill it so, and short
-    // enough that sixteen splits of one packet a lane cover them, take those: 8 x
-    // 32000 10.3 us (four splits of four packets 11.0).  Two packets a lane instead
-    // of four: 1024 x 128000 64 us against 54.
-    if (p.vocab <= 8 * kPass && p.rows >= 16 * cus) forward_units<T, kUnits, 1>(p, 1, device);
+    // A wave a row where rows of few chunks fill the device by themselves: 8000 x
+    // 1001 15 us (63 by four), but 8192 x 32000 105 (96).  Alternatives cost every
+    // wave its own bound, list and merges: a wave a row also of longer rows, the
+    // longer the more of them there are: with five 4096 x 32000 76 (86), 8212 x
+    // 65000 242 (258), 4120 x 50257 130 (122).  Else a block a split, four packets a
+    // lane.  Rows too few to fill the device so, and short enough that sixteen splits
+    // of one packet a lane cover them, take those: 8 x 32000 10.4 us (four splits of
+    // four packets 11.0).  Two packets a lane instead of four: 1024 x 128000 64 us
+    // against 54.
+    const int64_t by_wave = p.top > 0 ? std::max<int64_t>(8, p.rows / cus) : 8;
+    if (p.rows >= 16 * cus && p.vocab <= by_wave * kPass) forward_units<T, kUnits, 1>(p, 1, device);
     else if (p.vocab > kMostSplits * kPass || p.rows >= 2 * cus) forward_units<T, kUnits, kWaves>(p, 4 * cus / p.rows, device);
     else forward_units<T, 1, kWaves>(p, 2 * cus / p.rows, device);
 }

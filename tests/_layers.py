@@ -125,9 +125,9 @@ FLUSH = 2.0 ** -125
 
 
 class Probs:
-    """Rows [R, V] of logits (float64 of their type)."""
+    """Rows [R, V] of logits (float64 of their type), summed by `lanes` at least."""
 
-    def __init__(self, x, targets=None, scale=1.0, ignore=-100):
+    def __init__(self, x, targets=None, scale=1.0, ignore=-100, lanes=256):
         self.x, self.t, self.scale = x, targets, scale
         rows, v = x.shape
         self.skipped = np.zeros(rows, bool) if targets is None else targets == ignore
@@ -143,7 +143,7 @@ class Probs:
             far = np.where(np.isfinite(d), -d, 0.0)
             # weights fall as e^d, so e^d |d| sums to what the entropy's own terms do
             size = np.where(np.isfinite(d), e * far, 0.0).sum(1) / self.s
-            chain = 1.25 * v / 256 + 80
+            chain = 1.25 * v / lanes + 80
             srel = (chain + 10 * size) * U
             self.ls_bound = srel + 3 * U * np.abs(self.ls)
             spread = np.where(np.isfinite(d), e * far * far, 0.0).sum(1) / self.s

@@ -380,12 +380,12 @@ def rows_of_logits(rows, vocab, dtype, seed, std=2.5):
     return x
 
 
-def check_probs(ops, dtype, x, targets, scale=1.0, top=0, ignore=-100, view=None, entropy=True, back=True):
+def check_probs(ops, dtype, x, targets, scale=1.0, top=0, ignore=-100, view=None, entropy=True, back=True, lanes=256):
     logits = view if view is not None else put(x, dtype)
     t = None if targets is None else put(targets)
     got = ops.token_log_probs(logits, t, scale, top, entropy, ignore)
     x64 = wide(x, dtype)
-    want = Probs(x64, None if targets is None else targets.astype(np.int64), float(np.float32(scale)), ignore)
+    want = Probs(x64, None if targets is None else targets.astype(np.int64), float(np.float32(scale)), ignore, lanes)
     assert (got[0] is None) == (targets is None) and (got[1] is None) == (not entropy)
     assert (got[3] is None) == (got[4] is None) == (top == 0)
     if targets is not None:
@@ -456,6 +456,31 @@ def test_alternatives_of_equal_and_ordered_logits(dev, ops, dtype, rows, vocab):
                 np.where(np.arange(vocab) < 10, -np.inf, 1.0)):
         x = bits(np.broadcast_to(row, (rows, vocab)), dtype)
         check_probs(ops, dtype, np.ascontiguousarray(x), np.full(rows, vocab - 1), top=20, back=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("top", [1, 4, 16, 17, 64])
+@pytest.mark.parametrize("rows,vocab", [(2, 700), (3, 5000), (2, 40000), (700, 20000)])
+def test_alternatives_of_rising_and_equal_logits(dev, ops, dtype, rows, vocab, top):
+    rng = np.random.default_rng(15)
+    step = np.arange(vocab) * (40.0 / vocab) - 20.0
+    for row in (np.zeros(vocab), step, -step, rng.integers(0, 3, vocab) - 1.0, np.where(np.arange(vocab) % 64 == 63, step, -20.0),
+                np.where(np.arange(vocab) < 10, 1.0, -np.inf), np.where(rng.random(vocab) < 0.01, np.nan, step)):
+        x = bits(np.broadcast_to(row, (rows, vocab)), dtype)
+        check_probs(ops, dtype, np.ascontiguousarray(x), np.full(rows, vocab - 1), top=top, back=False)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("top", [1, 5, 17])
+def test_alternatives_of_many_long_rows(dev, ops, dtype, top):
+    """Rows enough for a wave each."""
+    rows, vocab = 4099, 9001 if dtype == F32 else 17001
+    x = rows_of_logits(64, vocab, dtype, top)
+    x = np.ascontiguousarray(np.concatenate([x] * 65)[:rows])  # (only 64 of them differ)
+    x[7, 100:] = bits([-np.inf], dtype)[0]
+    x[4098] = x[4098][::-1]
+    t = np.random.default_rng(top).integers(0, vocab, rows)
+    check_probs(ops, dtype, x, t, top=top, back=False, lanes=64)
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
