@@ -59,13 +59,23 @@ struct RowScalars {
     float r1, r2;
 };
 
-// u = b drop(m1 w1) of one element, kept by bit j.
-template <bool NORM, bool DROP>
-__device__ __forceinline__ float branch_of(float m1, float w1, float bs, uint32_t keep, int j) {
+// g b drop(m1 w1) of one element, kept by bit j: whatever m1, w1 and g hold, 0
+// where it is dropped.  (A gate that is not finite makes the forward's sum of a
+// dropped element NaN and r2 with it: so are m2 and the norm's gradient here.)
+template <bool NORM, bool DROP, bool GATED>
+__device__ __forceinline__ float branch_of(float m1, float w1, float g, float bs, uint32_t keep, int j) {
     float u = m1 * bs;
     if constexpr (NORM) u *= w1;
+    if constexpr (GATED) u *= g;
     if constexpr (DROP) u = kept(u, keep, j);
     return u;
+}
+
+// A column's or row's sum times the gate or weight it has in common: elements
+// that were all dropped make it 0, whatever that factor holds.
+template <bool DROP>
+__device__ __forceinline__ float shared_factor(float sum, float factor) {
+    return DROP && sum == 0.0f ? 0.0f : sum * factor;
 }
 
 // What a part of a unit gives from its loads and weights: m1, m2 and d = dz +
@@ -92,8 +102,7 @@ __device__ __forceinline__ void terms_of(const Plan& w, const Loaded<T, V, GATE>
 #pragma unroll
     for (int j = 0; j < P; ++j) {
         if constexpr (NORM) out.m1[j] *= row.r1;
-        t[j] = branch_of<NORM, DROP>(out.m1[j], NORM ? w1[j] : 1.0f, bs, keep, bit + j);
-        if constexpr (GATE == kGateRow) t[j] *= g[j];
+        t[j] = branch_of<NORM, DROP, GATE == kGateRow>(out.m1[j], NORM ? w1[j] : 1.0f, GATE == kGateRow ? g[j] : 1.0f, bs, keep, bit + j);
         out.m2[j] = fmaf(w.p.a, x[j], GATE == kGateOne ? g[j] * t[j] : t[j]) * row.r2;
         if (!w.p.norm2) out.m2[j] = 0.0f;  // (z may be infinite)
         v[j] = dh[j] * w2[j];
@@ -223,7 +232,7 @@ __global__ __launch_bounds__(WAVES ? kMaxWaves* kWave : 256, 4) void residual_no
                 one = g[0];
                 if (each && w.p.dgate != nullptr && lane == 0) static_cast<S_<T>*>(w.p.dgate)[r] = Elem<T>::store(tg);
             }
-            const float c1 = one * tg * w.inv_dim;
+            const float c1 = shared_factor<DROP>(tg, one) * w.inv_dim;
 #pragma unroll
             for (int k = 0; k < UPL; ++k) {
                 const Place<V> at((HELD ? here : stays(lane)) + k * w.lanes, dim);
@@ -247,16 +256,16 @@ __global__ __launch_bounds__(WAVES ? kMaxWaves* kWave : 256, 4) void residual_no
                         const int e = i * P + j;
                         const float G = fmaf(-cr, o.m2[j], o.d[j]);
                         dx[e] = w.p.a * G;
-                        float E = bs * G;
-                        if constexpr (DROP) E = kept(E, keep, k * V + e);
-                        dy[e] = E;
-                        if constexpr (GATE != kNoGate) dy[e] *= g[j];
+                        // Of a dropped element every product is masked, not G alone: m1, w1
+                        // and the gate need not be finite.
+                        const auto drop = [&](float v) { return DROP ? kept(v, keep, k * V + e) : v; };
+                        const float E = bs * G, q = GATE != kNoGate ? E * g[j] : E;
                         if constexpr (NORM || GATE != kNoGate) {
-                            se[k][e] = fmaf(GATE != kNoGate && each ? dy[e] : E, o.m1[j], se[k][e]);
+                            se[k][e] = fmaf(drop(GATE != kNoGate && each ? q : E), drop(o.m1[j]), se[k][e]);
                             now(se[k][e]);
                         }
-                        if constexpr (GATE == kGateRow) dg[e] = NORM ? E * o.m1[j] * w1[j] : E * o.m1[j];
-                        if constexpr (NORM) dy[e] = row.r1 * fmaf(-c1, o.m1[j], dy[e] * w1[j]);
+                        if constexpr (GATE == kGateRow) dg[e] = drop(NORM ? E * o.m1[j] * w1[j] : E * o.m1[j]);
+                        dy[e] = NORM ? row.r1 * fmaf(-c1, o.m1[j], drop(q * w1[j])) : drop(q);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -276,11 +285,11 @@ __global__ __launch_bounds__(WAVES ? kMaxWaves* kWave : 256, 4) void residual_no
         if ((NORM && part1 != nullptr) || w.gate_sums) {
             fold_teams<V, UPL>(w, se, stays(lane), team, fold, [&](int d, float t) {
                 if (NORM && part1 != nullptr) {
-                    const float f = GATE == kNoGate || each ? t : t * Elem<T>::load(GATE == kGateOne ? *gate : gate[d]);
+                    const float f = GATE == kNoGate || each ? t : shared_factor<DROP>(t, Elem<T>::load(GATE == kGateOne ? *gate : gate[d]));
                     part1[d] = first ? f : part1[d] + f;
                 }
                 if (GATE == kNoGate || !w.gate_sums) return;
-                if (NORM && w.p.w1 != nullptr) t *= Elem<T>::load(static_cast<const S_<T>*>(w.p.w1)[d]);
+                if (NORM && w.p.w1 != nullptr) t = shared_factor<DROP>(t, Elem<T>::load(static_cast<const S_<T>*>(w.p.w1)[d]));
                 if (GATE == kGateOne) one += t;
                 else if (w.per_group == 1) static_cast<S_<T>*>(w.p.dgate)[group * dim + d] = Elem<T>::store(t);
                 else w.part_gate[static_cast<int64_t>(blockIdx.x) * dim + d] = t;

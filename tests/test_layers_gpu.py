@@ -372,6 +372,65 @@ def test_join_without_a_gradient_of_its_norm(dev, ops, dtype, dim, branch_norm, 
             assert (wide(back[4].numpy(), dtype) == 0).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("gate", ["channel", "sequence", "sequence_one", "token", "full", "one"])
+@pytest.mark.parametrize("dim", [5, 36, 1028, 9000])
+def test_join_gate_of_dropped_elements_that_are_not_finite(dev, ops, dtype, gate, dim):
+    """A dropped element of the branch has no part in the gate's gradient,
+    whatever it holds."""
+    shape = (3, 4, dim)
+    x, y, dz, dh = (sample(shape, dtype, 80 + i) for i in range(4))
+    g, keep = sample(gate_shape(gate, shape), dtype, 84, 0.4, 0.9), kept(0.5, 6, shape)
+    out = np.flatnonzero(~keep)
+    for i, value in enumerate((np.inf, np.nan, -np.inf)):
+        y.reshape(-1)[out[i::7]] = bits([value], dtype)[0]
+    d = [put(v, dtype) for v in (x, y, g, dz, dh)]
+    z, h, _, r2 = ops.residual_norm(d[0], d[1], d[2], p=0.5, seed=6)
+    j = Join(wide(x, dtype), wide(y, dtype), wide(g, dtype).reshape(g.shape), keep=keep, p=0.5)
+    assert_within(z.numpy(), j.z, j.z_bound, dtype)
+    assert_within(h.numpy(), j.h, j.h_bound, dtype)
+    for grad_normed in (d[4], None):
+        got = ops.residual_norm_backward(d[3], grad_normed, d[0], d[1], None, r2, d[2], p=0.5, seed=6)
+        want, bound = j.backward(wide(dz, dtype), None if grad_normed is None else wide(dh, dtype), None, r2.numpy().astype(np.float64))
+        for a, name in zip(got, ("dx", "dy", "dgate")):
+            assert_within(a.numpy(), want[name], bound[name], dtype, name)
+        assert (wide(got[1].numpy(), dtype)[~keep] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("branch_norm", [False, True], ids=["", "branch_norm"])
+@pytest.mark.parametrize("dim", [5, 36, 1028, 9000])
+def test_join_infinite_gate_of_dropped_elements(dev, ops, dtype, dim, branch_norm):
+    """Nor has a dropped element a gradient by a gate or a weight that is not
+    finite."""
+    shape = (3, 4, dim)
+    x, y, dz = (sample(shape, dtype, 90 + i) for i in range(3))
+    w, infinite = sample((dim,), dtype, 93, 0.2, 1.0), bits([np.inf], dtype)[0]
+    eps1, weight = (1e-6, put(w, dtype)) if branch_norm else (None, None)
+    d = [put(v, dtype) for v in (x, y, dz)]
+    # a gate of its own for every element, infinite where that is dropped
+    g, keep = sample(shape, dtype, 94, 0.4, 0.9), kept(0.5, 7, shape)
+    hidden = g.copy()
+    hidden.reshape(-1)[np.flatnonzero(~keep)[::5]] = infinite
+    r1 = ops.residual_norm(d[0], d[1], put(hidden, dtype), weight, None, 1.0, 1.0, eps1, None, 0.5, 7)[2]
+    got = ops.residual_norm_backward(d[2], None, d[0], d[1], r1, None, put(hidden, dtype), weight, p=0.5, seed=7)
+    j = Join(wide(x, dtype), wide(y, dtype), wide(g, dtype), wide(w, dtype) if branch_norm else None, eps1=eps1, eps2=None, keep=keep, p=0.5)
+    want, bound = j.backward(wide(dz, dtype), None, None if r1 is None else r1.numpy().astype(np.float64))
+    for a, name in zip(got, ("dx", "dy", "dgate", "dw1")):
+        assert (a is not None) == (name in want)
+        if a is not None:
+            assert_within(a.numpy(), want[name], bound[name], dtype, name)
+    # every element dropped: no gradient at all but the residual's
+    w[dim // 2] = infinite
+    weight = put(w, dtype) if branch_norm else None
+    for kind in ("channel", "sequence", "sequence_one", "token", "full", "one"):
+        g = np.full(gate_shape(kind, shape), infinite)
+        got = ops.residual_norm_backward(d[2], None, d[0], d[1], r1, None, put(g, dtype), weight, p=1.0, seed=7)
+        assert_within(got[0].numpy(), wide(dz, dtype), 0.0, dtype, "dx")
+        for a in got[1:]:
+            assert a is None or (wide(a.numpy(), dtype) == 0).all(), kind
+
+
 # ---- log probabilities --------------------------------------------------------------------
 
 
