@@ -364,8 +364,9 @@ int tp_amd_residual_norm_backward(const tp_amd_tensor* grad_sum, const tp_amd_te
  * and dtype TP_AMD_UNDEFINED.  A row whose target is ignore_index (padding) is
  * not read: 0 in all its results, -1 in top_indices.  A token whose logit is
  * -inf has probability 0; a row with a NaN, +inf, or only -inf has NaN for every
- * number but its largest logit and, of only -inf, its log-sum-exp, -inf.  Declined for more than 64 alternatives, other
- * dtypes, or operands on different devices. */
+ * number but its largest logit and, of only -inf, its log-sum-exp, -inf.
+ * Declined for more than 64 alternatives, other dtypes, or operands on different
+ * devices; an error from 2^30 rows or 2^31 logits a row on, both directions. */
 int tp_amd_token_log_probs(const tp_amd_tensor* logits, const tp_amd_tensor* targets, double scale, int64_t top,
                            int want_entropy, int64_t ignore_index, tp_amd_tensor* logprob, tp_amd_tensor* entropy,
                            tp_amd_tensor* stats, tp_amd_tensor* top_logprobs, tp_amd_tensor* top_indices);

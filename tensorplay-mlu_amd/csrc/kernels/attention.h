@@ -12,6 +12,9 @@
 
 namespace tp_amd {
 
+// Blocks of so many threads that one launch takes: it counts fewer than 2^32 threads.
+inline int64_t most_blocks(int threads) { return ((int64_t{1} << 32) - 1) / threads; }
+
 // Blocks of a launch, whose threads are counted in 32 bits.
 inline unsigned grid_of(int64_t blocks, int threads, const char* op) {
     TP_AMD_CHECK(blocks * threads < (int64_t{1} << 32), op, ": too many rows for one launch");

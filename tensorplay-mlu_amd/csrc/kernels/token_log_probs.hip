@@ -51,6 +51,7 @@ using S_ = typename Elem<T>::storage;
 
 struct Plan {
     TokenProbsArgs p;
+    int64_t first;  // row of the launch
     int splits;
     int64_t span;  // elements of a split: whole chunks' packets
     float c;       // scale log2 e
@@ -343,7 +344,7 @@ __global__ __launch_bounds__(kBlock) void token_log_probs_kernel(Plan w) {
     __shared__ uint64_t lists[kWaves][TOP ? 2 * kWave : 1];
     __shared__ bool last;
     const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const int64_t r = WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * kWaves + wave : blockIdx.x / static_cast<unsigned>(w.splits);
+    const int64_t r = w.first + (WAVES == 1 ? static_cast<int64_t>(blockIdx.x) * kWaves + wave : blockIdx.x / static_cast<unsigned>(w.splits));
     const int split = WAVES == 1 ? 0 : static_cast<int>(blockIdx.x % static_cast<unsigned>(w.splits));
     if (WAVES == 1 && r >= w.p.rows) return;
     const int mine = WAVES == 1 ? lane : static_cast<int>(threadIdx.x);  // of the team
@@ -507,7 +508,7 @@ __global__ __launch_bounds__(kBlock) void token_log_probs_kernel(Plan w) {
 template <typename T, bool ENTROPY>
 __global__ __launch_bounds__(kBlock) void token_log_probs_backward_kernel(Plan w) {
     constexpr int N = Packet<T>::N;
-    const int64_t r = blockIdx.x / static_cast<unsigned>(w.splits);
+    const int64_t r = w.first + blockIdx.x / static_cast<unsigned>(w.splits);
     const int split = static_cast<int>(blockIdx.x % static_cast<unsigned>(w.splits));
     const int64_t first = split * w.span, end = first + w.span < w.p.vocab ? first + w.span : w.p.vocab;
     const S_<T>* x = static_cast<const S_<T>*>(w.p.logits.data) + r * w.p.logits.step;
@@ -566,16 +567,26 @@ void check_extent(const TokenProbsArgs& p) {
     TP_AMD_CHECK(p.rows < (int64_t{1} << 30), "token_log_probs: ", p.rows, " rows");
 }
 
+// The kernel over all rows, `per_block` of them a block or `splits` blocks each:
+// more of them than one launch takes go in several.
+template <typename Kernel>
+void launch_rows(Kernel* kernel, Plan w, int64_t per_block, int device) {
+    const int64_t at_once = most_blocks(kBlock) / w.splits * per_block;
+    for (w.first = 0; w.first < w.p.rows; w.first += at_once) {
+        const int64_t rows = std::min(at_once, w.p.rows - w.first);
+        kernel<<<static_cast<unsigned>((rows + per_block - 1) / per_block * w.splits), kBlock, 0, stream(device)>>>(w);
+        TP_AMD_HIP_CHECK(hipGetLastError());
+    }
+}
+
 template <typename T, int U, int WAVES>
 void forward_units(const TokenProbsArgs& p, int64_t splits, int device) {
     Plan w = plan_of(p, static_cast<int64_t>(WAVES) * kWave * Packet<T>::N * U, p.rows > kMaxSplitRows ? 1 : std::min<int64_t>(splits, kMostSplits));
     const Workspace part(w.splits > 1 ? static_cast<size_t>(p.rows * w.splits) * (2 + p.top) * sizeof(uint64_t) : 0, device);
     w.part = static_cast<uint64_t*>(part.get());
-    const unsigned blocks = grid_of(WAVES == 1 ? (p.rows + kWaves - 1) / kWaves : p.rows * w.splits, kBlock, "token_log_probs");
     auto* kernel = p.top > 0 ? (p.entropy != nullptr ? token_log_probs_kernel<T, U, WAVES, true, true> : token_log_probs_kernel<T, U, WAVES, false, true>)
                              : (p.entropy != nullptr ? token_log_probs_kernel<T, U, WAVES, true, false> : token_log_probs_kernel<T, U, WAVES, false, false>);
-    kernel<<<blocks, kBlock, 0, stream(device)>>>(w);
-    TP_AMD_HIP_CHECK(hipGetLastError());
+    launch_rows(kernel, w, WAVES == 1 ? kWaves : 1, device);
 }
 
 template <typename T>
@@ -600,10 +611,7 @@ void forward_typed(const TokenProbsArgs& p, int device) {
 template <typename T>
 void backward_typed(const TokenProbsArgs& p, int device) {
     const Plan w = plan_of(p, kBlock * Packet<T>::N * 4, p.vocab);
-    const unsigned blocks = grid_of(p.rows * w.splits, kBlock, "token_log_probs_backward");
-    auto* kernel = p.db != nullptr ? token_log_probs_backward_kernel<T, true> : token_log_probs_backward_kernel<T, false>;
-    kernel<<<blocks, kBlock, 0, stream(device)>>>(w);
-    TP_AMD_HIP_CHECK(hipGetLastError());
+    launch_rows(p.db != nullptr ? token_log_probs_backward_kernel<T, true> : token_log_probs_backward_kernel<T, false>, w, 1, device);
 }
 
 }  // namespace

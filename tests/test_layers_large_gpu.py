@@ -1,7 +1,8 @@
 """Dropout of more elements than 2^34: their generator's blocks have numbers
 past 32 bits.  The join's operands are one row expanded, so that only its
 result takes memory.  The join's backward and the log probabilities past 2^31
-elements."""
+elements.  More rows than one launch takes: 2^24 - 1 a block each, 2^26 - 4 a
+wave each."""
 
 import numpy as np
 import pytest
@@ -92,3 +93,24 @@ def test_log_probs(dev, ops, memory):
         assert_within(top[r: r + 1].numpy(), values, bound, F32, "alternatives")
         grad, bound = want.backward(da[r: r + 1], db[r: r + 1])
         assert_within(dx[r: r + 1].numpy(), grad, bound, BF16, "gradient")
+
+
+def test_log_probs_of_more_rows_than_a_launch_takes(dev, ops, memory):
+    vocab, rows, block = 5, (1 << 26) + 5, (1 << 24) - 1
+    x = ops.seeded_dropout(put(sample((1, vocab), BF16, 11), BF16).expand(rows, vocab), P, SEED)
+    t = np.random.default_rng(12).integers(0, vocab, rows, np.int32)
+    t[block], t[-1] = -100, vocab
+    da = np.random.default_rng(13).standard_normal(rows, np.float32)
+    lp, h, stats, top, index = ops.token_log_probs(x, put(t), top=2)
+    dx = ops.token_log_probs_backward(put(da), put(da), x, put(t), stats, h)
+    for first in (0, block - 3, 2 * block - 3, 4 * block - 3, (1 << 26) - 7, rows - 7):
+        at = slice(first, first + 7)
+        want = Probs(wide(x[at].numpy(), BF16), t[at].astype(np.int64), lanes=64)
+        given, bound = want.given()
+        assert_within(lp[at].numpy(), given, bound, F32, "logprob")
+        assert_within(h[at].numpy(), want.h, np.where(want.skipped, 0, want.h_bound), F32, "entropy")
+        order, values, bound = want.top(2)
+        assert np.array_equal(index[at].numpy(), order)
+        assert_within(top[at].numpy(), values, bound, F32, "alternatives")
+        grad, bound = want.backward(da[at], da[at])
+        assert_within(dx[at].numpy(), grad, bound, BF16, "gradient")
