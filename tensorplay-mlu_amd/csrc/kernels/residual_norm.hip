@@ -28,7 +28,7 @@ __global__ __launch_bounds__(kMaxWaves* kWave) void residual_norm_kernel(Plan w)
     const int lane = threadIdx.x % w.lanes;
     // (whole waves: a scalar, and with it the rows' addresses)
     const int team = WAVES ? __builtin_amdgcn_readfirstlane(threadIdx.x / w.lanes) : threadIdx.x / w.lanes;
-    const int64_t r0 = static_cast<int64_t>(blockIdx.x) * w.teams + team;
+    const int64_t r0 = w.first + static_cast<int64_t>(blockIdx.x) * w.teams + team;
     // a team past the last row goes through the last one again and stores nothing
     const bool there = r0 < w.p.rows;
     const int64_t r = there ? r0 : w.p.rows - 1;
@@ -161,14 +161,18 @@ void forward_typed(const ResidualNormArgs& p, int device) {
         three = many && s.unit > 1 && three_units((p.dim + s.unit - 1) / s.unit, p.drops, s.lanes);
         if (three) s.upl = 3, s.waves = false, s.teams = 256 / s.lanes;
     }
-    const Plan w = plan_of(p, s);
-    const unsigned blocks = grid_of((p.rows + s.teams - 1) / s.teams, s.threads(), "residual_norm");
+    Plan w = plan_of(p, s);
     auto* kernel = TP_AMD_RESIDUAL_KERNEL(residual_norm_kernel, T, s, p);
     if constexpr (sizeof(S_<T>) == 2) {
         if (three) kernel = TP_AMD_RESIDUAL_FORM(residual_norm_kernel, T, Packet<T>::N, 3, false, p);
     }
-    kernel<<<blocks, s.threads(), 0, stream(device)>>>(w);
-    TP_AMD_HIP_CHECK(hipGetLastError());
+    // (more rows than one launch takes go in several)
+    const int64_t at_once = most_blocks(s.threads()) * s.teams;
+    for (; w.first < p.rows; w.first += at_once) {
+        const int64_t rows = std::min(at_once, p.rows - w.first);
+        kernel<<<static_cast<unsigned>((rows + s.teams - 1) / s.teams), s.threads(), 0, stream(device)>>>(w);
+        TP_AMD_HIP_CHECK(hipGetLastError());
+    }
 }
 
 }  // namespace

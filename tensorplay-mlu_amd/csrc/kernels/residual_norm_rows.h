@@ -37,6 +37,7 @@ struct Plan {
     bool ragged;      // a thread's units hold elements of no row or of two units
     bool low;         // every generator's block has a number below 2^32
     float inv_dim;
+    int64_t first;  // forward: row of the launch
     // backward: blocks walk `groups` groups of `group_rows` rows, `per_group` blocks a group
     int64_t groups, group_rows;
     int per_group;

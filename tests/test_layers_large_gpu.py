@@ -114,3 +114,15 @@ def test_log_probs_of_more_rows_than_a_launch_takes(dev, ops, memory):
         assert_within(top[at].numpy(), values, bound, F32, "alternatives")
         grad, bound = want.backward(da[at], da[at])
         assert_within(dx[at].numpy(), grad, bound, BF16, "gradient")
+
+
+def test_norm_of_more_rows_than_a_launch_takes(dev, ops, memory):
+    """64 lanes a row: 2^26 - 4 rows a launch."""
+    width, rows, launch = 264, (1 << 26) + 5, (1 << 26) - 4
+    base = sample((1, width), BF16, 14)
+    _, h, _, r = ops.residual_norm(put(base, BF16).expand(rows, width))
+    j = Join(wide(base, BF16))
+    for first in (0, launch - 3, rows - 7):
+        at = slice(first, first + 7)
+        assert_within(h[at].numpy(), np.broadcast_to(j.h, (7, width)), j.h_bound, BF16, "normed")
+        assert_within(r[at].numpy(), np.broadcast_to(j.r2, 7), j.r2_bound, F32, "rstd")
