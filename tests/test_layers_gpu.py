@@ -581,6 +581,24 @@ def test_skipped_and_unknown_targets(dev, ops, dtype, rows, vocab):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("vocab", [1, 7, 65, 1001, 2049])
+def test_log_probs_of_many_short_rows(dev, ops, dtype, vocab):
+    """Rows enough for a wave each, the last block's not all there; some skipped,
+    some of unknown targets, some with masked tokens, NaN or nothing left."""
+    rows = 4099
+    x = wide(rows_of_logits(rows, vocab, dtype, vocab + 1), dtype)
+    t = np.random.default_rng(vocab).integers(0, vocab, rows)
+    t[3::50], t[4098], t[7::300], t[8::300] = -100, -100, vocab, -(1 << 40)
+    x[9::90, ::2] = -np.inf
+    x[11::200, vocab // 2], x[13::200], x[15::200, vocab - 1] = np.nan, -np.inf, np.inf
+    host = orc.from_float(x.astype(np.float32), dtype)
+    check_probs(ops, dtype, host, t, lanes=64)
+    check_probs(ops, dtype, host, t.astype(np.int32) if vocab == 7 else t, scale=0.7, entropy=False, back=vocab < 100, lanes=64)
+    check_probs(ops, dtype, host, t, top=min(3, vocab), back=False, lanes=64)
+    check_probs(ops, dtype, host, None, back=False, lanes=64)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("vocab", [200, 4001])
 def test_log_probs_of_views(dev, ops, dtype, vocab):
     """The last token of every sequence, rows that start at any element, a
