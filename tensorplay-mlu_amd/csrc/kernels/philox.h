@@ -2,9 +2,10 @@
 // random numbers: as easy as 1, 2, 3" (SC 2011): ten rounds of two 32 x 32
 // -> 64-bit multiplies on a 4-word counter under a 2-word key bumped by the
 // Weyl constants after each round.  Element e of a tensor takes word e % 4
-// of the block for counter (e / 4, 0, offset_lo, offset_hi) under the key
-// (seed_lo, seed_hi); its uniform is (word >> 8) * 2^-24 in [0, 1), and it is
-// kept when the uniform is >= p, decided exactly as word >> 8 >= ceil(p 2^24).
+// of the block for counter (low word of e / 4, its high word, offset_lo,
+// offset_hi) under the key (seed_lo, seed_hi); its uniform is (word >> 8) * 2^-24
+// in [0, 1), and it is kept when the uniform is >= p, decided exactly as
+// word >> 8 >= ceil(p 2^24).
 #pragma once
 
 #include <hip/hip_runtime.h>

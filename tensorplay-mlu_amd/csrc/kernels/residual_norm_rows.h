@@ -178,7 +178,6 @@ __device__ __forceinline__ void team_sums(float (&v)[K], int lanes, float (&red)
         const auto plus = [](float a, float b) { return a + b; };
 #pragma unroll
         for (int k = 0; k < K; ++k) v[k] = wave_allreduce(v[k], plus);
-        if (waves == 1) return;  // (teams of one wave share a block: the same for all)
         if (threadIdx.x % kWave == 0) {
 #pragma unroll
             for (int k = 0; k < K; ++k) red[turn][k][wave] = v[k];
