@@ -153,7 +153,10 @@ template <typename T>
 void forward_typed(const ResidualNormArgs& p, int device) {
     // Of rows that fill the device wide ones go to fewer threads, which wait for
     // each other less: bf16 8192 x 4096 with dropout 57 -> 53 us, 3400 x 8192 49 ->
-    // 44; eight rows of 4096 3.2 us by 512 threads, 3.6 by 256.
+    // 44; eight rows of 4096 3.2 us by 512 threads, 3.6 by 256.  Just past the border
+    // lanes lie idle either way: with one norm and both, 13618 x 2056 43 and 46 us (41
+    // and 51 by one packet a thread), 5600 x 5000 43 and 45 (42 and 54),
+    // float32 13618 x 1028 44 and 45 (42 and 47), 10937 x 1280 39 and 41 (38 and 41).
     const bool many = p.rows >= 2 * cu_count(device);
     Shape s = shape_of<T>(p.dim, 256, many ? 256 : kMaxWaves * kWave);
     bool three = false;

@@ -21,8 +21,10 @@
 // four elements after the other, and the sums made where their terms are
 // (left alone, the compiler moves the additions past the exchange, keeps every
 // term for them and spills).  bf16 8192 x 4096 (403 MB; an elementwise pass of
-// it 65 us): 71 us with one norm, 80 with both and a gate, 88 with dropout too,
-// and 5 us for the fold; 1700 x 16384 102 (54), float32 3003 x 1000 19 (12).
+// it 65 us): 70 us with one norm, 79 with both and a gate, 90 with dropout too,
+// and 5 us for the fold; 1700 x 16384 100 (54), float32 3003 x 1000 19 (12).  Masking
+// every product of a dropped element is 1 of the 90, and of 28 for float16 rows of
+// 768.
 
 #include "attention.h"
 #include "residual_norm_rows.h"

@@ -19,10 +19,11 @@
 // Bound by memory, with the exponentials' issue close behind for 16-bit logits;
 // waves share nothing until their ends meet, and have their next chunk's loads
 // out.  A row is split over blocks where rows are few, and its last block to
-// arrive joins the splits; many short rows go to a wave each.  bf16 4096 x 32000
-// (262 MB; 42.5 us as an elementwise pass) 48 us, backward (524 MB; 85) 87; 1024 x
-// 128000 with five alternatives 65 (54 without), 8 x 32000 with twenty 10.4,
-// 8000 x 1001 with one 13 (63 by four waves a row).
+// arrive joins the splits; many short rows go to a wave each.  Kernel times of a
+// trace: bf16 4096 x 32000 (262 MB; 42.5 us as an elementwise pass) 48 to 51 us,
+// with one alternative 54, backward (524 MB; 85) 87; 1024 x 128000 with five
+// alternatives 64 to 68 (50 without), 8 x 32000 with twenty 10.4, 8000 x 1001 with
+// one 13 (63 by four waves a row).
 
 #include <algorithm>
 
