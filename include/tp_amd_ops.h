@@ -324,9 +324,10 @@ int tp_amd_seeded_dropout_backward(const tp_amd_tensor* grad_output, double p, u
  * the norm, of the residual.  Results sum, normed (dense, the operands' dtype),
  * float32 branch_rstd and rstd [tokens...]; those not taken come back with data
  * NULL and dtype TP_AMD_UNDEFINED.  float32 arithmetic, rounded once: the norm is
- * of the sum before its rounding.  Declined for rows wider than 16384, other
- * dtypes, operands on different devices, or a gate that repeats over an axis
- * before one it has; an error from 2^30 rows on, both directions. */
+ * of the sum before its rounding; a mean square past float32's range has rstd 0.
+ * Declined for rows wider than 16384, other dtypes, operands on different
+ * devices, or a gate that repeats over an axis before one it has; an error from
+ * 2^30 rows on, both directions. */
 int tp_amd_residual_norm(const tp_amd_tensor* residual, const tp_amd_tensor* branch, const tp_amd_tensor* gate,
                          const tp_amd_tensor* branch_weight, const tp_amd_tensor* weight, double residual_scale,
                          double branch_scale, double branch_eps, double eps, double p, uint64_t seed,

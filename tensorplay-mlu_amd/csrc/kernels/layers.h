@@ -13,6 +13,8 @@ namespace tp_amd {
 
 void launch_seeded_dropout(int dtype, int64_t n, const void* x, const DropArgs& drop, void* out, int device);
 
+constexpr int64_t kMaxRows = int64_t{1} << 30;  // fewer than that, of all that follow
+
 // Rows of one tensor, the last axis dense.
 struct Rows {
     const void* data;  // null: not there

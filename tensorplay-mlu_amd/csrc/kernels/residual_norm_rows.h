@@ -240,7 +240,7 @@ inline Plan plan_of(const ResidualNormArgs& p, const Shape& s) {
 
 inline void check_extent(const ResidualNormArgs& p) {
     TP_AMD_CHECK(p.dim > 0 && p.dim <= kResidualNormMaxDim, "residual_norm: rows of ", p.dim);
-    TP_AMD_CHECK(p.rows < (int64_t{1} << 30), "residual_norm: ", p.rows, " rows");
+    TP_AMD_CHECK(p.rows < kMaxRows, "residual_norm: ", p.rows, " rows");
 }
 
 // The kernel of a form: KERNEL<T, V, UPL, WAVES, NORM, DROP, GATE> by shape,

@@ -565,7 +565,7 @@ Plan plan_of(const TokenProbsArgs& p, int64_t step, int64_t splits) {
 void check_extent(const TokenProbsArgs& p) {
     TP_AMD_CHECK(p.vocab > 0 && p.vocab < (int64_t{1} << 31), "token_log_probs: a vocabulary of ", p.vocab);
     TP_AMD_CHECK(p.top >= 0 && p.top <= kTokenProbsMaxTop && p.top <= p.vocab, "token_log_probs: ", p.top, " alternatives of ", p.vocab);
-    TP_AMD_CHECK(p.rows < (int64_t{1} << 30), "token_log_probs: ", p.rows, " rows");
+    TP_AMD_CHECK(p.rows < kMaxRows, "token_log_probs: ", p.rows, " rows");
 }
 
 // The kernel over all rows, `per_block` of them a block or `splits` blocks each:

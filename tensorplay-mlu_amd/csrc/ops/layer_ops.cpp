@@ -111,6 +111,7 @@ struct ResidualNorm {
             TP_AMD_CHECK(w->ndim == 1 && w->sizes[0] == dim, "residual_norm: a weight is one row of ", dim);
         }
         args.rows = rows_in(x);
+        TP_AMD_CHECK(args.rows < kMaxRows, "residual_norm: ", args.rows, " rows");
         args.dim = static_cast<int>(dim);
         args.norm1 = norm1;
         args.norm2 = norm2;
@@ -187,6 +188,7 @@ struct TokenProbs {
         args.rows = rows_in(x);
         args.vocab = x.sizes[x.ndim - 1];
         TP_AMD_CHECK(args.vocab > 0 || args.rows == 0, "token_log_probs: rows of no logits");
+        TP_AMD_CHECK(args.rows < kMaxRows && args.vocab < (int64_t{1} << 31), "token_log_probs: ", args.rows, " rows of ", args.vocab, " logits");
         args.ignore = ignore_index;
         if (targets != nullptr) {
             check_view(*targets, "targets");

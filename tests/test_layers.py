@@ -216,6 +216,21 @@ def test_log_probs_backward_refused(ops, change, error, message):
         ops.token_log_probs_backward(**a)
 
 
+@pytest.mark.parametrize("shape", [(1 << 30, 4), (1 << 15, 1 << 15, 4)], ids=str)
+def test_more_rows_than_are_counted(ops, shape):
+    x, row, strides = fake(shape), fake(shape[:-1], "float32"), (0,) * len(shape)
+    for call in (lambda: ops.residual_norm(x), lambda: ops.residual_norm(fake(shape, strides=strides), x),
+                 lambda: ops.residual_norm_backward(x, x, x, rstd=row), lambda: ops.token_log_probs(x, fake(shape[:-1], "int64")),
+                 lambda: ops.token_log_probs_backward(row, None, x, fake(shape[:-1], "int64"), fake(shape[:-1] + (2,), "float32"))):
+        with pytest.raises(mod("tensor").DeviceError, match=f"{1 << 30} rows"):
+            call()
+
+
+def test_more_logits_than_are_counted(ops):
+    with pytest.raises(mod("tensor").DeviceError, match="logits"):
+        ops.token_log_probs(fake((1, 1 << 31)))
+
+
 @pytest.mark.parametrize("call", ["dropout", "join", "probs"])
 def test_more_axes_than_a_tensor_has(ops, call):
     """Refused before an axis past the last one is looked at."""
