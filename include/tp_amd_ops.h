@@ -338,10 +338,11 @@ int tp_amd_residual_norm(const tp_amd_tensor* residual, const tp_amd_tensor* bra
  * the sum is the residual) with the forward's operands and statistics; a NULL
  * branch_rstd says that the branch was not normed.  output_mask (5 ints; NULL =
  * all) selects them; there is none of an operand that is NULL.  A dropped
- * element has no gradient and no part in those of gate and branch_weight,
- * whatever it holds.  Without grad_normed residual and weight are not read.
- * No token gives zero gradients of weights and of a gate that repeats over
- * tokens.  Sums in a fixed order. */
+ * element has no part in the gradients of gate and branch_weight, and none of its
+ * own but the branch norm's, whatever it, the gate and the weight hold there.
+ * Without grad_normed residual and weight are not read.  No token gives zero
+ * gradients of weights and of a gate that repeats over tokens.  Sums in a fixed
+ * order. */
 int tp_amd_residual_norm_backward(const tp_amd_tensor* grad_sum, const tp_amd_tensor* grad_normed,
                                   const tp_amd_tensor* residual, const tp_amd_tensor* branch,
                                   const tp_amd_tensor* branch_rstd, const tp_amd_tensor* rstd, const tp_amd_tensor* gate,
